@@ -39,7 +39,8 @@ enum { /* element types */
   LLMQRT_BF16 = 1,
   LLMQRT_F32 = 2,
   LLMQRT_E4M3 = 3,
-  LLMQRT_E5M2 = 4
+  LLMQRT_E5M2 = 4,
+  LLMQRT_I8 = 5
 };
 
 /* Message of the last failing call made by this thread (never NULL). */
@@ -90,6 +91,18 @@ int llmqrt_quantize_fp8_static(const void* x, int x_dtype, int64_t M, int64_t K,
 int llmqrt_quantize_fp8_alpha(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,
                               const float* static_scale, const float* weight_scale, uint8_t* q, float* alpha,
                               void* workspace, llmqrt_stream_t stream);
+
+/* FP8 e4m3 quantization with a scale for each token and group of 128 features, x's rows 16-byte aligned, K a multiple of 8:
+ * scale[m, g] = max(absmax of the group, 1e-12) / 448, q = e4m3(x * (448 / that maximum)); nothing is rounded to x's
+ * type in between.  q [M, K] and scale [M, ceil(K / 128)] are contiguous. */
+int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale,
+                              llmqrt_stream_t stream);
+
+/* RMS norm whose result leaves as llmqrt_quantize_fp8_block would have it: with h = T(x + residual), written to h_out (both
+ * or neither), or h = x,  y = h * weight / sqrt(mean(h^2) + eps) in fp32, quantized without a rounding to T.  Rows of x and
+ * residual 16-byte aligned, h_out [M, H] contiguous (it may be x or residual where their rows are contiguous), H a multiple of 8 up to 32768. */
+int llmqrt_rmsnorm_fp8_block(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* h_out, const void* weight,
+                             float eps, uint8_t* q, float* scale, int dtype, int64_t M, int64_t H, llmqrt_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * W8A8 GEMMs.   acc[m, n] = sum_k a[m, k] * w[n, k]
@@ -280,6 +293,55 @@ int llmqrt_attn_decode_step(const void* q, int64_t q_batch_stride, const void* k
                             int64_t cache_rows, const int32_t* seqlens, int32_t len_add, void* out, int dtype, int64_t B,
                             int64_t Hq, int64_t Hkv, int64_t d, int64_t max_seqlen, float softcap, void* workspace,
                             llmqrt_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * A paged key/value cache in 8 bits.  Codes [pages, Hkv, page, d] (LLMQRT_E4M3 or LLMQRT_I8; page = 16, 32, 64 or 128 tokens,
+ * d = 64 or 128; a page's rows of one head contiguous, page and head strides in elements, multiples of 16), scales
+ * fp32 [pages, Hkv] contiguous: a value is code * scale.  Request b's tokens lie in the pages that the first entries of its row
+ * of the block table name; slot = page number * page + row.  (The reference has 16-bit contiguous caches only.)
+ * ------------------------------------------------------------------------------------------ */
+
+/* Pages and slots of a step's new tokens.  Request b (of at most 8192) holds max(context[b], 0) tokens and is to get
+ * max(new_tokens[b], 0).  The pages it takes for them come from the top of the stack free_pages[0 .. free_count[0]), in the order
+ * of the requests.  A request gets nothing where its tokens end beyond max_tokens or its pages beyond the table's width, or
+ * where the stack does not hold its pages and those of the requests before it (a request that needs no page is served all
+ * the same).  Outputs:
+ *   block_table [B, width] the new pages, behind those in use;   free_left[1] the pages left (may be free_count);
+ *   seq_lens [B]           context + new tokens, or context (may be context);   cu_new [B + 1] running sum of the new tokens;
+ *   slots, positions [max_tokens]  of new token t of all requests, back to back: -1 and 0 behind the last one and for those of
+ *                          a request that gets nothing. */
+int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t* block_table, int64_t table_stride,
+                     const int32_t* free_pages, const int32_t* free_count, int32_t* free_left, int32_t* seq_lens, int32_t* cu_new,
+                     int64_t* slots, int32_t* positions, int64_t B, int64_t width, int64_t pool, int64_t page, int64_t max_tokens,
+                     llmqrt_stream_t stream);
+
+/* The pages of the requests with done[b] != 0 go back onto the stack (which has room for `pool`) and their lengths become 0. */
+int llmqrt_release_pages(const uint8_t* done, int32_t* lens, const int32_t* block_table, int64_t table_stride, int32_t* free_pages,
+                         int32_t* free_count, int64_t B, int64_t width, int64_t pool, int64_t page, llmqrt_stream_t stream);
+
+/* Keys and values of T tokens (k, v [T, Hkv, d], heads and d contiguous, strides multiples of 8) into their slots; a slot outside
+ * the cache is skipped.  With tables, keys are first rotated (half-split pairing) at row positions[t], where the tables have
+ * it.  The tokens of a page that one call writes stand next to one another in the order of their slots, without gaps: such a run
+ * and the rows ahead of it in the page get the scale max(the page's if the run is not at its start, scale(run's absmax)), the
+ * rows ahead being requantized where that grows; rows behind stay.  scale(a) = a / 127 (int8) or the least power of two not below
+ * a / 448 (e4m3), a at least 1e-12.  A call that writes two runs of one page leaves that page undefined. */
+int llmqrt_kv8_append(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int cache_type, int64_t page_stride,
+                      int64_t head_stride, const void* k, int64_t k_token_stride, const void* v, int64_t v_token_stride, int dtype,
+                      const int64_t* slots, const float* cos_table, const float* sin_table, int64_t table_rows,
+                      const int32_t* positions, int64_t T, int64_t pages, int64_t page, int64_t Hkv, int64_t d,
+                      llmqrt_stream_t stream);
+
+/* Attention of each sequence's newest Sq tokens (at most 16) over its cached tokens, themselves included: query token s sees the
+ * first seqlens[b] - Sq + 1 + s.  q [B, Sq, Hq, d] with the given strides (heads and d contiguous), out contiguous; at most
+ * 16 query heads per KV head.  With tables, q is rotated at row seqlens[b] - Sq + s first, where the tables have it.  max_seqlen
+ * bounds seqlens[b]; of a longer sequence the first max_seqlen tokens are attended to.  Table entries outside the cache and
+ * queries without a key get no weight and a row of zeros.  softcap as in llmqrt_attn_decode. */
+int llmqrt_attn_decode_kv8(const void* q, int64_t q_batch_stride, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                           int cache_type, int64_t page_stride, int64_t head_stride, const float* k_scale, const float* v_scale,
+                           const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* seqlens,
+                           const float* cos_table, const float* sin_table, int64_t table_rows, void* out, int dtype, int64_t B,
+                           int64_t Sq, int64_t Hq, int64_t Hkv, int64_t d, int64_t pages, int64_t page, int64_t max_seqlen,
+                           float softcap, void* workspace, llmqrt_stream_t stream);
 
 /* Prefill attention over the new tokens: q [B, S, Hq, d], k / v [B, S, Hkv, d], out [B, S, Hq, d],
  * token stride given in elements (heads and d contiguous), causal mask optional.

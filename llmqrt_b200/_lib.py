@@ -15,7 +15,7 @@ import torch
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libllmqrt_b200.so")
 
-F16, BF16, F32, E4M3, E5M2 = 0, 1, 2, 3, 4
+F16, BF16, F32, E4M3, E5M2, I8 = 0, 1, 2, 3, 4, 5
 _DTYPE_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32,
                torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
 
@@ -60,6 +60,13 @@ _PROTOS = {
                                           I64, I64, I64, F, P, P]),
     "llmqrt_attn_decode_step": (c_int, [P, I64, P, P, I64, P, P, I64, I32, P, P, I64, I64, I64, P, c_int32, P, I32,
                                         I64, I64, I64, I64, I64, F, P, P]),
+    "llmqrt_quantize_fp8_block": (c_int, [P, I32, I64, I64, I64, P, P, P]),
+    "llmqrt_rmsnorm_fp8_block": (c_int, [P, I64, P, I64, P, P, F, P, P, I32, I64, I64, P]),
+    "llmqrt_plan_step": (c_int, [P, P, P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P]),
+    "llmqrt_release_pages": (c_int, [P, P, P, I64, P, P, I64, I64, I64, I64, P]),
+    "llmqrt_kv8_append": (c_int, [P, P, P, P, I32, I64, I64, P, I64, P, I64, I32, P, P, P, I64, P, I64, I64, I64, I64, I64, P]),
+    "llmqrt_attn_decode_kv8": (c_int, [P, I64, I64, P, P, I32, I64, I64, P, P, P, I64, I64, P, P, P, I64, P, I32, I64, I64, I64,
+                                       I64, I64, I64, I64, I64, F, P, P]),
     "llmqrt_attn_prefill":(c_int, [P, I64, P, P, I64, P, I64, I32, I64, I64, I64, I64, I64, I32, F, P]),
     "llmqrt_rmsnorm": (c_int, [P, P, P, P, F, P, P, P, I32, I64, I64, P]),
     "llmqrt_rope_kv_write": (c_int, [P, I64, P, P, I64, P, P, I64, I64, c_int32, P, P, P, I64, I32, I64, I64, I64,

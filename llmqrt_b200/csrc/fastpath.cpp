@@ -436,6 +436,58 @@ FAST_FN(rope_kv_write) {
   FAST_END
 }
 
+// Rows [M, K] whose starts are 16-byte aligned and whose elements are contiguous; copies only if it must.
+Tensor aligned_rows(const Tensor& x) {
+  const Tensor r = rows(x);
+  const bool ok = r.stride(1) == 1 && r.stride(0) % 8 == 0 && r.stride(0) >= r.size(1) && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+constexpr int64_t kBlock = 128;                          // features of a quantization group, rows and columns of a weight's
+
+// x [..., K] -> (q e4m3 [M, K], scale fp32 [M, ceil(K / 128)])
+FAST_FN(quantize_fp8_block) {
+  FAST_BEGIN(1)
+  const Tensor x = tensor_arg(a[0], "x");
+  GilRelease gil;
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 8 == 0, "quantize_fp8_block: x must have a multiple of 8 features");
+  const int xd = dtype_code(x.scalar_type());
+  Call c(same_device({&x}));
+  const Tensor x2 = aligned_rows(x);
+  const int64_t M = x2.size(0), K = x2.size(1);
+  Tensor q = empty(x, {M, K}, at::kFloat8_e4m3fn), s = empty(x, {M, (K + kBlock - 1) / kBlock}, at::kFloat);
+  check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, x2.stride(0), static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), c.stream));
+  gil.done();
+  return wrap_tuple(q, s);
+  FAST_END
+}
+
+// (x, weight, eps, residual or None) -> (q e4m3 [M, H], scale fp32 [M, ceil(H / 128)], h or None)
+FAST_FN(rmsnorm_fp8_block) {
+  FAST_BEGIN(4)
+  const Tensor x = tensor_arg(a[0], "x"), w0 = tensor_arg(a[1], "weight"), res = tensor_arg(a[3], "residual");
+  const float eps = (float)float_arg(a[2]);
+  GilRelease gil;
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 8 == 0, "rmsnorm_fp8_block: x must have a multiple of 8 features");
+  const int64_t H = x.size(-1);
+  TORCH_CHECK(w0.defined() && w0.numel() == H, "rmsnorm_fp8_block: weight must have ", H, " elements");
+  TORCH_CHECK(!res.defined() || res.sizes() == x.sizes(), "rmsnorm_fp8_block: x and residual must have one shape");
+  TORCH_CHECK_TYPE(w0.scalar_type() == x.scalar_type() && (!res.defined() || res.scalar_type() == x.scalar_type()),
+                   "rmsnorm_fp8_block: x, weight and residual must share one dtype");
+  const int xd = dtype_code(x.scalar_type());
+  Call c(same_device({&x, &w0, &res}));
+  const Tensor x2 = aligned_rows(x), r2 = res.defined() ? aligned_rows(res) : Tensor();
+  Tensor w = w0.contiguous();
+  if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) w = w.clone();
+  const int64_t M = x2.size(0);
+  Tensor q = empty(x, {M, H}, at::kFloat8_e4m3fn), s = empty(x, {M, (H + kBlock - 1) / kBlock}, at::kFloat), h;
+  if (res.defined()) h = empty(x, x.sizes(), x.scalar_type());
+  check(llmqrt_rmsnorm_fp8_block(ptr(x2), x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0, mptr(h), ptr(w), eps,
+                                 static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), xd, M, H, c.stream));
+  gil.done();
+  return wrap_tuple(q, s, h);
+  FAST_END
+}
+
 // ---- attention -------------------------------------------------------------------------------------
 
 // [B, S, H, d] with heads and d contiguous and batches back to back; copies only if it must.
@@ -967,6 +1019,166 @@ FAST_FN(awq_block_step) {
   FAST_END
 }
 
+// ---- paged 8-bit cache -------------------------------------------------------------------------------
+
+// Caches and scales as the kernels index them; returns the codes' type.
+int check_kv8(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, const char* what) {
+  TORCH_CHECK_TYPE(kc.defined() && vc.defined() && (kc.scalar_type() == at::kChar || kc.scalar_type() == at::kFloat8_e4m3fn) &&
+                   vc.scalar_type() == kc.scalar_type(), what, ": the caches must both be int8 or both float8_e4m3fn");
+  TORCH_CHECK(kc.dim() == 4 && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc.stride(3) == 1 && kc.stride(2) == kc.size(3) &&
+              (kc.numel() == 0 || (kc.stride(1) >= kc.size(2) * kc.size(3) && kc.stride(0) >= kc.size(1) * kc.stride(1))),
+              what, ": the caches must be [pages, Hkv, page, d] with a page's rows of a head contiguous, both alike");
+  for (const Tensor* s : {&ks, &vs}) {
+    TORCH_CHECK_TYPE(s->defined() && s->scalar_type() == at::kFloat, what, ": the scales must be fp32");
+    TORCH_CHECK(s->dim() == 2 && s->size(0) == kc.size(0) && s->size(1) == kc.size(1) && s->is_contiguous(),
+                what, ": the scales must be contiguous [pages, Hkv]");
+  }
+  return kc.scalar_type() == at::kChar ? LLMQRT_I8 : LLMQRT_E4M3;
+}
+// fp32 [rows, d / 2], both or neither.
+void check_rotary(const Tensor& cos, const Tensor& sin, int64_t d, const char* what) {
+  TORCH_CHECK(cos.defined() == sin.defined(), what, ": cos and sin go together");
+  if (!cos.defined()) return;
+  TORCH_CHECK_TYPE(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, what, ": the rotary tables must be fp32");
+  TORCH_CHECK(cos.dim() == 2 && cos.size(1) == d / 2 && sin.sizes() == cos.sizes() && cos.is_contiguous() && sin.is_contiguous(),
+              what, ": the rotary tables must be contiguous [rows, d / 2]");
+}
+const Tensor& int32_vector(const Tensor& t, int64_t n, const char* name, const char* what) {
+  TORCH_CHECK_TYPE(t.defined() && t.scalar_type() == at::kInt, what, ": ", name, " must be int32");
+  TORCH_CHECK(t.dim() == 1 && (n < 0 || t.size(0) == n) && t.is_contiguous(), what, ": ", name, " must be contiguous [", n, "]");
+  return t;
+}
+const Tensor& table_arg(const Tensor& t, int64_t B, const char* what) {
+  TORCH_CHECK_TYPE(t.defined() && t.scalar_type() == at::kInt, what, ": block_table must be int32");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == B && (t.numel() == 0 || (t.stride(1) == 1 && (B <= 1 || t.stride(0) >= t.size(1)))),
+              what, ": block_table must be [", B, ", pages of a request] with contiguous rows");
+  return t;
+}
+int64_t table_stride(const Tensor& t) { return t.size(0) > 1 && t.size(1) > 0 ? t.stride(0) : t.size(1); }
+
+// (context, new_tokens, block_table, free_pages, free_count, page, max_tokens, free_left or None (in place), seq_lens or None (new)) ->
+// (seq_lens, cu_new, slots, positions)
+FAST_FN(plan_step) {
+  FAST_BEGIN(9)
+  const Tensor ctx = tensor_arg(a[0], "context_lens"), fresh = tensor_arg(a[1], "new_lens"), table = tensor_arg(a[2], "block_table");
+  const Tensor pages = tensor_arg(a[3], "free_pages"), count = tensor_arg(a[4], "free_count"), left0 = tensor_arg(a[7], "free_left");
+  Tensor seq = tensor_arg(a[8], "seq_lens");
+  const int64_t page = int_arg(a[5]), max_tokens = int_arg(a[6]);
+  GilRelease gil;
+  const Tensor& left = left0.defined() ? left0 : count;
+  const int64_t B = int32_vector(ctx, -1, "context_lens", "plan_step").size(0);
+  int32_vector(fresh, B, "new_lens", "plan_step");
+  table_arg(table, B, "plan_step");
+  int32_vector(pages, -1, "free_pages", "plan_step");
+  int32_vector(count, 1, "free_count", "plan_step");
+  int32_vector(left, 1, "free_left", "plan_step");
+  if (seq.defined()) int32_vector(seq, B, "seq_lens", "plan_step");
+  TORCH_CHECK(max_tokens >= 0, "plan_step: bad max_tokens");
+  Call c(same_device({&ctx, &fresh, &table, &pages, &count, &left, &seq}));
+  if (!seq.defined()) seq = empty(ctx, {B}, at::kInt);
+  Tensor cu = empty(ctx, {B + 1}, at::kInt), slots = empty(ctx, {max_tokens}, at::kLong);
+  Tensor positions = empty(ctx, {max_tokens}, at::kInt);
+  auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(mptr(t)); };
+  check(llmqrt_plan_step(i32(ctx), i32(fresh), i32(table), table_stride(table), i32(pages), i32(count), i32(left), i32(seq), i32(cu),
+                         static_cast<int64_t*>(mptr(slots)), i32(positions), B, table.size(1), pages.size(0), page, max_tokens, c.stream));
+  gil.done();
+  return wrap_tuple(seq, cu, slots, positions);
+  FAST_END
+}
+
+// (done bool, seq_lens, block_table, free_pages, free_count, page), in place.
+FAST_FN(release_pages) {
+  FAST_BEGIN(6)
+  const Tensor done = tensor_arg(a[0], "done"), lens = tensor_arg(a[1], "seq_lens"), table = tensor_arg(a[2], "block_table");
+  const Tensor pages = tensor_arg(a[3], "free_pages"), count = tensor_arg(a[4], "free_count");
+  const int64_t page = int_arg(a[5]);
+  GilRelease gil;
+  const int64_t B = int32_vector(lens, -1, "seq_lens", "release_pages").size(0);
+  TORCH_CHECK_TYPE(done.defined() && done.scalar_type() == at::kBool, "release_pages: done must be bool");
+  TORCH_CHECK(done.dim() == 1 && done.size(0) == B && done.is_contiguous(), "release_pages: done must be contiguous [", B, "]");
+  table_arg(table, B, "release_pages");
+  int32_vector(pages, -1, "free_pages", "release_pages");
+  int32_vector(count, 1, "free_count", "release_pages");
+  Call c(same_device({&done, &lens, &table, &pages, &count}));
+  auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(mptr(t)); };
+  check(llmqrt_release_pages(static_cast<const uint8_t*>(ptr(done)), i32(lens), i32(table), table_stride(table), i32(pages), i32(count), B,
+                             table.size(1), pages.size(0), page, c.stream));
+  gil.done();
+  Py_RETURN_NONE;
+  FAST_END
+}
+
+// (k_cache, v_cache, k_scale, v_scale, k, v, slots, cos, sin, positions), in place.
+FAST_FN(kv8_append) {
+  FAST_BEGIN(10)
+  const Tensor kc = tensor_arg(a[0], "k_cache"), vc = tensor_arg(a[1], "v_cache"), ks = tensor_arg(a[2], "k_scale"), vs = tensor_arg(a[3], "v_scale");
+  const Tensor k0 = tensor_arg(a[4], "k"), v0 = tensor_arg(a[5], "v"), slots = tensor_arg(a[6], "slots");
+  const Tensor cos = tensor_arg(a[7], "cos"), sin = tensor_arg(a[8], "sin"), positions = tensor_arg(a[9], "positions");
+  GilRelease gil;
+  const char* what = "kv8_append";
+  const int type = check_kv8(kc, vc, ks, vs, what);
+  TORCH_CHECK_TYPE(k0.defined() && v0.defined() && k0.scalar_type() == v0.scalar_type(), what, ": k and v must share one dtype");
+  const int dt = dtype_code(k0.scalar_type());
+  TORCH_CHECK(k0.dim() == 3 && v0.sizes() == k0.sizes() && k0.size(1) == kc.size(1) && k0.size(2) == kc.size(3),
+              what, ": k and v must be [T, ", kc.size(1), ", ", kc.size(3), "]");
+  const int64_t T = k0.size(0), Hkv = k0.size(1), d = k0.size(2);
+  TORCH_CHECK_TYPE(slots.defined() && slots.scalar_type() == at::kLong, what, ": slots must be int64");
+  TORCH_CHECK(slots.dim() == 1 && slots.size(0) == T && slots.is_contiguous(), what, ": slots must be contiguous [", T, "]");
+  check_rotary(cos, sin, d, what);
+  if (cos.defined()) int32_vector(positions, T, "positions", what);
+  Call c(same_device({&kc, &vc, &ks, &vs, &k0, &v0, &slots, &cos, &sin, &positions}));
+  auto usable = [&](const Tensor& t) {                   // (a slice of a fused projection's rows is)
+    return T == 0 || (t.stride(2) == 1 && t.stride(1) == d && (T == 1 || (t.stride(0) >= Hkv * d && t.stride(0) % 8 == 0)) &&
+                      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+  };
+  const Tensor k = usable(k0) ? k0 : k0.clone(at::MemoryFormat::Contiguous), v = usable(v0) ? v0 : v0.clone(at::MemoryFormat::Contiguous);
+  auto stride = [&](const Tensor& t) { return T > 1 ? t.stride(0) : Hkv * d; };
+  check(llmqrt_kv8_append(mptr(kc), mptr(vc), static_cast<float*>(mptr(ks)), static_cast<float*>(mptr(vs)), type, kc.stride(0), kc.stride(1),
+                          ptr(k), stride(k), ptr(v), stride(v), dt, static_cast<const int64_t*>(ptr(slots)),
+                          static_cast<const float*>(ptr(cos)), static_cast<const float*>(ptr(sin)), cos.defined() ? cos.size(0) : 0,
+                          static_cast<const int32_t*>(ptr(positions)), T, kc.size(0), kc.size(2), Hkv, d, c.stream));
+  gil.done();
+  Py_RETURN_NONE;
+  FAST_END
+}
+
+// (q [B, Hq, d] or [B, Sq, Hq, d], k_cache, v_cache, k_scale, v_scale, block_table, seqlens, max_seqlen, softcap, cos, sin) -> out like q
+FAST_FN(attn_decode_kv8) {
+  FAST_BEGIN(11)
+  const Tensor q0 = tensor_arg(a[0], "q"), kc = tensor_arg(a[1], "k_cache"), vc = tensor_arg(a[2], "v_cache");
+  const Tensor ks = tensor_arg(a[3], "k_scale"), vs = tensor_arg(a[4], "v_scale"), table = tensor_arg(a[5], "block_table");
+  const Tensor lens = tensor_arg(a[6], "seqlens"), cos = tensor_arg(a[9], "cos"), sin = tensor_arg(a[10], "sin");
+  const int64_t max_seqlen = int_arg(a[7]);
+  const float softcap = (float)float_arg(a[8]);
+  GilRelease gil;
+  const char* what = "attn_decode_kv8";
+  const int type = check_kv8(kc, vc, ks, vs, what);
+  TORCH_CHECK(q0.defined() && (q0.dim() == 3 || q0.dim() == 4) && q0.size(-1) == kc.size(3), what, ": q must be [B, Hq, ", kc.size(3),
+              "] or [B, Sq, Hq, ", kc.size(3), "]");
+  const int dt = dtype_code(q0.scalar_type());
+  Tensor q = q0.dim() == 3 ? q0.unsqueeze(1) : q0;
+  const int64_t B = q.size(0), Sq = q.size(1), Hq = q.size(2), d = q.size(3), Hkv = kc.size(1);
+  table_arg(table, B, what);
+  int32_vector(lens, B, "seqlens", what);
+  TORCH_CHECK(max_seqlen >= 0, what, ": bad max_seqlen");
+  check_rotary(cos, sin, d, what);
+  Call c(same_device({&q, &kc, &vc, &ks, &vs, &table, &lens, &cos, &sin}));
+  const bool usable = q.numel() == 0 ||
+                      (q.stride(3) == 1 && q.stride(2) == d && (Sq == 1 || (q.stride(1) >= Hq * d && q.stride(1) % 8 == 0)) &&
+                       (B == 1 || (q.stride(0) >= 0 && q.stride(0) % 8 == 0)) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0);
+  if (!usable) q = q.clone(at::MemoryFormat::Contiguous);
+  Tensor out = empty(q, q0.sizes(), q.scalar_type());
+  const int64_t token = Sq > 1 ? q.stride(1) : Hq * d;
+  check(llmqrt_attn_decode_kv8(ptr(q), B > 1 ? q.stride(0) : Sq * token, token, ptr(kc), ptr(vc), type, kc.stride(0), kc.stride(1),
+                               static_cast<const float*>(ptr(ks)), static_cast<const float*>(ptr(vs)), static_cast<const int32_t*>(ptr(table)),
+                               table_stride(table), table.size(1), static_cast<const int32_t*>(ptr(lens)),
+                               static_cast<const float*>(ptr(cos)), static_cast<const float*>(ptr(sin)), cos.defined() ? cos.size(0) : 0,
+                               mptr(out), dt, B, Sq, Hq, Hkv, d, kc.size(0), kc.size(2), max_seqlen, softcap, c.workspace(), c.stream));
+  gil.done();
+  return wrap(out);
+  FAST_END
+}
+
 FAST_FN(set_workspace_maker) {
   FAST_BEGIN(1)
   Py_INCREF(a[0]);
@@ -979,7 +1191,8 @@ FAST_FN(set_workspace_maker) {
 PyMethodDef methods[] = {FAST_DEF(sq_per_channel), FAST_DEF(sq_per_tensor), FAST_DEF(fp8_per_token), FAST_DEF(fp8_per_tensor),
                          FAST_DEF(awq_linear), FAST_DEF(awq_tail), FAST_DEF(rmsnorm), FAST_DEF(silu_mul), FAST_DEF(rope_kv_write),
                          FAST_DEF(attn_prefill), FAST_DEF(kv_append), FAST_DEF(attn_decode), FAST_DEF(attn_decode_step), FAST_DEF(tensor_key),
-                         FAST_DEF(set_block_classes), FAST_DEF(awq_block_step),
+                         FAST_DEF(set_block_classes), FAST_DEF(awq_block_step), FAST_DEF(quantize_fp8_block), FAST_DEF(rmsnorm_fp8_block),
+                         FAST_DEF(plan_step), FAST_DEF(release_pages), FAST_DEF(kv8_append), FAST_DEF(attn_decode_kv8),
                          FAST_DEF(set_workspace_maker), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "Native host path of llmqrt_b200.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,182 @@
+// New keys and values into a paged 8-bit cache.
+//
+// The new tokens of a page are a run: consecutive tokens of the call whose slots follow one another within the page.  For
+// each run and head, with a the run's greatest magnitude and s0 the page's scale if the page holds rows ahead of the run:
+//   s1 = max(s0, scale(a));   rows ahead: code <- code * (s0 / s1) rounded, where s1 is greater;   new: code = x / s1 rounded.
+// A page's scale thus only grows while it fills, and a page whose first row is written starts afresh.  Rows behind the run
+// stay as they were.  Keys are rotated first, if tables are given; nothing is rounded in between.
+//
+// A warp does one run of one head, of the keys or of the values: eight lanes (d = 64: four) hold a row, sixteen elements
+// each -- eight and the eight half a head away, the rotation's pairs -- so that two 16-byte loads fetch them and one
+// pass over the run finds the maximum, a second (whose reads come from L1) the codes.  No other warp touches
+// these codes or their scale, so there are no atomics and the result is the same on every run.
+//
+// A block looks for runs in a window of the call's tokens, one window for each head, keys and values; its warps take the runs
+// in turn.  Windows are short where the call is small: a decode step's tokens are runs of their own, each wants a warp.
+#include "kv8.cuh"
+
+namespace llmqrt {
+namespace {
+
+constexpr int kWarps = 4;
+
+struct AppendArgs {
+  uint8_t* cache[2];               // keys, values: [pages, Hkv, page, d]
+  float* scale[2];                 // [pages, Hkv]
+  const void* fresh[2];            // [T, Hkv, d], heads and d contiguous
+  int64_t token_stride[2];
+  int64_t page_stride, head_stride;
+  const int64_t* slots;            // [T]
+  const float* cos_tab;            // [table_rows, d / 2] or null
+  const float* sin_tab;
+  const int32_t* positions;        // [T]
+  int64_t num_slots;               // pages * page
+  int T, Hkv, page, table_rows, window;
+};
+
+template <typename T, int D, bool INT8>
+__global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes;  // lanes of a row, rows a warp takes at once
+  pdl_wait_then_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, kind = blockIdx.z;
+  const int piece = lane % kLanes, sub = lane / kLanes;
+  const int w0 = blockIdx.x * p.window, w1 = min(p.T, w0 + p.window);
+  const int shift = __ffs(p.page) - 1;
+  // the runs that begin in the window: one bit a token (a window has at most 32)
+  bool begins = false;
+  if (w0 + lane < w1) {
+    const int64_t s = p.slots[w0 + lane], before = w0 + lane > 0 ? p.slots[w0 + lane - 1] : -2;
+    begins = s >= 0 && s < p.num_slots && !(before + 1 == s && (s & (p.page - 1)) != 0);
+  }
+  unsigned runs = __ballot_sync(0xffffffffu, begins);
+  for (int nth = 0; runs; runs &= runs - 1, ++nth) {
+    if (nth % kWarps != warp) continue;
+    const int t0 = w0 + __ffs(runs) - 1;
+    const int64_t s0 = p.slots[t0];
+    const int row0 = (int)(s0 & (p.page - 1));
+    // length of the run: to the end of the page, or as far as the slots follow one another
+    int n = 1;
+    while (n < p.page - row0) {
+      const int i = n + lane;
+      const bool on = i < p.page - row0 && t0 + i < p.T && p.slots[t0 + i] == s0 + i;
+      const unsigned gap = ~__ballot_sync(0xffffffffu, on);
+      n += gap ? __ffs(gap) - 1 : 32;
+      if (gap) break;
+    }
+    const int64_t page = s0 >> shift;
+    uint8_t* tile = p.cache[kind] + page * p.page_stride + (int64_t)head * p.head_stride;
+    float* scale = p.scale[kind] + page * p.Hkv + head;
+    const bool rotated = kind == 0 && p.cos_tab != nullptr;
+    auto fetch = [&](int i, float (&x)[16]) {
+      const T* src = static_cast<const T*>(p.fresh[kind]) + (int64_t)(t0 + i) * p.token_stride[kind] + head * D + piece * 8;
+      const uint4 lo = *reinterpret_cast<const uint4*>(src), hi = *reinterpret_cast<const uint4*>(src + D / 2);
+      const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack_pair<T>(a[j]), g = unpack_pair<T>(b[j]);
+        x[2 * j] = f.x; x[2 * j + 1] = f.y;
+        x[8 + 2 * j] = g.x; x[8 + 2 * j + 1] = g.y;
+      }
+      if (rotated) {
+        const int at = p.positions[t0 + i];
+        if (at >= 0 && at < p.table_rows) {            // (outside the table: not rotated)
+          const float* cr = p.cos_tab + (int64_t)at * (D / 2) + piece * 8;
+          const float* sr = p.sin_tab + (int64_t)at * (D / 2) + piece * 8;
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(cr + j), s = *reinterpret_cast<const float4*>(sr + j);
+            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {              // (two products and their sum, each rounded: no contraction)
+              const float u = x[j + e], v = x[8 + j + e];
+              x[j + e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(v, sn[e]));
+              x[8 + j + e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(v, cs[e]));
+            }
+          }
+        }
+      }
+    };
+    float top = 0.f;
+    for (int i = sub; i < n; i += kRows) {
+      float x[16];
+      fetch(i, x);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[j]));
+    }
+    top = warp_max(top);
+    const float was = row0 > 0 ? *scale : 0.f;
+    const float now = fmaxf(was, kv8_scale<INT8>(top)), inv = __fdiv_rn(1.f, now);
+    // lane `piece` of a row holds elements 8 piece .. + 7 and D / 2 further: two 8-byte stores
+    for (int i = sub; i < n; i += kRows) {
+      float x[16];
+      fetch(i, x);
+      const uint4 c = kv8_encode<INT8>(x, inv);
+      uint8_t* dst = tile + (int64_t)(row0 + i) * D + piece * 8;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(c.x, c.y);
+      *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(c.z, c.w);
+    }
+    if (now != was) {
+      if (row0 > 0) {
+        const float ratio = __fdiv_rn(was, now);
+        for (int i = sub; i < row0; i += kRows) {
+          uint8_t* at = tile + (int64_t)i * D + piece * 16;
+          float x[16];
+          kv8_decode<INT8>(*reinterpret_cast<const uint4*>(at), x);
+          *reinterpret_cast<uint4*>(at) = kv8_encode<INT8>(x, ratio);
+        }
+      }
+      __syncwarp();                                    // (every lane has read the old scale)
+      if (lane == 0) *scale = now;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace llmqrt
+
+using namespace llmqrt;
+
+extern "C" int llmqrt_kv8_append(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int cache_type, int64_t page_stride,
+                                 int64_t head_stride, const void* k, int64_t k_token_stride, const void* v, int64_t v_token_stride,
+                                 int dtype, const int64_t* slots, const float* cos_table, const float* sin_table, int64_t table_rows,
+                                 const int32_t* positions, int64_t T, int64_t pages, int64_t page, int64_t Hkv, int64_t d,
+                                 llmqrt_stream_t stream) {
+  LLMQRT_REQUIRE(dtype == LLMQRT_F16 || dtype == LLMQRT_BF16, "kv8_append: dtype must be fp16 or bf16");
+  LLMQRT_REQUIRE(cache_type == LLMQRT_E4M3 || cache_type == LLMQRT_I8, "kv8_append: the cache holds e4m3 or int8");
+  LLMQRT_REQUIRE(d == 64 || d == 128, "kv8_append: head_dim must be 64 or 128 (got %lld)", (long long)d);
+  LLMQRT_REQUIRE(page >= 16 && page <= 128 && (page & (page - 1)) == 0, "kv8_append: pages hold 16, 32, 64 or 128 tokens (got %lld)",
+                 (long long)page);
+  LLMQRT_REQUIRE(T >= 0 && T <= 0x7fffff00ll && Hkv > 0 && Hkv < 65536 && pages >= 0 && pages <= 0x7fffffffll, "kv8_append: bad shape");
+  LLMQRT_REQUIRE(head_stride >= page * d && page_stride >= Hkv * head_stride && head_stride % 16 == 0 && page_stride % 16 == 0,
+                 "kv8_append: the cache is [pages, Hkv, page, d] with contiguous pages, strides multiples of 16");
+  LLMQRT_REQUIRE((cos_table == nullptr) == (sin_table == nullptr) && (!cos_table || positions || T == 0),
+                 "kv8_append: cos, sin and positions go together");
+  if (T == 0 || pages == 0) return LLMQRT_OK;
+  LLMQRT_REQUIRE(k_cache && v_cache && k_scale && v_scale && k && v && slots, "kv8_append: null pointer");
+  LLMQRT_REQUIRE(k_token_stride >= Hkv * d && v_token_stride >= Hkv * d && k_token_stride % 8 == 0 && v_token_stride % 8 == 0 &&
+                 ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_cache) |
+                   reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0, "kv8_append: rows and caches must be 16-byte aligned");
+  LLMQRT_REQUIRE(!cos_table || (table_rows > 0 && table_rows <= 0x7fffffffll &&
+                                ((reinterpret_cast<uintptr_t>(cos_table) | reinterpret_cast<uintptr_t>(sin_table)) & 15) == 0),
+                 "kv8_append: rotary tables must be 16-byte aligned fp32 [table_rows, d/2]");
+  AppendArgs a{};
+  a.cache[0] = static_cast<uint8_t*>(k_cache); a.cache[1] = static_cast<uint8_t*>(v_cache);
+  a.scale[0] = k_scale; a.scale[1] = v_scale;
+  a.fresh[0] = k; a.fresh[1] = v;
+  a.token_stride[0] = k_token_stride; a.token_stride[1] = v_token_stride;
+  a.page_stride = page_stride; a.head_stride = head_stride;
+  a.slots = slots; a.cos_tab = cos_table; a.sin_tab = sin_table; a.positions = positions;
+  a.num_slots = pages * page;
+  a.T = (int)T; a.Hkv = (int)Hkv; a.page = (int)page; a.table_rows = (int)table_rows;
+  a.window = T <= 2048 ? kWarps : 32;
+  const dim3 grid((unsigned)ceil_div(T, a.window), (unsigned)Hkv, 2);
+  auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
+  const bool i8 = cache_type == LLMQRT_I8;
+  auto pick = [&](auto tag) {
+    using T_ = decltype(tag);
+    return d == 128 ? (i8 ? go(kv8_append_kernel<T_, 128, true>) : go(kv8_append_kernel<T_, 128, false>))
+                    : (i8 ? go(kv8_append_kernel<T_, 64, true>) : go(kv8_append_kernel<T_, 64, false>));
+  };
+  if (int rc = dtype == LLMQRT_F16 ? pick(__half()) : pick(__nv_bfloat16())) return rc;
+  return check_launch("kv8_append");
+}

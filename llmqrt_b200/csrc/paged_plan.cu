@@ -1,0 +1,215 @@
+// Pages and slots of a serving step, from the requests' lengths, on the GPU.
+//
+// Request b holds context[b] tokens in ceil(context[b] / page) pages, named by the first entries of its row of the block
+// table, and is to get new[b] more.  The pages that this takes come from the top of a stack of free page numbers, in the
+// order of the requests; then every new token has a slot, page number * page + row, and a position.
+//
+// Latency-bound (a step of 64 requests touches 3 KB): one launch of at most eight blocks, a cluster.  Each of them adds up
+// all requests for itself -- two scans, the second over what the first lets through -- and keeps the sums in shared memory;
+// tokens and table rows are then dealt out, a token finding its request by bisection.  The stack's count and the lengths
+// may be updated in place: nothing is written before every block of the cluster has read them.
+#include "common.cuh"
+
+namespace llmqrt {
+namespace {
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanMaxRequests = 8192;                 // three words each in shared memory
+
+struct PlanArgs {
+  const int32_t* context;          // [B]
+  const int32_t* fresh;            // [B] new tokens
+  int32_t* table;                  // [B, width] with row stride table_stride
+  int64_t table_stride;
+  const int32_t* free_pages;       // [pool]
+  const int32_t* free_count;       // [1]
+  int32_t* free_left;              // [1], may be free_count
+  int32_t* seq;                    // [B], may be context
+  int32_t* cu;                     // [B + 1]
+  int64_t* slots;                  // [max_tokens]
+  int32_t* positions;              // [max_tokens]
+  int B, width, pool, page, max_tokens;
+};
+
+// Exclusive sum over the block's threads in thread order; the total comes back in `total`.
+__device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_sums, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t n = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += n;
+  }
+  if (lane == 31) warp_sums[warp] = s;
+  __syncthreads();
+  int64_t w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t n = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += n;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  __syncthreads();                                     // (the words may be used again)
+  return s - v + (warp > 0 ? before : 0);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(PlanArgs p) {
+  extern __shared__ int32_t plan_smem[];
+  __shared__ int64_t warp_sums[kPlanThreads / 32];
+  int32_t* cu_s = plan_smem;                           // [B] first token of the request
+  int32_t* ctx_s = cu_s + p.B;                         // [B] its context
+  int32_t* off_s = ctx_s + p.B;                        // [B] its first page's place below the stack's top; -1: it gets nothing
+  const int cl = gridDim.x, rank = blockIdx.x;
+  pdl_wait_then_trigger();
+  const int64_t count = min(max(*p.free_count, 0), p.pool);
+  int64_t tokens = 0, wanted = 0, taken = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool in = b < p.B;
+    const int64_t ctx = in ? max(p.context[b], 0) : 0, n = in ? max(p.fresh[b], 0) : 0;
+    const int64_t have = (ctx + p.page - 1) / p.page, all = (ctx + n + p.page - 1) / p.page;
+    int64_t sum;
+    const int64_t cu = tokens + block_exclusive_sum(n, warp_sums, sum);
+    tokens += sum;
+    bool fits = cu + n <= p.max_tokens && all <= p.width;
+    const int64_t need = fits ? all - have : 0;
+    const int64_t off = wanted + block_exclusive_sum(need, warp_sums, sum);
+    wanted += sum;
+    fits = fits && (need == 0 || off + need <= count);
+    // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
+    block_exclusive_sum(fits ? need : 0, warp_sums, sum);
+    taken += sum;
+    if (in) {
+      cu_s[b] = (int32_t)min(cu, (int64_t)0x7fffffff);
+      ctx_s[b] = (int32_t)ctx;
+      off_s[b] = !fits ? -1 : need ? (int32_t)off : 0;
+    }
+  }
+  __syncthreads();
+  if (cl > 1) {                                        // every block has read the lengths and the count
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (rank == 0) {
+    for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+      const int32_t next = b + 1 < p.B ? cu_s[b + 1] : (int32_t)min(tokens, (int64_t)0x7fffffff);
+      p.cu[b + 1] = next;
+      p.seq[b] = ctx_s[b] + (off_s[b] >= 0 ? next - cu_s[b] : 0);
+    }
+    if (threadIdx.x == 0) {
+      p.cu[0] = 0;
+      *p.free_left = (int32_t)(count - taken);
+    }
+  }
+  const int lane = threadIdx.x & 31, warps = cl * (kPlanThreads / 32);
+  for (int b = rank * (kPlanThreads / 32) + (threadIdx.x >> 5); b < p.B; b += warps) {
+    const int off = off_s[b];
+    if (off < 0) continue;
+    const int n = (b + 1 < p.B ? cu_s[b + 1] : (int)tokens) - cu_s[b];
+    const int have = (int)(((int64_t)ctx_s[b] + p.page - 1) / p.page), all = (int)(((int64_t)ctx_s[b] + n + p.page - 1) / p.page);
+    for (int j = lane; j < all - have; j += 32) p.table[(int64_t)b * p.table_stride + have + j] = p.free_pages[count - 1 - off - j];
+  }
+  const int shift = __ffs(p.page) - 1;
+  for (int64_t t = rank * kPlanThreads + threadIdx.x; t < p.max_tokens; t += cl * kPlanThreads) {
+    int64_t slot = -1;
+    int32_t position = 0;
+    if (t < tokens) {
+      int lo = 0, hi = p.B;                            // the last request whose first token is at most t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cu_s[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int off = off_s[lo];
+      if (off >= 0) {
+        position = ctx_s[lo] + (int32_t)(t - cu_s[lo]);
+        const int have = (int)(((int64_t)ctx_s[lo] + p.page - 1) >> shift), j = position >> shift;
+        // (a page taken in this step is read from the stack: another block may write the table's entry)
+        const int id = j < have ? p.table[(int64_t)lo * p.table_stride + j] : p.free_pages[count - 1 - off - (j - have)];
+        if (id >= 0) slot = ((int64_t)id << shift) + (position & (p.page - 1));
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = position;
+  }
+}
+
+// Pages of the requests that `done` marks go back onto the stack, in the order of the requests and of their rows, and
+// their lengths become zero.  One block: a step releases a few requests.
+__global__ void __launch_bounds__(kPlanThreads)
+release_kernel(const uint8_t* __restrict__ done, int32_t* __restrict__ lens, const int32_t* __restrict__ table,
+               int64_t table_stride, int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count, int B, int width, int pool,
+               int page) {
+  __shared__ int64_t warp_sums[kPlanThreads / 32];
+  __shared__ int32_t first[kPlanThreads];
+  __shared__ int32_t pages[kPlanThreads];
+  pdl_wait_then_trigger();
+  int64_t count = min(max(*free_count, 0), pool);
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool go = b < B && done[b] != 0;
+    const int64_t n = go ? min(((int64_t)max(lens[b], 0) + page - 1) / page, (int64_t)width) : 0;
+    int64_t sum;
+    const int64_t at = count + block_exclusive_sum(n, warp_sums, sum);
+    first[threadIdx.x] = (int32_t)min(at, (int64_t)pool);
+    pages[threadIdx.x] = (int32_t)n;
+    if (go) lens[b] = 0;
+    count = min(count + sum, (int64_t)pool);
+    __syncthreads();
+    for (int r = threadIdx.x >> 5; r < min(kPlanThreads, B - b0); r += kPlanThreads / 32)
+      for (int j = threadIdx.x & 31; j < pages[r]; j += 32)
+        if (first[r] + j < pool) free_pages[first[r] + j] = table[(int64_t)(b0 + r) * table_stride + j];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *free_count = (int32_t)count;
+}
+
+int check_table(const char* what, const void* table, int64_t table_stride, const void* free_pages, const void* free_count, int64_t B,
+                int64_t width, int64_t pool, int64_t page) {
+  LLMQRT_REQUIRE(page >= 16 && page <= 128 && (page & (page - 1)) == 0, "%s: pages hold 16, 32, 64 or 128 tokens (got %lld)", what,
+                 (long long)page);
+  LLMQRT_REQUIRE(B >= 0 && B <= kPlanMaxRequests, "%s: at most %d requests (got %lld)", what, kPlanMaxRequests, (long long)B);
+  LLMQRT_REQUIRE(width >= 0 && pool >= 0 && width * page <= 0x7fffffffll && pool <= 0x7fffffffll && table_stride >= width,
+                 "%s: bad table or pool", what);
+  LLMQRT_REQUIRE(free_count && (free_pages || pool == 0) && (table || B == 0 || width == 0), "%s: null pointer", what);
+  return LLMQRT_OK;
+}
+
+}  // namespace
+}  // namespace llmqrt
+
+using namespace llmqrt;
+
+extern "C" {
+
+int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t* block_table, int64_t table_stride,
+                     const int32_t* free_pages, const int32_t* free_count, int32_t* free_left, int32_t* seq_lens, int32_t* cu_new,
+                     int64_t* slots, int32_t* positions, int64_t B, int64_t width, int64_t pool, int64_t page, int64_t max_tokens,
+                     llmqrt_stream_t stream) {
+  if (int rc = check_table("plan_step", block_table, table_stride, free_pages, free_count, B, width, pool, page)) return rc;
+  LLMQRT_REQUIRE(max_tokens >= 0 && max_tokens < 0x7fffffffll, "plan_step: bad max_tokens");
+  LLMQRT_REQUIRE(free_left && cu_new && (B == 0 || (context && new_tokens && seq_lens)) && (max_tokens == 0 || (slots && positions)),
+                 "plan_step: null pointer");
+  const int cluster = max_tokens > 16384 ? 8 : max_tokens > 2048 || B > 256 ? 4 : 1;
+  PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
+             (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
+  const int smem = (int)(3 * 4 * B);
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(plan_step_kernel), smem)) return rc;
+  if (int rc = launch_chained(plan_step_kernel, dim3((unsigned)cluster), dim3(kPlanThreads), (size_t)smem, (cudaStream_t)stream, cluster, p))
+    return rc;
+  return check_launch("plan_step");
+}
+
+int llmqrt_release_pages(const uint8_t* done, int32_t* lens, const int32_t* block_table, int64_t table_stride, int32_t* free_pages,
+                         int32_t* free_count, int64_t B, int64_t width, int64_t pool, int64_t page, llmqrt_stream_t stream) {
+  if (int rc = check_table("release_pages", block_table, table_stride, free_pages, free_count, B, width, pool, page)) return rc;
+  if (B == 0) return LLMQRT_OK;
+  LLMQRT_REQUIRE(done && lens, "release_pages: null pointer");
+  if (int rc = launch_chained(release_kernel, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, 1, done, lens, block_table,
+                              table_stride, free_pages, free_count, (int)B, (int)width, (int)pool, (int)page))
+    return rc;
+  return check_launch("release_pages");
+}
+
+}  // extern "C"

@@ -53,6 +53,14 @@ def rmsnorm(x, weight, eps: float, residual=None, quantize: bool = False, want_y
     return (y.reshape(shape) if y is not None else None, h.reshape(shape), q, s)
 
 
+def rmsnorm_fp8_block(x, weight, eps: float, residual=None):
+    """RMS norm over the last dimension whose result leaves in e4m3 with a scale for each token and 128 features, the input of
+    ops.fp8_linear_block.  With a residual, h = x + residual (rounded to x's type) is normalised and returned as well.
+    y = h * weight / sqrt(mean(h^2) + eps) stays in fp32 until it is quantized (glue.rmsnorm rounds it to x's type, twice).
+    Returns (q [M, H], scale [M, ceil(H / 128)], h or None); H a multiple of 8, at most 32768."""
+    return L.fast.rmsnorm_fp8_block(x, weight, eps, residual)
+
+
 def rope_tables(head_dim: int, max_seq_len: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
     """cos / sin of pos * theta**(-2i/d), fp32 [max_seq_len, d/2], built on the CPU exactly like the
     reference's freqs_cis table (runtime/nn_models/modules/nonlinear/attn.py:37-43) and then moved."""

@@ -63,6 +63,12 @@ def quantize_fp8_static(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     return q
 
 
+def quantize_fp8_block(x: torch.Tensor):
+    """A scale for each token and group of 128 features (the last group may be shorter): returns (q e4m3 [M, K], scale fp32
+    [M, ceil(K / 128)]), scale = max(absmax, 1e-12) / 448 and q = e4m3(x / scale) without a rounding to x's type in between."""
+    return L.fast.quantize_fp8_block(x)
+
+
 # ---------------------------------------------------------------------------------------------
 # W8A8 GEMMs.  `w` is always the [N, K] row-major weight.
 #
