@@ -171,6 +171,14 @@ int llmqrt_f8f8bf16_rowwise(const uint8_t* a, int a_format, int64_t lda, const u
                             const void* bias, int bias_dtype, const float* x_scale, const float* w_scale, void* out,
                             int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace, llmqrt_stream_t stream, int flags);
 
+/* FP8 e4m3 GEMM with a scale for each block of 128: out[m, n] = T( sum over groups g of 128 inputs of
+ * (sum_{k in g} a[m, k] w[n, k]) * (a_scale[m, g] * w_scale[n / 128, g]) + bias[n] ), T fp16 or bf16, sums in fp32.  a_scale
+ * [M, ceil(K / 128)] (llmqrt_quantize_fp8_block, llmqrt_rmsnorm_fp8_block) and w_scale [ceil(N / 128), ceil(K / 128)] are
+ * contiguous, bias optional.  (The reference scales per tensor or per row only.) */
+int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint8_t* w, int64_t ldw, const void* bias, int bias_dtype,
+                            const float* a_scale, const float* w_scale, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
+                            int64_t K, void* workspace, llmqrt_stream_t stream, int flags);
+
 /* Per-token quantization and per-token x per-channel GEMM of a few tokens in one kernel, the same bits as
  * llmqrt_quantize_int8 / _fp8 followed by llmqrt_w8a8_int8_linear_per_channel / llmqrt_f8f8bf16_rowwise.
  * llmqrt_w8a8_dynamic_fits says whether it takes the sizes; x (fp16 / bf16) has 16-byte aligned rows. */

@@ -314,6 +314,80 @@ FAST_FN(fp8_per_tensor) {
   FAST_END
 }
 
+constexpr int64_t kBlock = 128;                          // features of a quantization group, rows and columns of a weight's
+
+// Rows [M, K] whose starts are 16-byte aligned and whose elements are contiguous; copies only if it must.
+Tensor aligned_rows(const Tensor& x) {
+  const int64_t per16 = 16 / x.element_size();
+  const Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+  const bool ok = r.stride(1) == 1 && (r.size(0) <= 1 || (r.stride(0) % per16 == 0 && r.stride(0) >= r.size(1))) &&
+                  reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_stride(const Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
+
+// A weight e4m3 [N, K] and its scales fp32 [ceil(N / 128), ceil(K / 128)], as the block-scaled GEMM reads them.
+void check_block_weight(const Tensor& w, const Tensor& ws, const Tensor& bias, int64_t K) {
+  TORCH_CHECK_TYPE(w.defined() && w.scalar_type() == at::kFloat8_e4m3fn, "fp8 block linear: the weight must be float8_e4m3fn");
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == K && w.size(0) > 0 && w.stride(1) == 1, "fp8 block linear: the weight must be [N, ", K, "] with contiguous rows");
+  TORCH_CHECK_TYPE(ws.defined() && ws.scalar_type() == at::kFloat, "fp8 block linear: the scales must be fp32");
+  TORCH_CHECK(ws.dim() == 2 && ws.size(0) == (w.size(0) + kBlock - 1) / kBlock && ws.size(1) == (K + kBlock - 1) / kBlock && ws.is_contiguous(),
+              "fp8 block linear: the weight's scales must be contiguous [ceil(N / 128), ceil(K / 128)]");
+  TORCH_CHECK(!bias.defined() || (bias.numel() == w.size(0) && bias.is_contiguous()), "fp8 block linear: bias must be contiguous [N]");
+}
+
+// (a e4m3 [M, K], w e4m3 [N, K], bias or None, a_scale [M, ceil(K / 128)], w_scale [ceil(N / 128), ceil(K / 128)], out dtype, static weight) ->
+// out [M, N]
+FAST_FN(fp8_linear_block) {
+  FAST_BEGIN(7)
+  const Tensor x = tensor_arg(a[0], "a"), w = tensor_arg(a[1], "w"), bias = tensor_arg(a[2], "bias"), as = tensor_arg(a[3], "a_scale");
+  const Tensor ws = tensor_arg(a[4], "w_scale");
+  TORCH_CHECK_TYPE(THPDtype_Check(a[5]), "llmqrt_b200: the result's dtype must be a torch.dtype");
+  const at::ScalarType od = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+  const int flags = bool_arg(a[6]) ? LLMQRT_GEMM_STATIC_WEIGHT : 0;
+  GilRelease gil;
+  TORCH_CHECK_TYPE(x.defined() && x.scalar_type() == at::kFloat8_e4m3fn, "fp8 block linear: a must be float8_e4m3fn");
+  TORCH_CHECK(x.dim() == 2, "fp8 block linear: a must be [M, K]");
+  const int64_t M = x.size(0), K = x.size(1);
+  check_block_weight(w, ws, bias, K);
+  TORCH_CHECK_TYPE(as.defined() && as.scalar_type() == at::kFloat, "fp8 block linear: the scales must be fp32");
+  TORCH_CHECK(as.dim() == 2 && as.size(0) == M && as.size(1) == (K + kBlock - 1) / kBlock && as.is_contiguous(),
+              "fp8 block linear: a's scales must be contiguous [M, ceil(K / 128)]");
+  const int dt = dtype_code(od), bd = bias.defined() ? dtype_code(bias.scalar_type()) : LLMQRT_F16;
+  Call c(same_device({&x, &w, &bias, &as, &ws}));
+  const Tensor x2 = aligned_rows(x), w2 = aligned_rows(w);
+  const int64_t N = w.size(0);
+  Tensor out = empty(x, {M, N}, od);
+  check(llmqrt_fp8_linear_block(static_cast<const uint8_t*>(ptr(x2)), row_stride(x2), static_cast<const uint8_t*>(ptr(w2)), row_stride(w2), ptr(bias), bd,
+                                static_cast<const float*>(ptr(as)), static_cast<const float*>(ptr(ws)), mptr(out), dt, N, M, N, K, c.workspace(),
+                                c.stream, w2.data_ptr() == w.data_ptr() ? flags : 0));
+  gil.done();
+  return wrap(out);
+  FAST_END
+}
+
+// (x [..., K], weight e4m3, bias or None, weight_scale) -> y [..., N] in x's dtype: quantized per token and 128 features, then the same.
+FAST_FN(fp8_block) {
+  FAST_BEGIN(4)
+  const Tensor x = tensor_arg(a[0], "x"), w = tensor_arg(a[1], "weight"), bias = tensor_arg(a[2], "bias"), ws = tensor_arg(a[3], "weight_scale");
+  GilRelease gil;
+  TORCH_CHECK(x.defined() && x.dim() >= 1 && x.size(-1) > 0, "fp8 block linear: x must be [..., K]");
+  const int64_t K = x.size(-1), groups = (K + kBlock - 1) / kBlock;
+  check_block_weight(w, ws, bias, K);
+  const int xd = dtype_code(x.scalar_type()), bd = bias.defined() ? dtype_code(bias.scalar_type()) : LLMQRT_F16;
+  Call c(same_device({&x, &w, &bias, &ws}));
+  const Tensor x2 = aligned_rows(x), w2 = aligned_rows(w);
+  const int64_t M = x2.size(0), N = w.size(0);
+  Tensor out = empty(x, out_shape(x, N), x.scalar_type());
+  QuantScratch s(x, M, K, M * groups);
+  check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, row_stride(x2), s.q, s.scale, c.stream));
+  check(llmqrt_fp8_linear_block(s.q, K, static_cast<const uint8_t*>(ptr(w2)), row_stride(w2), ptr(bias), bd, s.scale, static_cast<const float*>(ptr(ws)),
+                                mptr(out), xd, N, M, N, K, c.workspace(), c.stream, w2.data_ptr() == w.data_ptr() ? LLMQRT_GEMM_STATIC_WEIGHT : 0));
+  gil.done();
+  return wrap(out);
+  FAST_END
+}
+
 // (x fp16, wq_t, sz_t, bias or None, K, N, G) -> y fp16 [..., N].
 FAST_FN(awq_linear) {
   FAST_BEGIN(7)
@@ -436,14 +510,6 @@ FAST_FN(rope_kv_write) {
   FAST_END
 }
 
-// Rows [M, K] whose starts are 16-byte aligned and whose elements are contiguous; copies only if it must.
-Tensor aligned_rows(const Tensor& x) {
-  const Tensor r = rows(x);
-  const bool ok = r.stride(1) == 1 && r.stride(0) % 8 == 0 && r.stride(0) >= r.size(1) && reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
-  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
-}
-constexpr int64_t kBlock = 128;                          // features of a quantization group, rows and columns of a weight's
-
 // x [..., K] -> (q e4m3 [M, K], scale fp32 [M, ceil(K / 128)])
 FAST_FN(quantize_fp8_block) {
   FAST_BEGIN(1)
@@ -455,7 +521,7 @@ FAST_FN(quantize_fp8_block) {
   const Tensor x2 = aligned_rows(x);
   const int64_t M = x2.size(0), K = x2.size(1);
   Tensor q = empty(x, {M, K}, at::kFloat8_e4m3fn), s = empty(x, {M, (K + kBlock - 1) / kBlock}, at::kFloat);
-  check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, x2.stride(0), static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), c.stream));
+  check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, row_stride(x2), static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), c.stream));
   gil.done();
   return wrap_tuple(q, s);
   FAST_END
@@ -481,7 +547,7 @@ FAST_FN(rmsnorm_fp8_block) {
   const int64_t M = x2.size(0);
   Tensor q = empty(x, {M, H}, at::kFloat8_e4m3fn), s = empty(x, {M, (H + kBlock - 1) / kBlock}, at::kFloat), h;
   if (res.defined()) h = empty(x, x.sizes(), x.scalar_type());
-  check(llmqrt_rmsnorm_fp8_block(ptr(x2), x2.stride(0), ptr(r2), r2.defined() ? r2.stride(0) : 0, mptr(h), ptr(w), eps,
+  check(llmqrt_rmsnorm_fp8_block(ptr(x2), row_stride(x2), ptr(r2), r2.defined() ? row_stride(r2) : 0, mptr(h), ptr(w), eps,
                                  static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), xd, M, H, c.stream));
   gil.done();
   return wrap_tuple(q, s, h);
@@ -1192,6 +1258,7 @@ PyMethodDef methods[] = {FAST_DEF(sq_per_channel), FAST_DEF(sq_per_tensor), FAST
                          FAST_DEF(awq_linear), FAST_DEF(awq_tail), FAST_DEF(rmsnorm), FAST_DEF(silu_mul), FAST_DEF(rope_kv_write),
                          FAST_DEF(attn_prefill), FAST_DEF(kv_append), FAST_DEF(attn_decode), FAST_DEF(attn_decode_step), FAST_DEF(tensor_key),
                          FAST_DEF(set_block_classes), FAST_DEF(awq_block_step), FAST_DEF(quantize_fp8_block), FAST_DEF(rmsnorm_fp8_block),
+                         FAST_DEF(fp8_linear_block), FAST_DEF(fp8_block),
                          FAST_DEF(plan_step), FAST_DEF(release_pages), FAST_DEF(kv8_append), FAST_DEF(attn_decode_kv8),
                          FAST_DEF(set_workspace_maker), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", "Native host path of llmqrt_b200.", -1, methods,

@@ -1,0 +1,664 @@
+// FP8 GEMM with a scale for each block of 128: activations a[M, K] with a scale for each token and 128 inputs, weights w[N, K] with
+// one for each 128 outputs x 128 inputs,
+//   out[m, n] = T( sum_g ( sum_{k in g} a[m, k] w[n, k] ) * (a_scale[m, g] * w_scale[n / 128, g]) + bias[n] ).
+//
+// A block of 128 inputs is one K block of the tensor cores (128 bytes, four MMAs), and its products have to be scaled before they are
+// added up: the accumulator in tensor memory holds ONE K block's sums, and the epilogue warps take it over block by
+// block, tcgen05.ld, one multiply-add an element into running sums in registers.  Accumulators rotate, so that the tensor cores
+// work on the next block meanwhile.
+//
+//   TMA (SWIZZLE_128B) -> shared-memory ring -> tcgen05.mma -> tensor memory -> tcgen05.ld -> registers -> epilogue
+//
+// Two kernels:
+//   block_pair_kernel   tokens are the 128-lane operand, the two CTAs of a cluster share a tile of 256 tokens x 256 (128) weight
+//                       rows (cta_group::2).  A thread of the epilogue holds half of a token's row of it: its scale is one number
+//                       a K block, a_scale of its token times w_scale of its columns.
+//   block_split_kernel  few tokens: weights are the 128-lane operand (128 rows: one row of scales), the tokens the 16 .. 128
+//                       columns, and the reduction is shared out to a cluster, whose CTAs add their sums up through
+//                       distributed shared memory in rank order.
+// All waits are bounded as in gemm_tc.cu.
+#include "gemm_w8a8.cuh"
+#include "tc_tiles.cuh"
+
+#include <algorithm>
+
+namespace llmqrt {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxDevices = 64;
+
+struct BlockParams {
+  const float* a_scale;            // [M, k_blocks]
+  const float* w_scale;            // [ceil(N / 128), k_blocks]
+  const void* bias;                // [N] or null
+  void* out;                       // [M, ldo] 16-bit
+  int64_t ldo;
+  int bias_dtype, bf16;
+  int M, N, k_blocks;
+  int tiles_p, tiles_q, splits, early_w, tma_out;
+  uint32_t idesc;
+  unsigned* status;
+};
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int bf16) {
+  return bf16 ? pack_pair<__nv_bfloat16>(a, b) : pack_pair<__half>(a, b);
+}
+__device__ __forceinline__ F2 f2_of(uint32_t a, uint32_t b) { return f2(__uint_as_float(a), __uint_as_float(b)); }
+
+// ---- few tokens --------------------------------------------------------------------------------------
+constexpr int kSplitThreads = 192;                     // TMA warp, MMA warp, four epilogue warps
+constexpr int kSplitBufs = 4;                          // accumulators of BN columns
+template <int BN> constexpr int split_stage_bytes() { return (kBM + BN) * kRowBytes; }
+template <int BN> constexpr int split_stages() {
+  const int s = 200 * 1024 / split_stage_bytes<BN>();  // (some shared memory is left for the small kernels ahead in a chain)
+  return s > 10 ? 10 : s;
+}
+template <int BN> constexpr int split_smem() { return split_stages<BN>() * split_stage_bytes<BN>() + 1024; }
+template <int BN> constexpr uint32_t split_tmem_cols() { return kSplitBufs * BN; }
+
+template <int BN>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const BlockParams prm) {
+  constexpr int kStages = split_stages<BN>(), kStageBytes = split_stage_bytes<BN>();
+  constexpr int kPer = BN < 32 ? 1 : BN / 32;          // token scales a lane fetches
+  constexpr int kChunk = BN < 32 ? BN : 32;            // columns a tcgen05.ld takes
+  static_assert(kStages * kStageBytes >= BN * kBM * 4, "the ring holds the partial sums");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t bar_full[kStages];
+  __shared__ __align__(8) uint64_t bar_empty[kStages];
+  __shared__ __align__(8) uint64_t bar_acc_full[kSplitBufs];
+  __shared__ __align__(8) uint64_t bar_acc_empty[kSplitBufs];
+  __shared__ __align__(16) float scales[4][2][BN];     // each epilogue warp's own: the tokens' scales of a K block
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &abort_flag;
+  const uint32_t abort_u32 = tc::smem_u32(&abort_flag);
+  const int S = prm.splits, rank = S > 1 ? (int)cluster_ctarank() : 0;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(tc::smem_u32(&bar_full[s]), 1);
+      tc::mbar_init(tc::smem_u32(&bar_empty[s]), 1);
+    }
+    for (int b = 0; b < kSplitBufs; ++b) {
+      tc::mbar_init(tc::smem_u32(&bar_acc_full[b]), 1);
+      tc::mbar_init(tc::smem_u32(&bar_acc_empty[b]), 4);
+    }
+    tc::mbar_fence_init();
+    tc::tma_prefetch_descriptor(&tm_w);
+    tc::tma_prefetch_descriptor(&tm_a);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tc::smem_u32(&tmem_base_slot), split_tmem_cols<BN>());
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = tmem_base_slot;
+  if (threadIdx.x != 0) {                              // (the producer's thread may first request weights)
+    pdl_wait();
+    pdl_trigger();
+  }
+  // S > 1: a cluster for each tile; otherwise a persistent walk.
+  const int num_tiles = prm.tiles_p * prm.tiles_q;
+  const int first_tile = (int)blockIdx.x / S, tile_step = S > 1 ? num_tiles : (int)gridDim.x;
+  const int kb_begin = (int)((int64_t)rank * prm.k_blocks / S);
+  const int kb_count = (int)((int64_t)(rank + 1) * prm.k_blocks / S) - kb_begin;
+
+  F2 acc[BN / 2];                                      // epilogue: row quad * 32 + lane of the tile, all tokens
+  const int quad = warp & 3, wrow = quad * 32 + lane;
+  const float* a_scale = prm.a_scale;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage_i = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      // weights of the first ring ahead of the wait for the preceding kernel, if they are a stored layer's
+      const int pre = first_tile < num_tiles ? min(kStages, kb_count) : 0;
+      const int tp0 = first_tile / prm.tiles_q, tq0 = first_tile % prm.tiles_q;
+      if (!prm.early_w) {
+        pdl_wait();
+        pdl_trigger();
+      }
+      for (int i = 0; i < pre; ++i) {
+        const uint32_t full = tc::smem_u32(&bar_full[i]);
+        tc::mbar_arrive_expect_tx(full, kStageBytes);
+        tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes), &tm_w, full, (kb_begin + i) * kRowBytes, tp0 * kBM);
+      }
+      if (prm.early_w) {
+        pdl_wait();
+        pdl_trigger();
+      }
+      for (int i = 0; i < pre; ++i)
+        tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes + kBM * kRowBytes), &tm_a, tc::smem_u32(&bar_full[i]),
+                        (kb_begin + i) * kRowBytes, tq0 * BN);
+      stage_i = pre == kStages ? 0 : pre;
+      if (pre == kStages) phase = 1;
+      int done = pre;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+        const int tp = tile / prm.tiles_q, tq = tile % prm.tiles_q;
+        for (int it = done; it < kb_count; ++it) {
+          tc::mbar_wait_or_flag(tc::smem_u32(&bar_empty[stage_i]), phase ^ 1u, abort_u32);
+          const uint32_t full = tc::smem_u32(&bar_full[stage_i]);
+          const uint32_t sp = tc::smem_u32(tiles + stage_i * kStageBytes);
+          tc::mbar_arrive_expect_tx(full, kStageBytes);
+          tc::tma_load_2d(sp, &tm_w, full, (kb_begin + it) * kRowBytes, tp * kBM);
+          tc::tma_load_2d(sp + kBM * kRowBytes, &tm_a, full, (kb_begin + it) * kRowBytes, tq * BN);
+          if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
+          if ((it & 3) == 3 && *abort) { ok = false; break; }
+        }
+        done = 0;
+        if (*abort) ok = false;
+      }
+    }
+  } else if (warp == 1) {
+    int stage_i = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      for (int it = 0; it < kb_count; ++it) {
+        if (!tc::mbar_wait_warp(tc::smem_u32(&bar_acc_empty[buf]), acc_phase ^ 1u, abort)) { ok = false; break; }
+        tc::mbar_wait_or_flag(tc::smem_u32(&bar_full[stage_i]), phase, abort_u32);
+        __syncwarp();
+        tc::fence_after_sync();
+        const uint32_t sp = tc::smem_u32(tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(buf * BN);
+        const uint64_t dw = tc::smem_desc_k_major_sw128(sp), da = tc::smem_desc_k_major_sw128(sp + kBM * kRowBytes);
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int j = 0; j < kRowBytes / 32; ++j)
+            tc::mma_ss<tc::MMA_F8>(d, dw + (uint64_t)(2 * j), da + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
+          tc::mma_commit(tc::smem_u32(&bar_empty[stage_i]));
+          tc::mma_commit(tc::smem_u32(&bar_acc_full[buf]));
+        }
+        __syncwarp();
+        if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
+        if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
+      }
+      if (tc::warp_aborted(abort)) ok = false;
+    }
+  } else {
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      const int tp = tile / prm.tiles_q, tq = tile % prm.tiles_q;
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) acc[i] = f2(0.f, 0.f);
+      const float* ws = prm.w_scale + (int64_t)tp * prm.k_blocks + kb_begin;
+      const float* as[kPer];
+      float next[kPer], w_next = __ldg(ws);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {                 // (tokens behind the last one: any valid scale, their columns are not written)
+        as[i] = a_scale + (int64_t)min(tq * BN + i * 32 + lane, prm.M - 1) * prm.k_blocks + kb_begin;
+        next[i] = *as[i];
+      }
+#pragma unroll 1
+      for (int it = 0; it < kb_count; ++it) {
+        float* mine = scales[warp - 2][it & 1];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (BN >= 32 || lane < BN) mine[i * 32 + lane] = __fmul_rn(next[i], w_next);
+        if (it + 1 < kb_count) {
+          w_next = __ldg(ws + it + 1);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) next[i] = as[i][it + 1];
+        }
+        __syncwarp();
+        if (!tc::mbar_wait_warp(tc::smem_u32(&bar_acc_full[buf]), acc_phase, abort)) { ok = false; break; }
+        tc::fence_after_sync();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN);
+#pragma unroll
+        for (int c0 = 0; c0 < BN; c0 += kChunk) {
+          uint32_t r[kChunk];
+          if constexpr (BN >= 32) {
+            tc::tmem_ld_32x32(taddr + (uint32_t)c0, r);
+          } else {
+            tc::tmem_ld_32x8(taddr, *reinterpret_cast<uint32_t(*)[8]>(r));
+            tc::tmem_ld_32x8(taddr + 8u, *reinterpret_cast<uint32_t(*)[8]>(r + 8));
+          }
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < kChunk; c += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(mine + c0 + c);
+            F2& lo = acc[(c0 + c) / 2];
+            F2& hi = acc[(c0 + c) / 2 + 1];
+            lo = f2_fma(f2_of(r[c], r[c + 1]), f2(s.x, s.y), lo);
+            hi = f2_fma(f2_of(r[c + 2], r[c + 3]), f2(s.z, s.w), hi);
+          }
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&bar_acc_empty[buf]));
+        if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
+      }
+      if (S == 1 && ok) {                              // straight from registers: a warp writes 32 neighbours of a token's row
+        const int n = tp * kBM + wrow, tokens = min(BN, prm.M - tq * BN);
+        if (n < prm.N) {
+          const float b = prm.bias ? load_as_f32(prm.bias, n, prm.bias_dtype) : 0.f;
+#pragma unroll
+          for (int i = 0; i < BN; ++i) {
+            float lo, hi;
+            f2_split(acc[i / 2], lo, hi);
+            if (i < tokens) store_from_f32(prm.out, (int64_t)(tq * BN + i) * prm.ldo + n, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, (i & 1 ? hi : lo) + b);
+          }
+        }
+      }
+    }
+  }
+
+  if (S > 1) {
+    // The ring is idle once every MMA of this CTA has been seen to finish: each CTA leaves its sums there, [token][row], and
+    // takes its share of the tokens from all of them, in rank order.
+    const int tp = first_tile / prm.tiles_q, tq = first_tile % prm.tiles_q, tokens = min(BN, prm.M - tq * BN);
+    float* part = reinterpret_cast<float*>(tiles);
+    __syncthreads();
+    if (warp >= 2) {
+#pragma unroll
+      for (int i = 0; i < BN; ++i) {
+        float lo, hi;
+        f2_split(acc[i / 2], lo, hi);
+        if (i < tokens) part[i * kBM + wrow] = i & 1 ? hi : lo;
+      }
+    }
+    cluster_sync_all();
+    const int m0 = rank * tokens / S, m1 = (rank + 1) * tokens / S, n = tp * kBM + wrow;
+    if (warp >= 2 && n < prm.N) {
+      const float b = prm.bias ? load_as_f32(prm.bias, n, prm.bias_dtype) : 0.f;
+      for (int m = m0; m < m1; ++m) {
+        const uint32_t local = tc::smem_u32(part + m * kBM + wrow);
+        float v[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+          v[r] = 0.f;
+          if (r < S) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(tc::cluster_addr(local, (uint32_t)r)) : "memory");
+        }
+        float sum = v[0];
+#pragma unroll
+        for (int r = 1; r < kMaxCluster; ++r) sum += v[r];
+        store_from_f32(prm.out, (int64_t)(tq * BN + m) * prm.ldo + n, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, sum + b);
+      }
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (abort_flag) {                                    // a wait ran out: copies still in flight are given time to land
+    const uint64_t t0 = tc::global_timer_ns();
+    while (tc::global_timer_ns() - t0 < 100000ull) __nanosleep(1000);
+  }
+  if (S > 1) cluster_sync_all();                       // nobody leaves while a peer may read its sums
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem_base, split_tmem_cols<BN>());
+  }
+  if (threadIdx.x == 0 && abort_flag && prm.status) *prm.status = 1u;
+}
+
+// ---- many tokens -------------------------------------------------------------------------------------
+constexpr int kPairThreads = 64 + 256;                 // TMA warp, MMA warp, eight epilogue warps
+constexpr int kPairOutBytes = 32 * 128;                // staging tile of an epilogue warp
+template <int BN> constexpr int pair_stage_bytes() { return (kBM + BN / 2) * kRowBytes; }
+template <int BN> constexpr int pair_stages() { return BN == 256 ? 6 : 8; }
+template <int BN> constexpr int pair_bufs() { return 512 / BN; }
+template <int BN>
+struct PairShared {
+  uint8_t tiles[pair_stages<BN>() * pair_stage_bytes<BN>()];
+  uint8_t out[8 * kPairOutBytes];
+  uint64_t bar_full[pair_stages<BN>()];                // used in the leader only
+  uint64_t bar_empty[pair_stages<BN>()];
+  uint64_t bar_acc_full[pair_bufs<BN>()];
+  uint64_t bar_acc_empty[pair_bufs<BN>()];             // used in the leader only: one arrival per epilogue warp of both CTAs
+  uint32_t tmem_base_slot;
+  int abort_flag;
+};
+
+template <int BN>
+__global__ void __launch_bounds__(kPairThreads, 1)
+block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_out, const BlockParams prm) {
+  extern __shared__ __align__(1024) uint8_t smem_pair[];
+  constexpr int kStages = pair_stages<BN>(), kStageBytes = pair_stage_bytes<BN>(), kHalf = BN / 2, kBufs = pair_bufs<BN>();
+  PairShared<BN>& sh = *reinterpret_cast<PairShared<BN>*>(smem_pair);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &sh.abort_flag;
+  const uint32_t abort_u32 = tc::smem_u32(&sh.abort_flag);
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    sh.abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      tc::mbar_init(tc::smem_u32(&sh.bar_full[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sh.bar_empty[s]), 1);
+    }
+    for (int b = 0; b < kBufs; ++b) {
+      tc::mbar_init(tc::smem_u32(&sh.bar_acc_full[b]), 1);
+      tc::mbar_init(tc::smem_u32(&sh.bar_acc_empty[b]), 16);
+    }
+    tc::mbar_fence_init();
+    tc::tma_prefetch_descriptor(&tm_a);
+    tc::tma_prefetch_descriptor(&tm_w);
+    tc::tma_prefetch_descriptor(&tm_out);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc_pair(tc::smem_u32(&sh.tmem_base_slot), 512);
+    tc::tmem_relinquish_pair();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                                  // both CTAs' barriers exist before anything signals them
+  tc::fence_after_sync();
+  const uint32_t tmem_base = sh.tmem_base_slot;
+  pdl_wait();
+  pdl_trigger();
+  const int num_tiles = prm.tiles_p * prm.tiles_q;     // of 256 tokens x BN rows of weights
+  const int first_tile = (int)(blockIdx.x >> 1), tile_step = (int)(gridDim.x >> 1);
+  const int kb_count = prm.k_blocks;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full0 = tc::cluster_addr(tc::smem_u32(&sh.bar_full[0]), 0u);
+      int stage_i = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+        int tp, tq;
+        pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
+        const int row_a = tp * 2 * kBM + (int)rank * kBM, row_w = tq * BN + (int)rank * kHalf;
+        for (int it = 0; it < kb_count; ++it) {
+          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_empty[stage_i]), phase ^ 1u, abort_u32);
+          if (leader) tc::mbar_arrive_expect_tx(tc::smem_u32(&sh.bar_full[stage_i]), 2u * kStageBytes);
+          const uint32_t full = full0 + (uint32_t)stage_i * 8u;
+          const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes);
+          tc::tma_load_2d_pair(sp, &tm_a, full, it * kRowBytes, row_a);
+          tc::tma_load_2d_pair(sp + kBM * kRowBytes, &tm_w, full, it * kRowBytes, row_w);
+          if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
+        }
+        if (*abort) ok = false;
+      }
+    }
+  } else if (warp == 1) {
+    if (leader) {
+      int stage_i = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+        for (int it = 0; it < kb_count; ++it) {
+          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_empty[buf]), acc_phase ^ 1u, abort_u32);
+          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_full[stage_i]), phase, abort_u32);
+          __syncwarp();
+          tc::fence_after_sync();
+          const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(buf * BN);
+          const uint64_t da = tc::smem_desc_k_major_sw128(sp), db = tc::smem_desc_k_major_sw128(sp + kBM * kRowBytes);
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int j = 0; j < kRowBytes / 32; ++j)
+              tc::mma_ss_pair<tc::MMA_F8>(d, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
+            tc::mma_commit_pair(tc::smem_u32(&sh.bar_empty[stage_i]));
+            tc::mma_commit_pair(tc::smem_u32(&sh.bar_acc_full[buf]));
+          }
+          __syncwarp();
+          if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
+          if (++buf == kBufs) { buf = 0; acc_phase ^= 1u; }
+        }
+        if (tc::warp_aborted(abort)) ok = false;
+      }
+    }
+  } else {
+    // Two warps a lane quadrant, each taking half of the tile's columns: with 256 columns, one block of w_scale.
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* out_tile = sh.out + (warp - 2) * kPairOutBytes;
+    const uint32_t acc_empty0 = tc::cluster_addr(tc::smem_u32(&sh.bar_acc_empty[0]), 0u);
+    const int last_block = (prm.N - 1) / 128;
+    int buf = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      int tp, tq;
+      pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
+      const int row0 = tp * 2 * kBM + (int)rank * kBM + quad * 32, row = row0 + lane, x0 = tq * BN + half * kHalf;
+      // (rows and columns behind the matrix take some valid scale: they are not written)
+      const float* as = prm.a_scale + (int64_t)min(row, prm.M - 1) * kb_count;
+      const float* ws = prm.w_scale + (int64_t)min(x0 / 128, last_block) * kb_count;
+      F2 acc[kHalf / 2];
+#pragma unroll
+      for (int i = 0; i < kHalf / 2; ++i) acc[i] = f2(0.f, 0.f);
+      float a_next = __ldg(as), w_next = __ldg(ws);
+#pragma unroll 1
+      for (int it = 0; it < kb_count; ++it) {
+        const float s = __fmul_rn(a_next, w_next);
+        const F2 ss = f2(s, s);
+        if (it + 1 < kb_count) {
+          a_next = __ldg(as + it + 1);
+          w_next = __ldg(ws + it + 1);
+        }
+        if (!tc::mbar_wait_warp(tc::smem_u32(&sh.bar_acc_full[buf]), acc_phase, abort)) { ok = false; break; }
+        tc::fence_after_sync();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * kHalf);
+#pragma unroll
+        for (int c0 = 0; c0 < kHalf; c0 += 32) {
+          uint32_t r[32];
+          tc::tmem_ld_32x32(taddr + (uint32_t)c0, r);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) acc[(c0 + c) / 2] = f2_fma(f2_of(r[c], r[c + 1]), ss, acc[(c0 + c) / 2]);
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(acc_empty0 + (uint32_t)buf * 8u);
+        if (++buf == kBufs) { buf = 0; acc_phase ^= 1u; }
+      }
+      if (!ok) break;
+      // 64 columns at a time through the warp's staging tile, 16-byte unit u of row r at u ^ (r & 7)
+#pragma unroll
+      for (int c0 = 0; c0 < kHalf; c0 += 64) {
+        const int cols = prm.N - x0 - c0;              // columns left of the matrix (may be <= 0)
+        if (prm.tma_out && lane == 0) tma_stores_read();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint32_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float lo, hi;
+            f2_split(acc[(c0 + 8 * k) / 2 + e], lo, hi);
+            if (prm.bias) {
+              const int n = x0 + c0 + 8 * k + 2 * e;
+              if (n < prm.N) lo += load_as_f32(prm.bias, n, prm.bias_dtype);
+              if (n + 1 < prm.N) hi += load_as_f32(prm.bias, n + 1, prm.bias_dtype);
+            }
+            v[e] = pack16(lo, hi, prm.bf16);
+          }
+          *reinterpret_cast<uint4*>(out_tile + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        if (prm.tma_out) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && row0 < prm.M && cols > 0) tma_store_2d(&tm_out, tc::smem_u32(out_tile), x0 + c0, row0);
+        } else {                                       // rows of the output that do not begin on 16 bytes
+          __syncwarp();
+          for (int r = 0; r < min(32, prm.M - row0); ++r) {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(prm.out) + (int64_t)(row0 + r) * prm.ldo + x0 + c0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = h * 32 + lane;
+              if (c < cols) dst[c] = *reinterpret_cast<const uint16_t*>(out_tile + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (prm.tma_out && lane == 0) tma_stores_done();
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (sh.abort_flag) {
+    const uint64_t t0 = tc::global_timer_ns();
+    while (tc::global_timer_ns() - t0 < 100000ull) __nanosleep(1000);
+  }
+  cluster_sync_all();                                  // nobody leaves while its peer may still signal it
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (threadIdx.x == 0 && sh.abort_flag && prm.status) *prm.status = 1u;
+}
+
+// ---- host side ---------------------------------------------------------------------------------------
+
+template <typename Kern>
+cudaLaunchConfig_t config(Kern, int grid, int cluster, int threads, int smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (pdl_enabled()) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  return cfg;
+}
+// How many clusters of 1 .. kMaxCluster CTAs of a kernel can be resident at once (asked once per device and kernel).
+template <typename Kern>
+void ask_clusters(Kern kern, int threads, int smem, int lo, int hi, int* known) {
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem) != LLMQRT_OK) return;
+  for (int c = lo; c <= hi; ++c) {
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = config(kern, c, c, threads, smem, nullptr, attr);
+    if (cudaOccupancyMaxActiveClusters(&known[c], kern, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      known[c] = 0;
+    }
+  }
+}
+template <int BN> const int* split_clusters() {
+  static std::once_flag once[kMaxDevices];
+  static int known[kMaxDevices][kMaxCluster + 1];
+  static const int none[kMaxCluster + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return none;
+  std::call_once(once[dev], [dev] { ask_clusters(block_split_kernel<BN>, kSplitThreads, split_smem<BN>(), 1, kMaxCluster, known[dev]); });
+  return known[dev];
+}
+template <int BN> int pair_clusters() {
+  static std::once_flag once[kMaxDevices];
+  static int known[kMaxDevices][3];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
+  std::call_once(once[dev], [dev] { ask_clusters(block_pair_kernel<BN>, kPairThreads, (int)sizeof(PairShared<BN>), 2, 2, known[dev]); });
+  return known[dev][2];
+}
+
+// The cluster that shares a reduction: waves of co-resident clusters x (K blocks of a CTA + what a CTA costs beside them).
+int pick_splits(int64_t tiles, int k_blocks, const int* active, double* blocks) {
+  const double fixed = 8., sms = sm_count();
+  int splits = 1;
+  double best = (double)ceil_div(tiles, (int64_t)sms) * (k_blocks + fixed);
+  for (int s = 2; s <= kMaxCluster && k_blocks >= 2 * s && tiles < sms; ++s) {
+    if (active[s] <= 0) continue;
+    const double t = (double)ceil_div(tiles, (int64_t)active[s]) * ((double)k_blocks / s + fixed);
+    if (t < best) { best = t; splits = s; }
+  }
+  if (blocks) *blocks = best;
+  return splits;
+}
+
+struct Operands {
+  const void* a;
+  const void* w;
+  int64_t lda, ldw, K;
+};
+
+template <int BN>
+int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
+  prm.tiles_p = (int)ceil_div(prm.N, kBM);
+  prm.tiles_q = (int)ceil_div(prm.M, BN);
+  prm.idesc = tc::instr_desc(1, 0, 0, kBM, BN);
+  const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
+  LLMQRT_REQUIRE(tiles <= 0x7fffffffll / kMaxCluster, "fp8 block linear: too many tiles");
+  prm.splits = pick_splits(tiles, prm.k_blocks, split_clusters<BN>(), nullptr);
+  CUtensorMap tm_w, tm_a;
+  if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, kBM)) return rc;
+  if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, BN)) return rc;
+  auto kern = block_split_kernel<BN>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), split_smem<BN>())) return rc;
+  const int64_t grid = prm.splits > 1 ? tiles * prm.splits : std::min(tiles, (int64_t)sm_count());
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = config(kern, (int)grid, prm.splits, kSplitThreads, split_smem<BN>(), st, attr);
+  LLMQRT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, prm));
+  return check_launch("fp8 block linear");
+}
+
+template <int BN>
+int launch_pair(const Operands& o, BlockParams prm, cudaStream_t st) {
+  const int clusters = pair_clusters<BN>();
+  if (clusters <= 0) return set_error(LLMQRT_ERR_CUDA, "fp8 block linear: no cluster of two CTAs fits on this device");
+  prm.tiles_p = (int)ceil_div(prm.M, 2 * kBM);
+  prm.tiles_q = (int)ceil_div(prm.N, BN);
+  prm.idesc = tc::instr_desc(1, 0, 0, 2 * kBM, BN);
+  const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
+  LLMQRT_REQUIRE(tiles <= 0x7fffffffll, "fp8 block linear: too many tiles");
+  prm.tma_out = (reinterpret_cast<uintptr_t>(prm.out) & 15) == 0 && prm.ldo % 8 == 0;
+  CUtensorMap tm_a, tm_w, tm_out;
+  if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, kBM)) return rc;
+  if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, BN / 2)) return rc;
+  if (!prm.tma_out) tm_out = tm_a;                     // (not used)
+  else if (int rc = make_output_map(&tm_out, prm.out, 2, prm.M, prm.N, prm.ldo)) return rc;
+  auto kern = block_pair_kernel<BN>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)sizeof(PairShared<BN>))) return rc;
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = config(kern, 2 * (int)std::min(tiles, (int64_t)clusters), 2, kPairThreads, (int)sizeof(PairShared<BN>), st, attr);
+  LLMQRT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tm_a, tm_w, tm_out, prm));
+  return check_launch("fp8 block linear");
+}
+
+}  // namespace
+}  // namespace llmqrt
+
+using namespace llmqrt;
+
+extern "C" int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint8_t* w, int64_t ldw, const void* bias, int bias_dtype,
+                                       const float* a_scale, const float* w_scale, void* out, int out_dtype, int64_t ldo, int64_t M,
+                                       int64_t N, int64_t K, void* workspace, llmqrt_stream_t stream, int flags) {
+  LLMQRT_REQUIRE(M >= 0 && N > 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31),
+                 "fp8 block linear: bad shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  LLMQRT_REQUIRE(K % 16 == 0 && lda >= K && ldw >= K && lda % 16 == 0 && ldw % 16 == 0,
+                 "fp8 block linear: K=%lld and leading dimensions must be multiples of 16, lda=%lld / ldw=%lld at least K", (long long)K,
+                 (long long)lda, (long long)ldw);
+  LLMQRT_REQUIRE(ldo >= N, "fp8 block linear: ldo=%lld < N", (long long)ldo);
+  LLMQRT_REQUIRE(out_dtype == LLMQRT_F16 || out_dtype == LLMQRT_BF16, "fp8 block linear: out must be fp16 or bf16");
+  LLMQRT_REQUIRE(!bias || bias_dtype == LLMQRT_F16 || bias_dtype == LLMQRT_BF16 || bias_dtype == LLMQRT_F32, "fp8 block linear: bad bias dtype");
+  LLMQRT_REQUIRE((flags & ~LLMQRT_GEMM_STATIC_WEIGHT) == 0, "fp8 block linear: unknown flags 0x%x", flags);
+  if (M == 0) return LLMQRT_OK;
+  LLMQRT_REQUIRE(a && w && a_scale && w_scale && out, "fp8 block linear: null pointer");
+  LLMQRT_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) == 0, "fp8 block linear: operands must be 16-byte aligned");
+  BlockParams p{};
+  p.a_scale = a_scale; p.w_scale = w_scale; p.bias = bias; p.bias_dtype = bias_dtype; p.out = out; p.ldo = ldo;
+  p.bf16 = out_dtype == LLMQRT_BF16; p.M = (int)M; p.N = (int)N; p.k_blocks = (int)ceil_div(K, kRowBytes);
+  p.early_w = flags & LLMQRT_GEMM_STATIC_WEIGHT ? 1 : 0;
+  p.status = workspace ? ws_scalars(workspace) + 1 : nullptr;
+  const Operands o{a, w, lda, ldw, K};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (M <= 16) return launch_split<16>(o, p, st);
+  if (M <= 32) return launch_split<32>(o, p, st);
+  if (M <= 64) return launch_split<64>(o, p, st);
+  if (M <= 128) return launch_split<128>(o, p, st);
+  const int64_t rows = ceil_div(M, 2 * kBM), clusters = sm_count() / 2;
+  if (rows * ceil_div(N, 256) >= clusters) return launch_pair<256>(o, p, st);
+  return launch_pair<128>(o, p, st);
+}

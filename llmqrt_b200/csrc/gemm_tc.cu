@@ -37,7 +37,7 @@
 // a row-parallel layer straight into the other GPUs' all-reduce buffers.
 #include "gemm_w8a8.cuh"
 #include "peer_comm.cuh"
-#include "tc_primitives.cuh"
+#include "tc_tiles.cuh"
 
 #include <algorithm>
 #include <mutex>
@@ -51,7 +51,6 @@ constexpr int kAwqGroups = 4;                 // groups of four warps that dequa
 constexpr int kAwqWarps = 4 * kAwqGroups;
 constexpr int kThreadsAwq = kThreads + kAwqWarps * 32 + 32;      // (+ the warp that fetches the packed tiles)
 constexpr int kBM = 128;           // rows of P per tile (UMMA M)
-constexpr int kRowBytes = 128;     // bytes of K per stage row (one swizzle span)
 constexpr int kMaxCluster = 8;     // CTAs that may share a reduction
 constexpr int kMaxDevices = 64;
 constexpr int kSmemBudget = 226 * 1024;   // of the 227 KiB a block may use
@@ -126,14 +125,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
 // Bulk asynchronous copy of `bytes` from this CTA's shared memory to the same offsets' counterpart in
 // CTA `cta_rank` of the cluster; completion is counted (complete_tx) on that CTA's mbarrier.
 // dst_local / bar_local are addresses in THIS CTA's window; mapa translates them to the peer's.
@@ -950,33 +941,6 @@ template <int BN> constexpr int pair_smem_bytes() {
 constexpr int kPairThreads = 64 + 256;                                 // producer warp, MMA warp, eight epilogue warps
 __device__ __forceinline__ void pair_epi_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// 32 bytes from registers to global memory (an address that is a multiple of 32): every lane writes a whole sector.
-__device__ __forceinline__ void st_global_256(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
-               "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
-}
-// A 2-D tile from shared memory to global memory; the issuing thread's stores are counted in bulk groups.
-__device__ __forceinline__ void tma_store_2d(const void* tensor_map, uint32_t src_smem, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t"
-               "cp.async.bulk.commit_group;" ::"l"(tensor_map), "r"(src_smem), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
-// Tile order: the weight tiles are walked in groups of kPairGroup; inside a group the token tile
-// changes fastest.  The clusters that run at the same time then share a few weight tiles and a few
-// token tiles, and a weight group (8 x 256 rows) stays in L2 until every token tile has used it -- with
-// the weight tile changing fastest instead, a weight matrix larger than L2 (gate_up of Qwen2-7B: 136 MB)
-// is streamed from HBM once per token tile.
-constexpr int kPairGroup = 8;
-__device__ __forceinline__ void pair_tile_coords(int tile, int tiles_p, int tiles_q, int& tp, int& tq) {
-  const int per_group = tiles_p * kPairGroup;
-  const int group = tile / per_group, within = tile - group * per_group;
-  const int gw = min(kPairGroup, tiles_q - group * kPairGroup);         // weight tiles in this group
-  tp = within / gw;
-  tq = group * kPairGroup + within - tp * gw;
-}
-
 template <int KIND, int BN, bool DIRECT>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
@@ -1262,54 +1226,6 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 }
 
 // ---- host side -------------------------------------------------------------------------------
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-// 2-D K-major operand [rows, K] with `ld` elements between rows; box = 128 bytes x box_rows.
-int make_operand_map(CUtensorMap* map, const void* base, int elt_bytes, int64_t rows, int64_t K, int64_t ld,
-                     int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return set_error(LLMQRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(ld * elt_bytes)};
-  cuuint32_t box[2] = {(cuuint32_t)(kRowBytes / elt_bytes), (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, elt_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
-                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(LLMQRT_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return LLMQRT_OK;
-}
-
-// 2-D output [rows, cols] with `ld` elements between rows; box = 128 bytes x 32 rows, the two-CTA kernel's staging tile.
-int make_output_map(CUtensorMap* map, void* base, int elt_bytes, int64_t rows, int64_t cols, int64_t ld) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return set_error(LLMQRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(ld * elt_bytes)};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / elt_bytes), 32};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, elt_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box,
-                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(LLMQRT_ERR_CUDA, "cuTensorMapEncodeTiled (output) failed with code %d", (int)r);
-  return LLMQRT_OK;
-}
 
 // Packed 4-bit weights as a 2-D uint32 matrix [rows, words] (row-major); box = 8 words x box_rows, no swizzle.
 int make_packed_map(CUtensorMap* map, const void* base, int64_t rows, int64_t words, int box_rows) {

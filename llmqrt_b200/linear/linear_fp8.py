@@ -147,3 +147,58 @@ class FP8StaticLinear(_FP8Base):
             qout = ops.quantize_fp8_static(out, self.output_scale.data).view(out.shape)
             out = qout.to(out.dtype) * self.output_scale.data
         return out.to(x.dtype)
+
+
+def quantize_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 [N, K], fp32 scales [ceil(N / 128), ceil(K / 128)]) of a weight, absmax / 448 for each block of 128 x 128; set-up code."""
+    N, K = weight.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    q = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=weight.device)
+    scale = torch.empty((nb, kb), dtype=torch.float32, device=weight.device)
+    for n in range(nb):                                      # (a row of blocks at a time: no fp32 copy of the whole weight)
+        rows = weight[128 * n:128 * n + 128].float()
+        pad = torch.nn.functional.pad(rows, (0, kb * 128 - K)).view(rows.shape[0], kb, 128)
+        s = pad.abs().amax((0, 2)).clamp_min(1e-12) / 448.0
+        scale[n] = s
+        q[128 * n:128 * n + 128] = (pad / s[None, :, None]).clamp(-448, 448).view(rows.shape[0], -1)[:, :K].to(torch.float8_e4m3fn)
+    return q, scale
+
+
+class FP8BlockLinear(LinearBase):
+    """e4m3 weights with an fp32 scale for each block of 128 x 128 (weight_scale [ceil(out / 128), ceil(in / 128)], a value is
+    weight * its block's scale), activations quantized per token and 128 features.  The reference has scales per tensor and
+    per row only (linear_fp8.py:134-313).  `weight` holds the fp8 values themselves.
+
+    forward(x) quantizes x and multiplies, two kernels and one native call; `forward_quantized` takes what
+    glue.rmsnorm_fp8_block or ops.quantize_fp8_block left."""
+
+    def __init__(self, in_features, out_features, bias, dev="cuda:0", dtype=torch.bfloat16):
+        super().__init__()
+        if in_features % 16:
+            raise ValueError("FP8BlockLinear: in_features must be a multiple of 16")
+        self.dtype, self.in_features, self.out_features = dtype, in_features, out_features
+        P = torch.nn.Parameter
+        self.weight = P(torch.zeros((out_features, in_features), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn), requires_grad=False)
+        self.weight_scale = P(torch.ones((-(-out_features // 128), -(-in_features // 128)), dtype=torch.float32, device=dev), requires_grad=False)
+        self.bias = P(torch.zeros(out_features, dtype=dtype, device=dev), requires_grad=False) if bias else None
+
+    @classmethod
+    def from_linear(cls, module: torch.nn.Linear, w_bit=8, group_size=128, init_only=True, dtype=torch.bfloat16):
+        assert w_bit == 8 and group_size == 128, "fp8 block quant has blocks of 128"
+        layer = cls(module.in_features, module.out_features, module.bias is not None, module.weight.device, dtype)
+        if init_only:
+            return layer
+        q, scale = quantize_blocks(module.weight.data)
+        layer.weight.data.copy_(q)
+        layer.weight_scale.data.copy_(scale)
+        if module.bias is not None:
+            layer.bias.data.copy_(module.bias.data.to(dtype))
+        return layer
+
+    def forward(self, x):
+        assert x.device == self.weight.device, "when fp8 linear fwd, input and qweight must be same device!"
+        return fast.fp8_block(x, self.weight, self.bias, self.weight_scale)
+
+    def forward_quantized(self, q, scale, out_dtype=None):
+        """q e4m3 [M, in_features], scale fp32 [M, ceil(in_features / 128)] -> [M, out_features] in out_dtype (default: the layer's)."""
+        return fast.fp8_linear_block(q, self.weight, self.bias, scale, self.weight_scale, out_dtype or self.dtype, True)

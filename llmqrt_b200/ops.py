@@ -159,6 +159,13 @@ def fp8_linear_rowwise(a, w, bias, x_scale, w_scale, static_weight: bool = False
     return out
 
 
+def fp8_linear_block(a, w, bias, a_scale, w_scale, out_dtype, static_weight: bool = False) -> torch.Tensor:
+    """out [M, N] (fp16 / bf16) of a e4m3 [M, K] with a_scale [M, ceil(K / 128)] (quantize_fp8_block, glue.rmsnorm_fp8_block) and w
+    e4m3 [N, K] with w_scale [ceil(N / 128), ceil(K / 128)]: the sums over each 128 inputs are scaled in fp32 before they are added up.
+    K a multiple of 16; bias fp16, bf16 or fp32."""
+    return L.fast.fp8_linear_block(a, w, bias, a_scale, w_scale, out_dtype, static_weight)
+
+
 def gemm_16bit(a, w, bias=None) -> torch.Tensor:
     """out[M,N] = a[M,K] @ w[N,K]^T (+ bias) on tcgen05, fp32 accumulate; a, w, bias share one 16-bit dtype."""
     dev = L.require_cuda(a, w, bias)

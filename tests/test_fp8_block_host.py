@@ -1,0 +1,76 @@
+"""What the block-scaled fp8 layer refuses, before anything is launched (on CPU tensors: shapes and types are checked first)."""
+import pytest
+import torch
+
+F8 = torch.float8_e4m3fn
+
+
+def _call(M=4, N=200, K=256, **kw):
+    from llmqrt_b200 import ops
+    f8 = lambda *s: torch.zeros(s, dtype=torch.uint8).view(F8)  # noqa: E731
+    a = dict(a=f8(M, K), w=f8(N, K), bias=None, a_scale=torch.ones(M, -(-K // 128)), w_scale=torch.ones(-(-N // 128), -(-K // 128)),
+             out_dtype=torch.float16)
+    return ops.fp8_linear_block(**(a | kw))
+
+
+@pytest.mark.parametrize("kw,error,match", [
+    (dict(), RuntimeError, "CUDA device"),
+    (dict(a=torch.zeros(4, 256).half()), TypeError, "float8_e4m3fn"),
+    (dict(a=torch.zeros(4, 256, dtype=torch.uint8).view(torch.float8_e5m2)), TypeError, "float8_e4m3fn"),
+    (dict(w=torch.zeros(200, 256).half()), TypeError, "float8_e4m3fn"),
+    (dict(w=torch.zeros(200, 128, dtype=torch.uint8).view(F8)), RuntimeError, "weight must be"),
+    (dict(w=torch.zeros(256, 200, dtype=torch.uint8).view(F8).t()), RuntimeError, "weight must be"),
+    (dict(a_scale=torch.ones(4, 1)), RuntimeError, "a's scales"),
+    (dict(a_scale=torch.ones(2, 4).t()), RuntimeError, "a's scales"),
+    (dict(a_scale=torch.ones(4, 2).half()), TypeError, "fp32"),
+    (dict(w_scale=torch.ones(1, 2)), RuntimeError, "weight's scales"),
+    (dict(w_scale=torch.ones(2, 2).double()), TypeError, "fp32"),
+    (dict(bias=torch.zeros(128).half()), RuntimeError, "bias"),
+    (dict(out_dtype=torch.int32), TypeError, "dtype"),
+    (dict(out_dtype="fp16"), TypeError, "dtype"),
+])
+def test_refusals(kw, error, match):
+    with pytest.raises(error, match=match):
+        _call(**kw)
+
+
+def test_the_library_refuses():
+    """Sizes and pointers that the kernels do not take come back as a status; nothing is launched."""
+    from llmqrt_b200 import _lib
+
+    def call(M=1, N=1, K=128, lda=128, ldw=128, ldo=1, out=0, bias=None, bd=0, p=64, flags=0):
+        return _lib._lib.llmqrt_fp8_linear_block(p, lda, p, ldw, bias, bd, p, p, p, out, ldo, M, N, K, None, None, flags)
+    for kw in (dict(K=120), dict(K=0), dict(N=0), dict(M=-1), dict(lda=112), dict(ldw=136), dict(ldo=0), dict(out=2), dict(bias=64, bd=3), dict(p=None),
+               dict(p=8), dict(flags=2), dict(M=2 ** 31)):
+        assert call(**kw) == -1, kw
+    assert call(M=0) == 0
+
+    def rows(K=128, ldx=128, dt=0, p=64, M=1):
+        return _lib._lib.llmqrt_quantize_fp8_block(p, dt, M, K, ldx, p, p, None)
+    for kw in (dict(K=12), dict(K=0), dict(ldx=120), dict(ldx=132), dict(dt=2), dict(p=None), dict(p=68), dict(K=40000, ldx=40000), dict(M=-1)):
+        assert rows(**kw) == -1, kw
+    norm = lambda res, h: _lib._lib.llmqrt_rmsnorm_fp8_block(64, 128, res, 128, h, 64, 1e-6, 64, 64, 0, 1, 128, None)  # noqa: E731
+    assert norm(64, None) == -1 and norm(None, 64) == -1
+
+
+def test_module_refuses():
+    from llmqrt_b200.linear import FP8BlockLinear
+    with pytest.raises(ValueError):
+        FP8BlockLinear(200, 8, False, dev="cpu")
+    layer = FP8BlockLinear(160, 130, True, dev="cpu")
+    assert layer.weight.shape == (130, 160) and layer.weight_scale.shape == (2, 2) and layer.bias.shape == (130,)
+    with pytest.raises(AssertionError):
+        FP8BlockLinear.from_linear(torch.nn.Linear(32, 32), group_size=64)
+
+
+def test_quantized_blocks():
+    """A weight's codes and scales, on the CPU: within half a step of e4m3 of the weight, absmax at the greatest code."""
+    from llmqrt_b200.linear.linear_fp8 import quantize_blocks
+    w = torch.randn(300, 400, generator=torch.Generator().manual_seed(0))
+    w[:128, :128] *= 100
+    w[130:140] = 0
+    q, s = quantize_blocks(w)
+    assert q.shape == w.shape and q.dtype == F8 and s.shape == (3, 4)
+    full = s.repeat_interleave(128, 0)[:300].repeat_interleave(128, 1)[:, :400]
+    err = (q.float() * full - w).abs()
+    assert (err <= w.abs() * 2.0 ** -4 * 1.001 + full * 2.0 ** -10 * 1.001).all() and (q.float().abs().amax() == 448)
