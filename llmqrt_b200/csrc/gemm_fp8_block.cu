@@ -28,6 +28,7 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxDevices = 64;
+constexpr int kMaxPairs = 256;     // clusters of two CTAs that share tiles
 
 struct BlockParams {
   const float* a_scale;            // [M, k_blocks]
@@ -38,6 +39,9 @@ struct BlockParams {
   int bias_dtype, bf16;
   int M, N, k_blocks;
   int tiles_p, tiles_q, splits, early_w, tma_out;
+  int whole_tiles, sharers;        // pair kernel: the tiles behind these are shared out by K blocks among so many clusters
+  float* partials;                 // ... and what that needs of the workspace
+  int* counters;
   uint32_t idesc;
   unsigned* status;
 };
@@ -46,6 +50,17 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int bf16) {
   return bf16 ? pack_pair<__nv_bfloat16>(a, b) : pack_pair<__half>(a, b);
 }
 __device__ __forceinline__ F2 f2_of(uint32_t a, uint32_t b) { return f2(__uint_as_float(a), __uint_as_float(b)); }
+
+// One arrival on an mbarrier of the cluster that says only that this warp's tcgen05.ld are back (tcgen05.wait::ld has seen to
+// that).  Not a release: at cluster scope that waits for the warp's outstanding loads, here the next block's scales, 1400
+// cycles a K block.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
+// A load that stays where it stands in the program, one K block ahead of its use.  (Left to the compiler it is waited for early: 322
+// against 283 us for 4096 x 3584 x 18944.)
+__device__ __forceinline__ void load_now(const float* p, float& v) { asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p)); }
 
 // ---- few tokens --------------------------------------------------------------------------------------
 constexpr int kSplitThreads = 192;                     // TMA warp, MMA warp, four epilogue warps
@@ -220,8 +235,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
           if constexpr (BN >= 32) {
             tc::tmem_ld_32x32(taddr + (uint32_t)c0, r);
           } else {
-            tc::tmem_ld_32x8(taddr, *reinterpret_cast<uint32_t(*)[8]>(r));
-            tc::tmem_ld_32x8(taddr + 8u, *reinterpret_cast<uint32_t(*)[8]>(r + 8));
+            tc::tmem_ld_32x16(taddr, r);
           }
           tc::tmem_ld_wait();
 #pragma unroll
@@ -302,29 +316,79 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 }
 
 // ---- many tokens -------------------------------------------------------------------------------------
-constexpr int kPairThreads = 64 + 256;                 // TMA warp, MMA warp, eight epilogue warps
+// Accumulators are 128 columns wide, four of them, and take turns: a K block of 256 columns has two, each with an issuing warp and
+// epilogue warps of its own, a K block of 128 one, every second block by the other issuer.  An issuer needs about 500 cycles for
+// four MMAs and what goes with them -- to find a barrier complete takes 100, the MMAs and two commits 200 -- where the tensor
+// cores need 512 for a K block of 256 columns; and an accumulator's round (MMAs, commit, the epilogue's loads, the remote
+// arrival that frees it) is longer than either, so that the finer ones keep more going at a time.
+//
+// Work: tiles dealt out whole, in waves, and the tiles of a last wave that would be mostly empty as one long run of K blocks, of which
+// clusters get equal shares, tiles' borders falling where they may.  A tile that several clusters
+// have worked on is added up by the last of them to finish (counted off in the workspace, warp by warp, nobody waits), always
+// in the clusters' order: the same bits every time.
+constexpr int kPairThreads = 128 + 256;                // TMA warp, two MMA warps, one without work; eight epilogue warps
 constexpr int kPairOutBytes = 32 * 128;                // staging tile of an epilogue warp
 template <int BN> constexpr int pair_stage_bytes() { return (kBM + BN / 2) * kRowBytes; }
 template <int BN> constexpr int pair_stages() { return BN == 256 ? 6 : 8; }
-template <int BN> constexpr int pair_bufs() { return 512 / BN; }
+// An epilogue thread holds 128 running sums beside 64 columns on their way.  Three warps a scheduler are launched with 168 registers
+// each, and the epilogue's two take some of what the other does not need.
+// With 256 columns the epilogue wants every register it can have (40 + 2 * 232 = 3 * 168), with 128 it does not.
+template <int BN> constexpr int epilogue_regs() { return BN == 256 ? 232 : 224; }
+template <int BN> constexpr int other_regs() { return BN == 256 ? 40 : 56; }
+constexpr int kIssuers = 2;
+constexpr int kAccs = 4, kAccCols = 128;               // accumulators: all of tensor memory
 template <int BN>
 struct PairShared {
   uint8_t tiles[pair_stages<BN>() * pair_stage_bytes<BN>()];
   uint8_t out[8 * kPairOutBytes];
   uint64_t bar_full[pair_stages<BN>()];                // used in the leader only
   uint64_t bar_empty[pair_stages<BN>()];
-  uint64_t bar_acc_full[pair_bufs<BN>()];
-  uint64_t bar_acc_empty[pair_bufs<BN>()];             // used in the leader only: one arrival per epilogue warp of both CTAs
+  uint64_t bar_acc_full[kAccs];
+  uint64_t bar_acc_empty[kAccs];                       // used in the leader only: an arrival for each epilogue warp that reads it, of both CTAs
   uint32_t tmem_base_slot;
   int abort_flag;
 };
+
+// A cluster's share of the work: whole tiles, then its part of the run of K blocks.  (A run has fewer than 2^31 K blocks.)
+struct PairWork {
+  int tile_next, u, u_end;
+  __device__ PairWork(const BlockParams& p, int cluster) : tile_next(cluster), u(0), u_end(0) {
+    if (cluster < p.sharers) {
+      const int64_t run = (int64_t)(p.tiles_p * p.tiles_q - p.whole_tiles) * p.k_blocks;
+      u = (int)(cluster * run / p.sharers);
+      u_end = (int)((cluster + 1) * run / p.sharers);
+    }
+  }
+  // The next tile and its K blocks [k0, k1).
+  __device__ __forceinline__ bool next(const BlockParams& p, int& tile, int& k0, int& k1) {
+    if (tile_next < p.whole_tiles) {
+      tile = tile_next;
+      tile_next += (int)(gridDim.x >> 1);
+      k0 = 0;
+      k1 = p.k_blocks;
+      return true;
+    }
+    if (u >= u_end) return false;
+    tile = u / p.k_blocks;
+    k0 = u - tile * p.k_blocks;
+    tile += p.whole_tiles;
+    k1 = min(p.k_blocks, k0 + (u_end - u));
+    u += k1 - k0;
+    return true;
+  }
+};
+// Which of `sharers` clusters of a run of `total` K blocks has block u in its share.
+__device__ __forceinline__ int sharer_of(int64_t u, int64_t total, int sharers) { return (int)(((u + 1) * sharers - 1) / total); }
 
 template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1)
 block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_out, const BlockParams prm) {
   extern __shared__ __align__(1024) uint8_t smem_pair[];
-  constexpr int kStages = pair_stages<BN>(), kStageBytes = pair_stage_bytes<BN>(), kHalf = BN / 2, kBufs = pair_bufs<BN>();
+  constexpr int kStages = pair_stages<BN>(), kStageBytes = pair_stage_bytes<BN>();
+  constexpr int kAccOf = BN / kAccCols, kRounds = kAccs / kAccOf;      // accumulators of a K block, K blocks' worth of them
+  static_assert(kIssuers == 2 && kAccs % kIssuers == 0 && kStages % kIssuers == 0, "an issuer takes every second accumulator");
+  constexpr int kCols = BN / 2, kLd = 32;              // columns of an epilogue warp, and of a load
   PairShared<BN>& sh = *reinterpret_cast<PairShared<BN>*>(smem_pair);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sh.abort_flag;
@@ -335,11 +399,11 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     sh.abort_flag = 0;
     for (int s = 0; s < kStages; ++s) {
       tc::mbar_init(tc::smem_u32(&sh.bar_full[s]), 1);
-      tc::mbar_init(tc::smem_u32(&sh.bar_empty[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sh.bar_empty[s]), kAccOf);
     }
-    for (int b = 0; b < kBufs; ++b) {
+    for (int b = 0; b < kAccs; ++b) {
       tc::mbar_init(tc::smem_u32(&sh.bar_acc_full[b]), 1);
-      tc::mbar_init(tc::smem_u32(&sh.bar_acc_empty[b]), 16);
+      tc::mbar_init(tc::smem_u32(&sh.bar_acc_empty[b]), 16 / kAccOf);
     }
     tc::mbar_fence_init();
     tc::tma_prefetch_descriptor(&tm_a);
@@ -357,107 +421,172 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   const uint32_t tmem_base = sh.tmem_base_slot;
   pdl_wait();
   pdl_trigger();
-  const int num_tiles = prm.tiles_p * prm.tiles_q;     // of 256 tokens x BN rows of weights
-  const int first_tile = (int)(blockIdx.x >> 1), tile_step = (int)(gridDim.x >> 1);
-  const int kb_count = prm.k_blocks;
+  PairWork work(prm, (int)(blockIdx.x >> 1));               // (every role walks it for itself)
+  int tile, k0, k1;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full0 = tc::cluster_addr(tc::smem_u32(&sh.bar_full[0]), 0u);
-      int stage_i = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-        int tp, tq;
-        pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
-        const int row_a = tp * 2 * kBM + (int)rank * kBM, row_w = tq * BN + (int)rank * kHalf;
-        for (int it = 0; it < kb_count; ++it) {
-          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_empty[stage_i]), phase ^ 1u, abort_u32);
-          if (leader) tc::mbar_arrive_expect_tx(tc::smem_u32(&sh.bar_full[stage_i]), 2u * kStageBytes);
-          const uint32_t full = full0 + (uint32_t)stage_i * 8u;
-          const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes);
-          tc::tma_load_2d_pair(sp, &tm_a, full, it * kRowBytes, row_a);
-          tc::tma_load_2d_pair(sp + kBM * kRowBytes, &tm_w, full, it * kRowBytes, row_w);
-          if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
-        }
-        if (*abort) ok = false;
-      }
-    }
-  } else if (warp == 1) {
-    if (leader) {
-      int stage_i = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-        for (int it = 0; it < kb_count; ++it) {
-          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_empty[buf]), acc_phase ^ 1u, abort_u32);
-          tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_full[stage_i]), phase, abort_u32);
-          __syncwarp();
-          tc::fence_after_sync();
-          const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(buf * BN);
-          const uint64_t da = tc::smem_desc_k_major_sw128(sp), db = tc::smem_desc_k_major_sw128(sp + kBM * kRowBytes);
-          if (tc::elect_one()) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs<BN>()));
+    if (warp == 0) {
+      if (lane == 0) {
+        const uint32_t full0 = tc::cluster_addr(tc::smem_u32(&sh.bar_full[0]), 0u);
+        int stage_i = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        while (ok && work.next(prm, tile, k0, k1)) {
+          int tp, tq;
+          pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
+          // of each accumulator's 128 weight rows a CTA brings 64
+          const int row_a = tp * 2 * kBM + (int)rank * kBM, row_w = tq * BN + (int)rank * (kAccCols / 2);
+          for (int it = k0; it < k1; ++it) {
+            tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_empty[stage_i]), phase ^ 1u, abort_u32);
+            if (leader) tc::mbar_arrive_expect_tx(tc::smem_u32(&sh.bar_full[stage_i]), 2u * kStageBytes);
+            const uint32_t full = full0 + (uint32_t)stage_i * 8u;
+            const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes);
+            tc::tma_load_2d_pair(sp, &tm_a, full, it * kRowBytes, row_a);
 #pragma unroll
-            for (int j = 0; j < kRowBytes / 32; ++j)
-              tc::mma_ss_pair<tc::MMA_F8>(d, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
-            tc::mma_commit_pair(tc::smem_u32(&sh.bar_empty[stage_i]));
-            tc::mma_commit_pair(tc::smem_u32(&sh.bar_acc_full[buf]));
+            for (int h = 0; h < kAccOf; ++h)
+              tc::tma_load_2d_pair(sp + (kBM + h * (kAccCols / 2)) * kRowBytes, &tm_w, full, it * kRowBytes, row_w + h * kAccCols);
+            if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
           }
-          __syncwarp();
-          if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
-          if (++buf == kBufs) { buf = 0; acc_phase ^= 1u; }
+          if (*abort) ok = false;
         }
-        if (tc::warp_aborted(abort)) ok = false;
+      }
+    } else if (warp <= kIssuers) {
+      if (leader) {
+        // two accumulators a K block: this warp's is the w-th of every block; one: every second block's, from the w-th on
+        constexpr int kStep = kAccOf == 2 ? 1 : kIssuers;
+        const int w = warp - 1;
+        int stage_i = kAccOf == 2 ? 0 : w, acc_i = w, skip = kAccOf == 2 ? 0 : w;       // skip: blocks of the segment ahead of this warp's first
+        uint32_t phase = 0, acc_phase = 0;
+        while (work.next(prm, tile, k0, k1)) {
+          int left = k1 - k0 - skip;
+          if (kStep == 2) skip = (skip + k1 - k0) & 1;
+          for (; left > 0; left -= kStep) {
+            tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_empty[acc_i]), acc_phase ^ 1u, abort_u32);
+            tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_full[stage_i]), phase, abort_u32);
+            __syncwarp();
+            tc::fence_after_sync();
+            const uint32_t sp = tc::smem_u32(sh.tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(acc_i * kAccCols);
+            const uint64_t da = tc::smem_desc_k_major_sw128(sp);
+            const uint64_t db = tc::smem_desc_k_major_sw128(sp + (kBM + (kAccOf == 2 ? w * (kAccCols / 2) : 0)) * kRowBytes);
+            if (tc::elect_one()) {
+#pragma unroll
+              for (int j = 0; j < kRowBytes / 32; ++j)
+                tc::mma_ss_pair<tc::MMA_F8>(d, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
+              tc::mma_commit_pair(tc::smem_u32(&sh.bar_acc_full[acc_i]));
+              tc::mma_commit_pair(tc::smem_u32(&sh.bar_empty[stage_i]));
+            }
+            __syncwarp();
+            if ((stage_i += kStep) >= kStages) { stage_i -= kStages; phase ^= 1u; }
+            if ((acc_i += kIssuers) >= kAccs) { acc_i -= kAccs; acc_phase ^= 1u; }
+          }
+          if (tc::warp_aborted(abort)) break;
+        }
       }
     }
   } else {
-    // Two warps a lane quadrant, each taking half of the tile's columns: with 256 columns, one block of w_scale.
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* out_tile = sh.out + (warp - 2) * kPairOutBytes;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(epilogue_regs<BN>()));
+    // Two warps a lane quadrant, each taking half of the tile's columns: of one block of w_scale.
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* own = sh.out + (warp - 4) * kPairOutBytes;
     const uint32_t acc_empty0 = tc::cluster_addr(tc::smem_u32(&sh.bar_acc_empty[0]), 0u);
-    const int last_block = (prm.N - 1) / 128;
-    int buf = 0;
+    const int acc_h = kAccOf == 2 ? half : 0;
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * kCols);
+    int round = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+    while (work.next(prm, tile, k0, k1)) {
       int tp, tq;
       pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
-      const int row0 = tp * 2 * kBM + (int)rank * kBM + quad * 32, row = row0 + lane, x0 = tq * BN + half * kHalf;
-      // (rows and columns behind the matrix take some valid scale: they are not written)
-      const float* as = prm.a_scale + (int64_t)min(row, prm.M - 1) * kb_count;
-      const float* ws = prm.w_scale + (int64_t)min(x0 / 128, last_block) * kb_count;
-      F2 acc[kHalf / 2];
+      // Rows and columns behind the matrix take some valid scale: they are not written.
+      const float* as = prm.a_scale + (int64_t)min(tp * 2 * kBM + (int)rank * kBM + quad * 32 + lane, prm.M - 1) * prm.k_blocks;
+      const float* ws = prm.w_scale + (int64_t)min((tq * BN + half * kCols) / 128, (prm.N - 1) / 128) * prm.k_blocks;
+      float a_next, w_next;
+      load_now(as + k0, a_next);
+      load_now(ws + k0, w_next);
+      F2 acc[kCols / 2];
 #pragma unroll
-      for (int i = 0; i < kHalf / 2; ++i) acc[i] = f2(0.f, 0.f);
-      float a_next = __ldg(as), w_next = __ldg(ws);
+      for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
+      auto await = [&]() {                             // the next K block's accumulator
+        tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_full[round * kAccOf + acc_h]), acc_phase, abort_u32);
+        __syncwarp();
+        tc::fence_after_sync();
+      };
+      uint32_t r[2][kLd];
+      await();
+      tc::tmem_ld_32x32(t_lane + (uint32_t)(round * BN), r[0]);
 #pragma unroll 1
-      for (int it = 0; it < kb_count; ++it) {
+      for (int kb = k0; kb < k1; ++kb) {
         const float s = __fmul_rn(a_next, w_next);
         const F2 ss = f2(s, s);
-        if (it + 1 < kb_count) {
-          a_next = __ldg(as + it + 1);
-          w_next = __ldg(ws + it + 1);
-        }
-        if (!tc::mbar_wait_warp(tc::smem_u32(&sh.bar_acc_full[buf]), acc_phase, abort)) { ok = false; break; }
-        tc::fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * kHalf);
+        load_now(as + min(kb + 1, k1 - 1), a_next);
+        load_now(ws + min(kb + 1, k1 - 1), w_next);
+        // 32 columns are multiplied while the next ones come; after a block's last ones its accumulator is free, and the next
+        // block's first ones are asked for ahead of the products (behind them: 316 against 267 us)
+        const uint32_t taddr = t_lane + (uint32_t)(round * BN);
 #pragma unroll
-        for (int c0 = 0; c0 < kHalf; c0 += 32) {
-          uint32_t r[32];
-          tc::tmem_ld_32x32(taddr + (uint32_t)c0, r);
+        for (int k = 0; k < kCols / kLd; ++k) {
           tc::tmem_ld_wait();
+          if (k + 1 < kCols / kLd) {
+            tc::tmem_ld_32x32(taddr + (uint32_t)(kLd * k + kLd), r[(k + 1) & 1]);
+          } else {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + (uint32_t)(round * kAccOf + acc_h) * 8u);
+            if (++round == kRounds) { round = 0; acc_phase ^= 1u; }
+            if (kb + 1 < k1) {
+              await();
+              tc::tmem_ld_32x32(t_lane + (uint32_t)(round * BN), r[0]);
+            }
+          }
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) acc[(c0 + c) / 2] = f2_fma(f2_of(r[c], r[c + 1]), ss, acc[(c0 + c) / 2]);
+          for (int c = 0; c < kLd; c += 2) acc[(kLd * k + c) / 2] = f2_fma(f2_of(r[k & 1][c], r[k & 1][c + 1]), ss, acc[(kLd * k + c) / 2]);
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive_cluster(acc_empty0 + (uint32_t)buf * 8u);
-        if (++buf == kBufs) { buf = 0; acc_phase ^= 1u; }
       }
-      if (!ok) break;
+      if (tc::warp_aborted(abort)) break;
+      pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
+      const int row0 = tp * 2 * kBM + (int)rank * kBM + quad * 32, x0 = tq * BN + half * kCols;
+      if (k1 - k0 < prm.k_blocks) {
+        // a tile of several clusters: this one's sums to the workspace, four columns of a row a store
+        const int shared = tile - prm.whole_tiles;
+        const int64_t total = (int64_t)(prm.tiles_p * prm.tiles_q - prm.whole_tiles) * prm.k_blocks, u0 = (int64_t)shared * prm.k_blocks;
+        const int c_first = sharer_of(u0, total, prm.sharers), c_last = sharer_of(u0 + prm.k_blocks - 1, total, prm.sharers);
+        const int64_t mine = (int64_t)((int)rank * 8 + warp - 4) * (kCols * 32);
+        auto slot_of = [&](int c) {                    // a cluster has two slots: for the tile that its share begins with, and the last one
+          const int begins = (int)(c * total / prm.sharers / prm.k_blocks);
+          return prm.partials + (int64_t)(2 * c + (shared == begins ? 0 : 1)) * (2 * kBM * BN) + mine + lane * 4;
+        };
+        float* dst = slot_of((int)(blockIdx.x >> 1));
+#pragma unroll
+        for (int i = 0; i < kCols / 4; ++i) {
+          float4 v;
+          f2_split(acc[2 * i], v.x, v.y);
+          f2_split(acc[2 * i + 1], v.z, v.w);
+          __stcg(reinterpret_cast<float4*>(dst + i * 128), v);
+        }
+        __threadfence();
+        __syncwarp();
+        int before = 0;
+        int* counter = prm.counters + (shared * 2 + (int)rank) * 8 + warp - 4;
+        if (lane == 0) before = atomicAdd(counter, 1);
+        before = __shfl_sync(0xffffffffu, before, 0);
+        if (before < c_last - c_first) continue;       // another cluster will finish the tile
+        __threadfence();
+        if (lane == 0) *counter = 0;
+#pragma unroll
+        for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
+        for (int c = c_first; c <= c_last; ++c) {
+          const float* src = slot_of(c);
+#pragma unroll
+          for (int i = 0; i < kCols / 4; ++i) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i * 128));
+            acc[2 * i] = f2_add(acc[2 * i], f2(v.x, v.y));
+            acc[2 * i + 1] = f2_add(acc[2 * i + 1], f2(v.z, v.w));
+          }
+        }
+      }
       // 64 columns at a time through the warp's staging tile, 16-byte unit u of row r at u ^ (r & 7)
 #pragma unroll
-      for (int c0 = 0; c0 < kHalf; c0 += 64) {
+      for (int c0 = 0; c0 < kCols; c0 += 64) {
         const int cols = prm.N - x0 - c0;              // columns left of the matrix (may be <= 0)
         if (prm.tma_out && lane == 0) tma_stores_read();
         __syncwarp();
@@ -475,20 +604,20 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             }
             v[e] = pack16(lo, hi, prm.bf16);
           }
-          *reinterpret_cast<uint4*>(out_tile + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(own + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         if (prm.tma_out) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && row0 < prm.M && cols > 0) tma_store_2d(&tm_out, tc::smem_u32(out_tile), x0 + c0, row0);
+          if (lane == 0 && row0 < prm.M && cols > 0) tma_store_2d(&tm_out, tc::smem_u32(own), x0 + c0, row0);
         } else {                                       // rows of the output that do not begin on 16 bytes
           __syncwarp();
-          for (int r = 0; r < min(32, prm.M - row0); ++r) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(prm.out) + (int64_t)(row0 + r) * prm.ldo + x0 + c0;
+          for (int q = 0; q < min(32, prm.M - row0); ++q) {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(prm.out) + (int64_t)(row0 + q) * prm.ldo + x0 + c0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int c = h * 32 + lane;
-              if (c < cols) dst[c] = *reinterpret_cast<const uint16_t*>(out_tile + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+              if (c < cols) dst[c] = *reinterpret_cast<const uint16_t*>(own + q * 128 + (((c >> 3) ^ (q & 7)) << 4) + (c & 7) * 2);
             }
           }
           __syncwarp();
@@ -604,25 +733,48 @@ int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
   return check_launch("fp8 block linear");
 }
 
+// Clusters to launch, and how many tiles are dealt out whole.  What is left over of the whole waves is shared out by K blocks where
+// that saves more of them than the sums through the workspace cost; every share has a few, and a tile few shares.  (Shares begin
+// anywhere in K: the more clusters work like that, the less of the operands they find in L2.  Together with one of the waves, for
+// shares of one size, 4096 x 3584 x 18944 took 261 us.)
+constexpr int kShareCost = 20;                         // K blocks
+constexpr int kLeastShare = 4, kMostShares = 6;
+int deal_out(int64_t tiles, int clusters, BlockParams& prm) {
+  const int64_t rest = tiles % clusters, kb = prm.k_blocks;
+  prm.whole_tiles = (int)tiles;
+  prm.sharers = 0;
+  if (rest && prm.partials && clusters <= kMaxPairs) {
+    const int64_t sharers = std::min({(int64_t)clusters, rest * kb / kLeastShare, rest * kMostShares});
+    if (sharers > rest && kb - ceil_div(rest * kb, sharers) >= kShareCost && rest * 16 <= LLMQRT_WS_NUM_COUNTERS && rest * kb <= 0x7fffffffll) {
+      prm.whole_tiles = (int)(tiles - rest);
+      prm.sharers = (int)sharers;
+      return (int)(tiles > rest ? clusters : sharers);
+    }
+  }
+  return (int)std::min(tiles, (int64_t)clusters);
+}
+
 template <int BN>
 int launch_pair(const Operands& o, BlockParams prm, cudaStream_t st) {
   const int clusters = pair_clusters<BN>();
   if (clusters <= 0) return set_error(LLMQRT_ERR_CUDA, "fp8 block linear: no cluster of two CTAs fits on this device");
   prm.tiles_p = (int)ceil_div(prm.M, 2 * kBM);
   prm.tiles_q = (int)ceil_div(prm.N, BN);
-  prm.idesc = tc::instr_desc(1, 0, 0, 2 * kBM, BN);
+  prm.idesc = tc::instr_desc(1, 0, 0, 2 * kBM, kAccCols);
   const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
   LLMQRT_REQUIRE(tiles <= 0x7fffffffll, "fp8 block linear: too many tiles");
+  const int grid = deal_out(tiles, clusters, prm);
   prm.tma_out = (reinterpret_cast<uintptr_t>(prm.out) & 15) == 0 && prm.ldo % 8 == 0;
   CUtensorMap tm_a, tm_w, tm_out;
   if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, kBM)) return rc;
-  if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, BN / 2)) return rc;
+  if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, kAccCols / 2)) return rc;
   if (!prm.tma_out) tm_out = tm_a;                     // (not used)
   else if (int rc = make_output_map(&tm_out, prm.out, 2, prm.M, prm.N, prm.ldo)) return rc;
+  static_assert(2 * kMaxPairs * sizeof(float) * 2 * kBM * BN <= LLMQRT_WS_PARTIAL_BYTES, "two partial tiles for each cluster");
   auto kern = block_pair_kernel<BN>;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), (int)sizeof(PairShared<BN>))) return rc;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = config(kern, 2 * (int)std::min(tiles, (int64_t)clusters), 2, kPairThreads, (int)sizeof(PairShared<BN>), st, attr);
+  cudaLaunchConfig_t cfg = config(kern, 2 * grid, 2, kPairThreads, (int)sizeof(PairShared<BN>), st, attr);
   LLMQRT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tm_a, tm_w, tm_out, prm));
   return check_launch("fp8 block linear");
 }
@@ -651,7 +803,11 @@ extern "C" int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint
   p.a_scale = a_scale; p.w_scale = w_scale; p.bias = bias; p.bias_dtype = bias_dtype; p.out = out; p.ldo = ldo;
   p.bf16 = out_dtype == LLMQRT_BF16; p.M = (int)M; p.N = (int)N; p.k_blocks = (int)ceil_div(K, kRowBytes);
   p.early_w = flags & LLMQRT_GEMM_STATIC_WEIGHT ? 1 : 0;
-  p.status = workspace ? ws_scalars(workspace) + 1 : nullptr;
+  if (workspace) {
+    p.status = ws_scalars(workspace) + 1;
+    p.partials = reinterpret_cast<float*>(ws_partials(workspace));
+    p.counters = ws_counters(workspace);
+  }
   const Operands o{a, w, lda, ldw, K};
   cudaStream_t st = (cudaStream_t)stream;
   if (M <= 16) return launch_split<16>(o, p, st);
