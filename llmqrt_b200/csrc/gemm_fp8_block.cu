@@ -73,6 +73,9 @@ template <int BN> constexpr int split_stages() {
 template <int BN> constexpr int split_smem() { return split_stages<BN>() * split_stage_bytes<BN>() + 1024; }
 template <int BN> constexpr uint32_t split_tmem_cols() { return kSplitBufs * BN; }
 
+__device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[32]) { tc::tmem_ld_32x32(taddr, r); }
+__device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[16]) { tc::tmem_ld_32x16(taddr, r); }
+
 template <int BN>
 __global__ void __launch_bounds__(kSplitThreads, 1)
 block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const BlockParams prm) {
@@ -201,18 +204,19 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   } else {
     int buf = 0;
     uint32_t acc_phase = 0;
-    bool ok = true;
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+    bool ready = false;
+    for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
       const int tp = tile / prm.tiles_q, tq = tile % prm.tiles_q;
 #pragma unroll
       for (int i = 0; i < BN / 2; ++i) acc[i] = f2(0.f, 0.f);
       const float* ws = prm.w_scale + (int64_t)tp * prm.k_blocks + kb_begin;
       const float* as[kPer];
-      float next[kPer], w_next = __ldg(ws);
+      float next[kPer], w_next;
+      load_now(ws, w_next);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {                 // (tokens behind the last one: any valid scale, their columns are not written)
         as[i] = a_scale + (int64_t)min(tq * BN + i * 32 + lane, prm.M - 1) * prm.k_blocks + kb_begin;
-        next[i] = *as[i];
+        load_now(as[i], next[i]);
       }
 #pragma unroll 1
       for (int it = 0; it < kb_count; ++it) {
@@ -220,39 +224,42 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
           if (BN >= 32 || lane < BN) mine[i * 32 + lane] = __fmul_rn(next[i], w_next);
-        if (it + 1 < kb_count) {
-          w_next = __ldg(ws + it + 1);
+        const int ahead = min(it + 1, kb_count - 1);
+        load_now(ws + ahead, w_next);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) next[i] = as[i][it + 1];
-        }
+        for (int i = 0; i < kPer; ++i) load_now(as[i] + ahead, next[i]);
+        if (!ready) tc::mbar_wait_or_flag(tc::smem_u32(&bar_acc_full[buf]), acc_phase, abort_u32);
         __syncwarp();
-        if (!tc::mbar_wait_warp(tc::smem_u32(&bar_acc_full[buf]), acc_phase, abort)) { ok = false; break; }
         tc::fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN);
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN), empty = tc::smem_u32(&bar_acc_empty[buf]);
+        if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
+        uint32_t r[2][kChunk];
+        ld_chunk(taddr, r[0]);
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += kChunk) {
-          uint32_t r[kChunk];
-          if constexpr (BN >= 32) {
-            tc::tmem_ld_32x32(taddr + (uint32_t)c0, r);
-          } else {
-            tc::tmem_ld_32x16(taddr, r);
-          }
+          uint32_t(&v)[kChunk] = r[c0 / kChunk & 1];
+          // (whether the next block's accumulator is complete is asked for ahead: the answer takes 100 cycles, be it yes)
+          if (c0 + kChunk == BN) ready = tc::mbar_test_wait(tc::smem_u32(&bar_acc_full[buf]), acc_phase);
           tc::tmem_ld_wait();
+          if (c0 + kChunk < BN) {
+            ld_chunk(taddr + (uint32_t)(c0 + kChunk), r[(c0 / kChunk + 1) & 1]);
+          } else {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(empty);
+          }
 #pragma unroll
           for (int c = 0; c < kChunk; c += 4) {
             const float4 s = *reinterpret_cast<const float4*>(mine + c0 + c);
             F2& lo = acc[(c0 + c) / 2];
             F2& hi = acc[(c0 + c) / 2 + 1];
-            lo = f2_fma(f2_of(r[c], r[c + 1]), f2(s.x, s.y), lo);
-            hi = f2_fma(f2_of(r[c + 2], r[c + 3]), f2(s.z, s.w), hi);
+            lo = f2_fma(f2_of(v[c], v[c + 1]), f2(s.x, s.y), lo);
+            hi = f2_fma(f2_of(v[c + 2], v[c + 3]), f2(s.z, s.w), hi);
           }
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&bar_acc_empty[buf]));
-        if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
       }
-      if (S == 1 && ok) {                              // straight from registers: a warp writes 32 neighbours of a token's row
+      if (tc::warp_aborted(abort)) break;
+      if (S == 1) {                                    // straight from registers: a warp writes 32 neighbours of a token's row
         const int n = tp * kBM + wrow, tokens = min(BN, prm.M - tq * BN);
         if (n < prm.N) {
           const float b = prm.bias ? load_as_f32(prm.bias, n, prm.bias_dtype) : 0.f;
@@ -282,21 +289,36 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
       }
     }
     cluster_sync_all();
-    const int m0 = rank * tokens / S, m1 = (rank + 1) * tokens / S, n = tp * kBM + wrow;
+    const int m1 = (rank + 1) * tokens / S, n = tp * kBM + lane * 4;   // a warp takes a token's 128 columns, four a lane
     if (warp >= 2 && n < prm.N) {
-      const float b = prm.bias ? load_as_f32(prm.bias, n, prm.bias_dtype) : 0.f;
-      for (int m = m0; m < m1; ++m) {
-        const uint32_t local = tc::smem_u32(part + m * kBM + wrow);
-        float v[kMaxCluster];
+      float b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = prm.bias && n + j < prm.N ? load_as_f32(prm.bias, n + j, prm.bias_dtype) : 0.f;
+      const bool wide = n + 4 <= prm.N && prm.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 7) == 0;
+      for (int m = rank * tokens / S + warp - 2; m < m1; m += 4) {
+        const uint32_t local = tc::smem_u32(part + m * kBM + lane * 4);
+        float4 v[kMaxCluster];
 #pragma unroll
         for (int r = 0; r < kMaxCluster; ++r) {
-          v[r] = 0.f;
-          if (r < S) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[r]) : "r"(tc::cluster_addr(local, (uint32_t)r)) : "memory");
+          v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < S)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[r].x), "=f"(v[r].y), "=f"(v[r].z), "=f"(v[r].w)
+                         : "r"(tc::cluster_addr(local, (uint32_t)r)) : "memory");
         }
-        float sum = v[0];
+        float4 sum = v[0];
 #pragma unroll
-        for (int r = 1; r < kMaxCluster; ++r) sum += v[r];
-        store_from_f32(prm.out, (int64_t)(tq * BN + m) * prm.ldo + n, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, sum + b);
+        for (int r = 1; r < kMaxCluster; ++r) {
+          sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w;
+        }
+        const float o[4] = {sum.x + b[0], sum.y + b[1], sum.z + b[2], sum.w + b[3]};
+        const int64_t at = (int64_t)(tq * BN + m) * prm.ldo + n;
+        if (wide) {
+          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(prm.out) + at) = make_uint2(pack16(o[0], o[1], prm.bf16), pack16(o[2], o[3], prm.bf16));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < prm.N) store_from_f32(prm.out, at + j, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, o[j]);
+        }
       }
     }
   }
@@ -389,6 +411,7 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
   constexpr int kAccOf = BN / kAccCols, kRounds = kAccs / kAccOf;      // accumulators of a K block, K blocks' worth of them
   static_assert(kIssuers == 2 && kAccs % kIssuers == 0 && kStages % kIssuers == 0, "an issuer takes every second accumulator");
   constexpr int kCols = BN / 2, kLd = 32;              // columns of an epilogue warp, and of a load
+  constexpr bool kAhead = BN == 256;
   PairShared<BN>& sh = *reinterpret_cast<PairShared<BN>*>(smem_pair);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sh.abort_flag;
@@ -506,34 +529,43 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
       F2 acc[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
-      auto await = [&]() {                             // the next K block's accumulator
-        tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_full[round * kAccOf + acc_h]), acc_phase, abort_u32);
+      // 32 columns are multiplied while the next ones come; after a block's last ones its accumulator is free.  The wait for the next
+      // block's takes 100 cycles even where it is complete.  With 256 columns it stands ahead of the last products, together
+      // with the next first columns (behind them: 316 against 267 us without the scales); with 128, whether it is complete is
+      // asked for ahead of the last columns (1000 x 4608 x 3584 21.8 us, like the other 23.3; with 256 it costs registers: 627
+      // against 504 us for 4096 x 37888 x 3584).
+      uint32_t r[2][kLd];
+      bool ready = false;
+      auto await = [&]() {
+        if (!ready) tc::mbar_wait_or_flag(tc::smem_u32(&sh.bar_acc_full[round * kAccOf + acc_h]), acc_phase, abort_u32);
         __syncwarp();
         tc::fence_after_sync();
       };
-      uint32_t r[2][kLd];
-      await();
-      tc::tmem_ld_32x32(t_lane + (uint32_t)(round * BN), r[0]);
+      if (kAhead) {
+        await();
+        tc::tmem_ld_32x32(t_lane + (uint32_t)(round * BN), r[0]);
+      }
 #pragma unroll 1
       for (int kb = k0; kb < k1; ++kb) {
+        if (!kAhead) await();
+        const uint32_t taddr = t_lane + (uint32_t)(round * BN), empty = acc_empty0 + (uint32_t)(round * kAccOf + acc_h) * 8u;
+        if (!kAhead) tc::tmem_ld_32x32(taddr, r[0]);
         const float s = __fmul_rn(a_next, w_next);
         const F2 ss = f2(s, s);
         load_now(as + min(kb + 1, k1 - 1), a_next);
         load_now(ws + min(kb + 1, k1 - 1), w_next);
-        // 32 columns are multiplied while the next ones come; after a block's last ones its accumulator is free, and the next
-        // block's first ones are asked for ahead of the products (behind them: 316 against 267 us)
-        const uint32_t taddr = t_lane + (uint32_t)(round * BN);
+        if (++round == kRounds) { round = 0; acc_phase ^= 1u; }
 #pragma unroll
         for (int k = 0; k < kCols / kLd; ++k) {
+          if (!kAhead && k + 1 == kCols / kLd) ready = tc::mbar_test_wait(tc::smem_u32(&sh.bar_acc_full[round * kAccOf + acc_h]), acc_phase);
           tc::tmem_ld_wait();
           if (k + 1 < kCols / kLd) {
             tc::tmem_ld_32x32(taddr + (uint32_t)(kLd * k + kLd), r[(k + 1) & 1]);
           } else {
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0 + (uint32_t)(round * kAccOf + acc_h) * 8u);
-            if (++round == kRounds) { round = 0; acc_phase ^= 1u; }
-            if (kb + 1 < k1) {
+            if (lane == 0) mbar_arrive_cluster_relaxed(empty);
+            if (kAhead && kb + 1 < k1) {
               await();
               tc::tmem_ld_32x32(t_lane + (uint32_t)(round * BN), r[0]);
             }
@@ -694,17 +726,41 @@ template <int BN> int pair_clusters() {
 }
 
 // The cluster that shares a reduction: waves of co-resident clusters x (K blocks of a CTA + what a CTA costs beside them).
-int pick_splits(int64_t tiles, int k_blocks, const int* active, double* blocks) {
+int pick_splits(int64_t tiles, int k_blocks, const int* active, int* waves) {
   const double fixed = 8., sms = sm_count();
   int splits = 1;
-  double best = (double)ceil_div(tiles, (int64_t)sms) * (k_blocks + fixed);
+  *waves = (int)ceil_div(tiles, (int64_t)sms);
+  double best = *waves * (k_blocks + fixed);
   for (int s = 2; s <= kMaxCluster && k_blocks >= 2 * s && tiles < sms; ++s) {
     if (active[s] <= 0) continue;
-    const double t = (double)ceil_div(tiles, (int64_t)active[s]) * ((double)k_blocks / s + fixed);
-    if (t < best) { best = t; splits = s; }
+    const int w = (int)ceil_div(tiles, (int64_t)active[s]);
+    const double t = w * ((double)k_blocks / s + fixed);
+    if (t < best) { best = t; splits = s; *waves = w; }
   }
-  if (blocks) *blocks = best;
   return splits;
+}
+
+// How the pair kernel's tiles of 256 x BN are dealt out: `whole` of them one by one, the rest by K blocks among `sharers` clusters,
+// and the estimated microseconds.  A tile has at most three shares.  Fitted to 200 sizes, M = 130 .. 2048, N = 300 .. 8960, K = 2048 ..
+// 18944, with and without sharing: a K block takes 0.34 - 0.43 us (256 columns) or 0.23 - 0.27 (128), by how many clusters are at
+// work; the sums through the workspace, and shares that begin anywhere in K and so find less of the operands in L2, cost
+// 10 - 17 or 3 - 9.  256 x 300 x 18944: 29.7 us shared, 48.8 not; 2048 x 3584 x 18944 135 and 143; 333 x 3584 x 8960 28 and 23.
+struct Deal {
+  int64_t tiles, whole;
+  int sharers;
+  double us;
+};
+template <int BN> Deal deal_out(int64_t M, int64_t N, int64_t kb, bool workspace) {
+  const int64_t clusters = sm_count() / 2, tiles = ceil_div(M, 2 * kBM) * ceil_div(N, BN), rest = tiles % clusters, waves = tiles / clusters;
+  const double fill = std::min(1., (double)tiles / clusters);
+  const double block = BN == 256 ? 0.335 + 0.09 * fill : 0.225 + 0.04 * fill;
+  Deal d{tiles, tiles, 0, (BN == 256 ? 6.8 : 5.1) + (waves + (rest ? 1 : 0)) * (kb * block + 0.8)};
+  if (!workspace || !rest || clusters > kMaxPairs || rest * 16 > LLMQRT_WS_NUM_COUNTERS || rest * kb > 0x7fffffffll) return d;
+  const int64_t sharers = rest * 3 <= clusters ? rest * 3 : rest * 2 <= clusters ? rest * 2 : clusters;
+  const int64_t share = ceil_div(rest * kb, sharers);
+  const double saved = (kb - share) * block - (BN == 256 ? 10. + 0.1 * sharers : 2.5 + 0.08 * sharers);
+  if (saved > 0. && share >= 4) d = Deal{tiles, tiles - rest, (int)sharers, d.us - saved};
+  return d;
 }
 
 struct Operands {
@@ -720,7 +776,8 @@ int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
   prm.idesc = tc::instr_desc(1, 0, 0, kBM, BN);
   const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
   LLMQRT_REQUIRE(tiles <= 0x7fffffffll / kMaxCluster, "fp8 block linear: too many tiles");
-  prm.splits = pick_splits(tiles, prm.k_blocks, split_clusters<BN>(), nullptr);
+  int waves;
+  prm.splits = pick_splits(tiles, prm.k_blocks, split_clusters<BN>(), &waves);
   CUtensorMap tm_w, tm_a;
   if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, kBM)) return rc;
   if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, BN)) return rc;
@@ -733,37 +790,18 @@ int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
   return check_launch("fp8 block linear");
 }
 
-// Clusters to launch, and how many tiles are dealt out whole.  What is left over of the whole waves is shared out by K blocks where
-// that saves more of them than the sums through the workspace cost; every share has a few, and a tile few shares.  (Shares begin
-// anywhere in K: the more clusters work like that, the less of the operands they find in L2.  Together with one of the waves, for
-// shares of one size, 4096 x 3584 x 18944 took 261 us.)
-constexpr int kShareCost = 20;                         // K blocks
-constexpr int kLeastShare = 4, kMostShares = 6;
-int deal_out(int64_t tiles, int clusters, BlockParams& prm) {
-  const int64_t rest = tiles % clusters, kb = prm.k_blocks;
-  prm.whole_tiles = (int)tiles;
-  prm.sharers = 0;
-  if (rest && prm.partials && clusters <= kMaxPairs) {
-    const int64_t sharers = std::min({(int64_t)clusters, rest * kb / kLeastShare, rest * kMostShares});
-    if (sharers > rest && kb - ceil_div(rest * kb, sharers) >= kShareCost && rest * 16 <= LLMQRT_WS_NUM_COUNTERS && rest * kb <= 0x7fffffffll) {
-      prm.whole_tiles = (int)(tiles - rest);
-      prm.sharers = (int)sharers;
-      return (int)(tiles > rest ? clusters : sharers);
-    }
-  }
-  return (int)std::min(tiles, (int64_t)clusters);
-}
-
 template <int BN>
-int launch_pair(const Operands& o, BlockParams prm, cudaStream_t st) {
+int launch_pair(const Operands& o, BlockParams prm, Deal deal, cudaStream_t st) {
   const int clusters = pair_clusters<BN>();
   if (clusters <= 0) return set_error(LLMQRT_ERR_CUDA, "fp8 block linear: no cluster of two CTAs fits on this device");
   prm.tiles_p = (int)ceil_div(prm.M, 2 * kBM);
   prm.tiles_q = (int)ceil_div(prm.N, BN);
   prm.idesc = tc::instr_desc(1, 0, 0, 2 * kBM, kAccCols);
-  const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
-  LLMQRT_REQUIRE(tiles <= 0x7fffffffll, "fp8 block linear: too many tiles");
-  const int grid = deal_out(tiles, clusters, prm);
+  LLMQRT_REQUIRE(deal.tiles <= 0x7fffffffll, "fp8 block linear: too many tiles");
+  if (deal.sharers > clusters) deal = Deal{deal.tiles, deal.tiles, 0, 0.};      // (a device that does not hold a cluster on every two SMs)
+  prm.whole_tiles = (int)deal.whole;
+  prm.sharers = deal.sharers;
+  const int grid = (int)std::max((int64_t)deal.sharers, std::min(deal.whole, (int64_t)clusters));
   prm.tma_out = (reinterpret_cast<uintptr_t>(prm.out) & 15) == 0 && prm.ldo % 8 == 0;
   CUtensorMap tm_a, tm_w, tm_out;
   if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, kBM)) return rc;
@@ -814,7 +852,14 @@ extern "C" int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint
   if (M <= 32) return launch_split<32>(o, p, st);
   if (M <= 64) return launch_split<64>(o, p, st);
   if (M <= 128) return launch_split<128>(o, p, st);
-  const int64_t rows = ceil_div(M, 2 * kBM), clusters = sm_count() / 2;
-  if (rows * ceil_div(N, 256) >= clusters) return launch_pair<256>(o, p, st);
-  return launch_pair<128>(o, p, st);
+  const Deal wide = deal_out<256>(M, N, p.k_blocks, workspace != nullptr), narrow = deal_out<128>(M, N, p.k_blocks, workspace != nullptr);
+  const double pair = std::min(wide.us, narrow.us);
+  // Few tiles and a long reduction: panels of 64 tokens with it shared out, where the last panel is not nearly empty (a box that lies
+  // mostly behind the tokens comes slowly).  130 x 300 x 3584 7.7 us, in pairs 12.1; 512 x 1536 x 3584 15.8 and 11.6.
+  if (M <= 512 && (M - 1) % 64 >= 15) {
+    int waves;
+    const int s = pick_splits(ceil_div(N, kBM) * ceil_div(M, 64), p.k_blocks, split_clusters<64>(), &waves);
+    if (s > 1 && 6. + waves * (0.45 * p.k_blocks / s + 2.5) < pair) return launch_split<64>(o, p, st);
+  }
+  return wide.us < narrow.us ? launch_pair<256>(o, p, wide, st) : launch_pair<128>(o, p, narrow, st);
 }
