@@ -19,7 +19,7 @@
 // Grid (splits, Hkv * row tiles, B).  A block merges its four warps in shared memory; splits of one sequence are merged by the
 // thread-block cluster that they form, or, where there are more than eight, by a second kernel from the workspace.
 // Page numbers outside the cache and rows behind the last key are not read (zeros take their place) and get no weight.
-#include <cstdlib>
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -30,7 +30,7 @@ namespace llmqrt {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 16 * kWarps;
-constexpr int kRing = 6;                               // stages of a warp, 16 keys each
+template <int D> constexpr int kv8_ring() { return D == 128 ? 3 : 5; }  // stages of a warp, 16 keys each
 constexpr int kSpan = 4096;                            // keys whose page numbers and scales a block holds at a time
 constexpr int kMaxPages = kSpan / 16 + 1;              // pages that these touch
 constexpr int kClusterMergeMaxLen = 8192;               // greatest bound whose splits a cluster merges although it would take more than eight
@@ -50,14 +50,22 @@ struct Kv8Args {
   const float* cos_tab;            // [table_rows, D / 2] or null
   const float* sin_tab;
   uint16_t* out;                   // [B, Sq, Hq, D]
-  float* part_o;                   // [B * Sq * Hq, splits, D]
-  float* part_ml;                  // [B * Sq * Hq, splits, 2]
-  int table_rows, Sq, Hq, Hkv, pages, page, max_len, chunk, splits, tiles, cluster;
+  float* part_o;                   // [Hkv * tiles, blocks, 2, ROWS, D]
+  float* part_ml;                  // [Hkv * tiles, blocks, 2, ROWS, 2]
+  int table_rows, B, Sq, Hq, Hkv, pages, page, max_len, tiles, cluster;
   float scale, softcap;
 };
 
-__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst_smem, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(take ? 16 : 0) : "memory");
+template <int OFF> __device__ __forceinline__ void cp_async_16(uint32_t dst_smem, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %2], 16;" ::"r"(dst_smem), "l"(src), "n"(OFF) : "memory");
+}
+template <int OFF> __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst_smem, const uint8_t* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %3], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(take ? 16 : 0), "n"(OFF) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint4 lds_16(uint32_t addr) {
   uint4 v;
@@ -69,14 +77,70 @@ __device__ __forceinline__ uint2 lds_8(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
+// An 8 x 8 matrix of 16-bit values, row lane / 4, columns 2 (lane % 4) and + 1, turned over.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float2 unpack_half(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <bool BF16> __device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  return BF16 ? pack_pair<__nv_bfloat16>(a, b) : pack_pair<__half>(a, b);
+}
 template <bool BF16> __device__ __forceinline__ uint16_t round_bits(float f) {
   if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(f));
   else return __half_as_ushort(__float2half_rn(f));
+}
+
+// Units of kStep keys of a sequence; one without keys counts as one (its rows of zeros are written).
+__device__ __forceinline__ int units_of(const Kv8Args& p, int b) { return max(1, (max(0, min(p.seqlens[b], p.max_len)) + kStep - 1) / kStep); }
+// Their number over sequences [b0, b1), by the whole block; `scan` has a word for each of its warps.
+__device__ __forceinline__ int64_t sum_units(const Kv8Args& p, int b0, int b1, int64_t* scan) {
+  int64_t n = 0;
+  for (int b = b0 + (int)threadIdx.x; b < b1; b += blockDim.x) n += units_of(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scan[threadIdx.x >> 5] = n;
+  __syncthreads();
+  n = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) n += scan[w];
+  return n;
+}
+// The sequence that unit `u` of all lies in, and which of the sequence's it is.
+__device__ __forceinline__ int find_unit(const Kv8Args& p, int64_t u, int64_t* scan, int& unit) {
+  __shared__ int found[2];
+  int64_t before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    const int b = b0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = b < p.B ? units_of(p, b) : 0;
+    int64_t s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = s;
+    __syncthreads();
+    int64_t base = before;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += scan[w];
+      before += scan[w];
+    }
+    if (u >= base + s - n && u < base + s) {
+      found[0] = b;
+      found[1] = (int)(u - (base + s - n));
+    }
+    if (u < before) break;                             // (the whole block)
+  }
+  __syncthreads();
+  unit = found[1];
+  return found[0];
 }
 
 // Where a 16-byte chunk of a key's or a value's row lies in its tile of 16 rows, so that the fragment loads below meet no bank
@@ -93,27 +157,41 @@ template <int D> __device__ __forceinline__ uint32_t v_offset(int row, int chunk
 
 // ROWS: rows of queries that a block's tile holds, 8 or 16.
 template <int D, bool INT8, bool BF16, int ROWS>
-__global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args p) {
+__global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 2 : 3) attn_decode_kv8_kernel(const Kv8Args p) {
   constexpr int NJ = D / 64;                           // 16-byte pieces of a key's row a lane takes
   constexpr int NE = D / 8;                            // columns of the output a lane's V pieces hold
   constexpr int TILE = 16 * D, STAGE = 2 * TILE;
   constexpr bool REST = !BF16;                         // Q's and P's remainders take part
   constexpr int G = ROWS / 8;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int page_id[kMaxPages];
-  __shared__ float page_ks[kMaxPages], page_vs[kMaxPages];
+  __shared__ float4 pages[kMaxPages];                  // number (bits; -1: none), key scale, value scale
   pdl_wait();
   pdl_trigger();
-  const int split = blockIdx.x, hkv = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles, b = blockIdx.z;
+  const int hkv = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles;
   const int rep = p.Hq / p.Hkv, rows = p.Sq * rep;
-  const int L_raw = p.seqlens[b], L = max(0, min(L_raw, p.max_len));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  // A cluster's blocks share out the sequence's own length: the bound may be many times as long.
-  int chunk = p.chunk;
-  if (p.cluster > 1) chunk = max(kStep, ((L + p.cluster - 1) / p.cluster + kStep - 1) / kStep * kStep);
-  const int key_begin = min(split * chunk, L), key_end = min(L, key_begin + chunk);
-  if (p.cluster == 1 && key_begin >= key_end && split > 0) return;
-  const int n_splits = max(1, (L + chunk - 1) / chunk);
+  // The block's share: a cluster's blocks have a sequence's keys between them, otherwise every block of a KV head has as many units
+  // of kStep keys of all sequences together.
+  int b, unit;
+  int64_t units_left;
+  if (p.cluster > 1) {
+    b = blockIdx.z;
+    const int n = units_of(p, b), each = (n + p.cluster - 1) / p.cluster;
+    unit = min((int)blockIdx.x * each, n);
+    units_left = min(each, n - unit);
+  } else {
+    __shared__ int64_t scan[kWarps];
+    const int64_t total = sum_units(p, 0, p.B, scan), shares = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= shares) return;
+    const int64_t first = blockIdx.x * total / shares;
+    units_left = (blockIdx.x + 1) * total / shares - first;
+    b = find_unit(p, first, scan, unit);
+  }
+  for (bool more = true; more;) {
+  const int L_raw = p.seqlens[b], L = max(0, min(L_raw, p.max_len)), n_units = units_of(p, b);
+  const int unit_end = (int)min((int64_t)n_units, unit + units_left);
+  const bool whole = unit == 0 && unit_end == n_units;
+  const int key_begin = min(unit * kStep, L), key_end = min(L, unit_end * kStep);
 
   // ---- page numbers and scales of the keys from span_begin on ----
   const int shift = __ffs(p.page) - 1;
@@ -123,28 +201,51 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
     for (int i = tid; i < n; i += kThreads) {
       const int id = p.table[(int64_t)b * p.table_stride + page0 + i];
       const bool good = id >= 0 && id < p.pages;
-      page_id[i] = good ? id : -1;
-      page_ks[i] = good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f;
-      page_vs[i] = good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f;
+      pages[i] = make_float4(__int_as_float(good ? id : -1), good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f,
+                             good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f, 0.f);
     }
     __syncthreads();
   };
   load_pages();
 
   // ---- the ring's first stages ----
+  // A lane's pieces of a tile are 512 bytes apart in both memories; their swizzle is one of two.
+  constexpr int kRing = kv8_ring<D>();
+  constexpr int CPR = D / 16, kPieces = CPR / 2;       // 16-byte pieces of a row, and of a lane
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * kRing * STAGE);
+  const uint32_t k_dst = k_offset<D>(lane / CPR, lane % CPR);
+  const uint32_t v_dst0 = v_offset<D>(lane / CPR, lane % CPR), v_dst1 = v_offset<D>(lane / CPR + 32 / CPR, lane % CPR) - 512u;
   auto issue = [&](int key0, int stage) {
     if (key0 < span_end) {
-      constexpr int CPR = D / 16;
       const uint32_t base = ring + (uint32_t)(stage * STAGE);
-      const int id = page_id[(key0 >> shift) - page0];
-      const int64_t at = (int64_t)max(id, 0) * p.page_stride + (int64_t)hkv * p.head_stride + (int64_t)(key0 & (p.page - 1)) * D;
-#pragma unroll
-      for (int i = 0; i < 16 * CPR / 32; ++i) {
-        const int n = i * 32 + lane, r = n / CPR, c = n % CPR;
-        const bool take = id >= 0 && key0 + r < span_end;
-        cp_async_16_or_zero(base + k_offset<D>(r, c), p.k_cache + at + n * 16, take);
-        cp_async_16_or_zero(base + TILE + v_offset<D>(r, c), p.v_cache + at + n * 16, take);
+      const int id = __float_as_int(pages[(key0 >> shift) - page0].x);
+      const int64_t at = (int64_t)max(id, 0) * p.page_stride + (int64_t)hkv * p.head_stride + (int64_t)(key0 & (p.page - 1)) * D + lane * 16;
+      const uint8_t* ks = p.k_cache + at;
+      const uint8_t* vs = p.v_cache + at;
+      const uint32_t kd = base + k_dst, v0 = base + TILE + v_dst0, v1 = base + TILE + v_dst1;
+      if (id >= 0 && key0 + 16 <= span_end) {
+        cp_async_16<0>(kd, ks);
+        cp_async_16<0>(v0, vs);
+        cp_async_16<512>(kd, ks);
+        cp_async_16<512>(v1, vs);
+        if constexpr (kPieces == 4) {
+          cp_async_16<1024>(kd, ks);
+          cp_async_16<1024>(v0, vs);
+          cp_async_16<1536>(kd, ks);
+          cp_async_16<1536>(v1, vs);
+        }
+      } else {                                         // zeros for the rows that are not there
+        const int left = id >= 0 ? span_end - key0 - lane / CPR : 0;
+        cp_async_16_or_zero<0>(kd, ks, 0 < left);
+        cp_async_16_or_zero<0>(v0, vs, 0 < left);
+        cp_async_16_or_zero<512>(kd, ks, 32 / CPR < left);
+        cp_async_16_or_zero<512>(v1, vs, 32 / CPR < left);
+        if constexpr (kPieces == 4) {
+          cp_async_16_or_zero<1024>(kd, ks, 64 / CPR < left);
+          cp_async_16_or_zero<1024>(v0, vs, 64 / CPR < left);
+          cp_async_16_or_zero<1536>(kd, ks, 96 / CPR < left);
+          cp_async_16_or_zero<1536>(v1, vs, 96 / CPR < left);
+        }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");          // (always: the groups are counted)
@@ -157,43 +258,54 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
 
   // ---- Q: rows g and g + 8 of the tile; register 2i, 2i + 1 of a piece are the MMA's k slots 2t and 2t + 8 of step i ----
   uint32_t qa[G][NJ][8], qr[G][NJ][8];                 // fp16 and what it leaves over
-  float row_scale[G];
-  int sees[G];                                         // keys that the row's token sees
+  float scale_q[G][2];                                 // of rows 2t and 2t + 1, which the lane has scores of
+  int sees[G][2];                                      // keys that these rows' tokens see
 #pragma unroll
   for (int h = 0; h < G; ++h) {
     const int r = tile * ROWS + h * 8 + g;
     const bool on = r < rows;
     const int s = on ? r / rep : 0, head = hkv * rep + (on ? r - s * rep : 0);
-    sees[h] = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
+    const int sees_g = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
     const int angle = L_raw - p.Sq + s;
     const bool rotate = p.cos_tab != nullptr && angle >= 0 && angle < p.table_rows;
     const uint16_t* src = p.q + (int64_t)b * p.q_batch_stride + (int64_t)s * p.q_token_stride + (int64_t)head * D;
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    float x[NJ][16], other[NJ][16];                    // this lane's elements 16 (4j + t) .. + 15, and those they are rotated with
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int d0 = 16 * (4 * j + t), d1 = (d0 + D / 2) % D;
+    float x[NJ][16];                                   // this lane's elements 16 (4j + t) .. + 15
+    auto piece = [&](int d0, float (&y)[16]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0), w = v;
-        if (on) {
-          v = *reinterpret_cast<const uint4*>(src + d0 + 8 * i);
-          if (rotate) w = *reinterpret_cast<const uint4*>(src + d1 + 8 * i);
-        }
-        const uint32_t vw[4] = {v.x, v.y, v.z, v.w}, ww[4] = {w.x, w.y, w.z, w.w};
+        const uint4 v = on ? *reinterpret_cast<const uint4*>(src + d0 + 8 * i) : make_uint4(0, 0, 0, 0);
+        const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 a = unpack_pair<T>(vw[e]), c = unpack_pair<T>(ww[e]);
-          x[j][8 * i + 2 * e] = a.x; x[j][8 * i + 2 * e + 1] = a.y;
-          other[j][8 * i + 2 * e] = c.x; other[j][8 * i + 2 * e + 1] = c.y;
+          const float2 a = unpack_pair<T>(vw[e]);
+          y[8 * i + 2 * e] = a.x; y[8 * i + 2 * e + 1] = a.y;
         }
       }
-      if (rotate) {
-        const bool low = d0 < D / 2;
-        const float* cr = p.cos_tab + (int64_t)angle * (D / 2) + d0 % (D / 2);
-        const float* sr = p.sin_tab + (int64_t)angle * (D / 2) + d0 % (D / 2);
+    };
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[j][e] = low ? x[j][e] * cr[e] - other[j][e] * sr[e] : other[j][e] * sr[e] + x[j][e] * cr[e];
+    for (int j = 0; j < NJ; ++j) piece(16 * (4 * j + t), x[j]);
+    if (rotate) {                                      // pairs lie half a head apart: with d = 128 in the lane's own two pieces
+      const int i0 = D == 128 ? 16 * t : 16 * (t & 1);
+      const float4* cr = reinterpret_cast<const float4*>(p.cos_tab + (int64_t)angle * (D / 2) + i0);
+      const float4* sr = reinterpret_cast<const float4*>(p.sin_tab + (int64_t)angle * (D / 2) + i0);
+      float other[16];
+      if constexpr (D == 64) piece((16 * t + 32) % 64, other);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 c4 = __ldg(cr + k), s4 = __ldg(sr + k);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (D == 128) {
+            const float lo = x[0][4 * k + e], hi = x[1][4 * k + e];
+            x[0][4 * k + e] = lo * c[e] - hi * sn[e];
+            x[1][4 * k + e] = lo * sn[e] + hi * c[e];
+          } else {
+            const float own = x[0][4 * k + e], far = other[4 * k + e];
+            x[0][4 * k + e] = t < 2 ? own * c[e] - far * sn[e] : far * sn[e] + own * c[e];
+          }
+        }
       }
     }
     // fp16 keeps 11 bits between 2^-14 and 65504: the row's maximum goes to [2^13, 2^14)
@@ -206,31 +318,48 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);      // (an infinity or a NaN stays what it is)
     const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-    row_scale[h] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale;
+    const float scale_g = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale * (p.softcap != 0.f ? 1.f : kLog2e);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      scale_q[h][c] = __shfl_sync(0xffffffffu, scale_g, 4 * (2 * t + c));
+      sees[h][c] = __shfl_sync(0xffffffffu, sees_g, 4 * (2 * t + c));
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = x[j][2 * e] * up, c = x[j][2 * e + 1] * up;
         qa[h][j][e] = pack_half(a, c);
-        if (REST) {
+        if constexpr (REST) {
           const float2 f = unpack_half(qa[h][j][e]);
           qr[h][j][e] = pack_half(a - f.x, c - f.y);
         }
       }
   }
 
-  float o[NE][4];                                      // ROWS 8: c0, c1 of P's fp16 part, c2, c3 of the rest; 16: rows g and g + 8
+  float o[NE / 2][G][4];                               // columns 2e and 2e + 1 of the lane's NE, rows 2t and 2t + 1 each
 #pragma unroll
-  for (int e = 0; e < NE; ++e)
+  for (int e = 0; e < NE / 2; ++e)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[e][c] = 0.f;
-  float m_run[G], l_run[G], v_ref = 0.f;
+    for (int h = 0; h < G; ++h)
 #pragma unroll
-  for (int h = 0; h < G; ++h) {
-    m_run[h] = -INFINITY;
-    l_run[h] = 0.f;
-  }
+      for (int c = 0; c < 4; ++c) o[e][h][c] = 0.f;
+  // The reference that a row's scores are taken against moves only when one exceeds it by more than 2^kSlack: P is then at most
+  // that, fp16 rounds it all the same, and most steps need no maximum over the lanes and leave O and the sums alone.
+  // (kLift takes P to the upper end of fp16's range, 2^15: a page whose scale is 2^-20 of the greatest one keeps some bits.)
+  constexpr float kSlack = 6.f, kLift = 512.f, kNothing = -1e30f;
+  float m_run[G][2], l_run[G][2], v_ref = 0.f, v_inv = 0.f;
+  int sees_all = 0x7fffffff;                           // keys that every row of the tile sees
+#pragma unroll
+  for (int h = 0; h < G; ++h)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      m_run[h][c] = kNothing;
+      l_run[h][c] = 0.f;
+      sees_all = min(sees_all, tile * ROWS + h * 8 + 2 * t + c < rows ? sees[h][c] : 0x7fffffff);
+    }
+#pragma unroll
+  for (int o_ = 16; o_ > 0; o_ >>= 1) sees_all = min(sees_all, __shfl_xor_sync(0xffffffffu, sees_all, o_));
 
   for (;;) {
     int it = 0;
@@ -240,92 +369,115 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
       __syncwarp();
       const uint32_t st = ring + (uint32_t)((it % kRing) * STAGE);
       const int pi = (key0 >> shift) - page0;
-      const float ks = page_ks[pi], vs = page_vs[pi];
-      const bool good = page_id[pi] >= 0;
+      const float4 info = pages[pi];
+      const float ks = info.y, vs = info.z;
+      const bool good = __float_as_int(info.x) >= 0;
 
-      // ---- S = Q K^T for 16 keys: this lane gets keys 8 nb + 2t, + 1 of rows g (and g + 8) ----
-      float s_acc[2][4];
+      // ---- S^T = K Q^T: this lane gets keys g and g + 8 of rows 2t and 2t + 1 ----
+      float s_acc[G][NJ][4];
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
+      for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s_acc[nb][c] = 0.f;
+        for (int h = 0; h < G; ++h)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const uint4 kw = lds_16(st + k_offset<D>(8 * nb + g, 4 * j + t));
-          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+          for (int c = 0; c < 4; ++c) s_acc[h][j][c] = 0.f;
+        const uint4 k0 = lds_16(st + k_offset<D>(g, 4 * j + t)), k1 = lds_16(st + k_offset<D>(8 + g, 4 * j + t));
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t lo, hi;
-            kv8_word_to_half<INT8>(w[i], lo, hi);
-            if constexpr (ROWS == 8) {
-              mma_16816<false>(s_acc[nb], qa[0][j][2 * i], REST ? qr[0][j][2 * i] : 0u, qa[0][j][2 * i + 1], REST ? qr[0][j][2 * i + 1] : 0u, lo, hi);
-            } else {
-              mma_16816<false>(s_acc[nb], qa[0][j][2 * i], qa[1][j][2 * i], qa[0][j][2 * i + 1], qa[1][j][2 * i + 1], lo, hi);
-              if (REST) mma_16816<false>(s_acc[nb], qr[0][j][2 * i], qr[1][j][2 * i], qr[0][j][2 * i + 1], qr[1][j][2 * i + 1], lo, hi);
-            }
+        for (int i = 0; i < 4; ++i) {
+          uint32_t a0, a1, a2, a3;
+          kv8_word_to_half<INT8>(w0[i], a0, a2);
+          kv8_word_to_half<INT8>(w1[i], a1, a3);
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            mma_16816<false>(s_acc[h][j], a0, a1, a2, a3, qa[h][j][2 * i], qa[h][j][2 * i + 1]);
+            if constexpr (REST) mma_16816<false>(s_acc[h][j], a0, a1, a2, a3, qr[h][j][2 * i], qr[h][j][2 * i + 1]);
           }
         }
       }
 
       // ---- running softmax ----
-      float pv[G][2][2], corr[G];
-      const float ref_new = fmaxf(v_ref, vs), share = ref_new > 0.f ? __fdividef(vs, ref_new) : 0.f;
-      bool moved = ref_new != v_ref;
-      const float ref_corr = ref_new > 0.f ? __fdividef(v_ref, ref_new) : 0.f;
-#pragma unroll
-      for (int h = 0; h < G; ++h) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float s = ROWS == 8 ? (REST ? s_acc[nb][c] + s_acc[nb][c + 2] : s_acc[nb][c]) : s_acc[nb][2 * h + c];
-            s *= ks * row_scale[h];
-            if (p.softcap != 0.f) s = p.softcap * tanhf(s / p.softcap);
-            s *= kLog2e;
-            if (!good || key0 + 8 * nb + 2 * t + c >= sees[h]) s = -INFINITY;
-            pv[h][nb][c] = s;
-            mx = fmaxf(mx, s);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[h], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-        moved |= m_new != m_run[h];
-        corr[h] = exp2f(m_run[h] - m_use);
-        m_run[h] = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            pv[h][nb][c] = exp2f(pv[h][nb][c] - m_use);
-            sum += pv[h][nb][c];
-            pv[h][nb][c] *= share;
-          }
-        l_run[h] = l_run[h] * corr[h] + sum;
-        corr[h] *= ref_corr;
-      }
-      v_ref = ref_new;
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          o[e][0] *= corr[0]; o[e][1] *= corr[0];
-          if (ROWS == 16 || REST) { o[e][2] *= corr[G - 1]; o[e][3] *= corr[G - 1]; }
-        }
-      }
-      uint32_t pa[G][2], pr[G][2];                       // key slots 2t, 2t + 1 and 2t + 8, 2t + 9
+      float pv[G][2][2];                                 // [.][key g, key g + 8][row]
+      bool beyond = false;
 #pragma unroll
       for (int h = 0; h < G; ++h)
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          pa[h][nb] = pack_half(pv[h][nb][0], pv[h][nb][1]);
-          if (REST) {
-            const float2 f = unpack_half(pa[h][nb]);
-            pr[h][nb] = pack_half(pv[h][nb][0] - f.x, pv[h][nb][1] - f.y);
+        for (int c = 0; c < 2; ++c) {
+          const float f = ks * scale_q[h][c];
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            float s = s_acc[h][0][2 * kb + c];
+            if constexpr (NJ == 2) s += s_acc[h][1][2 * kb + c];
+            pv[h][kb][c] = s * f;
+          }
+        }
+      if (p.softcap != 0.f) {
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pv[h][i >> 1][i & 1] = p.softcap * tanhf(pv[h][i >> 1][i & 1] / p.softcap) * kLog2e;
+      }
+      if (!good || key0 + 16 > sees_all) {
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!good || key0 + 8 * (i >> 1) + g >= sees[h][i & 1]) pv[h][i >> 1][i & 1] = -INFINITY;
+      }
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) beyond |= fmaxf(pv[h][0][c], pv[h][1][c]) > m_run[h][c] + kSlack;
+      if (__any_sync(0xffffffffu, beyond) || vs > v_ref) {
+        const float ref_corr = vs > v_ref ? v_ref / vs : 1.f;
+        if (vs > v_ref) {
+          v_ref = vs;
+          v_inv = kLift / vs;
+        }
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(pv[h][0][c], pv[h][1][c]);
+#pragma unroll
+            for (int o_ = 4; o_ < 32; o_ <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o_));
+            const float m_new = fmaxf(m_run[h][c], mx);
+            float corr = ex2(m_run[h][c] - m_new);
+            m_run[h][c] = m_new;
+            l_run[h][c] *= corr;
+            corr *= ref_corr;
+#pragma unroll
+            for (int e = 0; e < NE / 2; ++e) {
+              o[e][h][c] *= corr;
+              o[e][h][c + 2] *= corr;
+            }
+          }
+      }
+      const float share = vs * v_inv;
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float e = ex2(pv[h][kb][c] - m_run[h][c]);
+            l_run[h][c] += e;
+            pv[h][kb][c] = e * share;
+          }
+      uint32_t pa[G][2], pr[G][2];                       // of row g: keys 2t, 2t + 1 and 2t + 8, 2t + 9
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint32_t whole_p = pack_half(pv[h][kb][0], pv[h][kb][1]);
+          pa[h][kb] = transpose_8x8(whole_p);
+          if constexpr (REST) {
+            const float2 f = unpack_half(whole_p);
+            pr[h][kb] = transpose_8x8(pack_half(pv[h][kb][0] - f.x, pv[h][kb][1] - f.y));
           }
         }
 
-      // ---- O += P V: a lane holds d = NE g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9 ----
+      // ---- O^T += V^T P^T: a lane holds d = NE g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9 ----
       uint32_t vw[4][NE / 4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -339,6 +491,49 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
         }
       }
       __syncwarp();                                      // every lane has read the stage: it may be filled again
+      // A NaN among the values is for the rows that see its key alone (0 * NaN is not 0): it leaves the product, and the rows and
+      // columns that it belongs to are counted by a product of their own.
+      if (!INT8 && key0 + 16 > sees_all) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int w = 0; w < NE / 4; ++w) any |= __vcmpeq4(vw[s][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+        if (__any_sync(0xffffffffu, any != 0)) {
+          uint32_t seen[G][2];
+#pragma unroll
+          for (int h = 0; h < G; ++h)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+              const int k = key0 + 8 * kb + g;
+              seen[h][kb] = transpose_8x8((k < sees[h][0] ? 0x3c00u : 0u) | (k < sees[h][1] ? 0x3c000000u : 0u));
+            }
+#pragma unroll
+          for (int w = 0; w < NE / 4; ++w) {
+            uint32_t one[4], b0[4], b1[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              const uint32_t m = __vcmpeq4(vw[s][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              one[s] = m & 0x38383838u;                  // (1 in e4m3)
+              vw[s][w] &= ~m;
+            }
+            kv8_word_to_half<INT8>(__byte_perm(one[0], one[1], 0x5140), b0[0], b0[1]);
+            kv8_word_to_half<INT8>(__byte_perm(one[0], one[1], 0x7362), b0[2], b0[3]);
+            kv8_word_to_half<INT8>(__byte_perm(one[2], one[3], 0x5140), b1[0], b1[1]);
+            kv8_word_to_half<INT8>(__byte_perm(one[2], one[3], 0x7362), b1[2], b1[3]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+#pragma unroll
+              for (int h = 0; h < G; ++h) {
+                float n[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_16816<false>(n, b0[e], b0[e + 1], b1[e], b1[e + 1], seen[h][0], seen[h][1]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (n[c] > 0.f) o[2 * w + e / 2][h][c] = __int_as_float(0x7fffffff);
+              }
+          }
+        }
+      }
 #pragma unroll
       for (int w = 0; w < NE / 4; ++w) {
         uint32_t b0[4], b1[4];
@@ -347,15 +542,12 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
         kv8_word_to_half<INT8>(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
         kv8_word_to_half<INT8>(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float(&acc)[4] = o[4 * w + e];
-          if constexpr (ROWS == 8) {
-            mma_16816<false>(acc, pa[0][0], REST ? pr[0][0] : 0u, pa[0][1], REST ? pr[0][1] : 0u, b0[e], b1[e]);
-          } else {
-            mma_16816<false>(acc, pa[0][0], pa[1][0], pa[0][1], pa[1][1], b0[e], b1[e]);
-            if (REST) mma_16816<false>(acc, pr[0][0], pr[1][0], pr[0][1], pr[1][1], b0[e], b1[e]);
+        for (int e = 0; e < 4; e += 2)
+#pragma unroll
+          for (int h = 0; h < G; ++h) {
+            mma_16816<false>(o[2 * w + e / 2][h], b0[e], b0[e + 1], b1[e], b1[e + 1], pa[h][0], pa[h][1]);
+            if constexpr (REST) mma_16816<false>(o[2 * w + e / 2][h], b0[e], b0[e + 1], b1[e], b1[e + 1], pr[h][0], pr[h][1]);
           }
-        }
       }
     }
 
@@ -370,72 +562,71 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
   }
 
   // ---- merge the warps ----
-  constexpr int kPitch = D + 4;                        // (rows of the tile start in different banks)
+  // A lane has NE neighbouring columns of two rows; every other lane's have their quarters of 32 bytes the other way round, so
+  // that eight lanes' 16 bytes meet no bank twice.
+  constexpr int kPitch = D + 4;
+  auto at = [](int dd) { return dd ^ ((dd / NE & 1) << 2); };
   float* sm_o = reinterpret_cast<float*>(smem);        // [kWarps][ROWS][kPitch]
   float* sm_m = sm_o + kWarps * ROWS * kPitch;         // [kWarps][ROWS]
   float* sm_l = sm_m + kWarps * ROWS;
   float* cl_o = sm_l + kWarps * ROWS;                  // [ROWS][D] and [ROWS][2]: for the cluster's merge
   float* cl_ml = cl_o + ROWS * D;
+  const float unlift = v_ref * (1.f / kLift);
 #pragma unroll
-  for (int h = 0; h < G; ++h) {
-    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
-    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
-    const int r = h * 8 + g;
-    if (t == 0) {
-      sm_m[warp * ROWS + r] = m_run[h];
-      sm_l[warp * ROWS + r] = l_run[h];
-    }
-    float* row = sm_o + (warp * ROWS + r) * kPitch;
+  for (int h = 0; h < G; ++h)
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const float a = ROWS == 16 ? o[e][2 * h] : REST ? o[e][0] + o[e][2] : o[e][0];
-      const float c = ROWS == 16 ? o[e][2 * h + 1] : REST ? o[e][1] + o[e][3] : o[e][1];
-      row[NE * (2 * t) + e] = a * v_ref;
-      row[NE * (2 * t + 1) + e] = c * v_ref;
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int o_ = 4; o_ < 32; o_ <<= 1) l_run[h][c] += __shfl_xor_sync(0xffffffffu, l_run[h][c], o_);
+      const int r = h * 8 + 2 * t + c;
+      if (g == 0) {
+        sm_m[warp * ROWS + r] = m_run[h][c] > kNothing ? m_run[h][c] : l_run[h][c] == 0.f ? -INFINITY : 0.f;      // (nothing but NaN stays NaN)
+        sm_l[warp * ROWS + r] = l_run[h][c];
+      }
+      float* row = sm_o + (warp * ROWS + r) * kPitch;
+#pragma unroll
+      for (int e = 0; e < NE / 2; e += 2)
+        *reinterpret_cast<float4*>(row + at(NE * g + 2 * e)) =
+            make_float4(unlift * o[e][h][c], unlift * o[e][h][c + 2], unlift * o[e + 1][h][c], unlift * o[e + 1][h][c + 2]);
     }
-  }
   __syncthreads();
   const int here = min(ROWS, rows - tile * ROWS);      // rows of this tile
   auto out_row = [&](int r) -> int64_t {
     const int rr = tile * ROWS + r, s = rr / rep;
     return ((int64_t)b * p.Sq + s) * p.Hq + hkv * rep + (rr - s * rep);
   };
-  for (int i = tid; i < here * D; i += kThreads) {
-    const int r = i / D, dd = i - r * D;
+  // (a block's first segment goes to its first slot, its last one to the second)
+  const int64_t slot = (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (unit > 0 ? 0 : 1)) * ROWS;
+  for (int i = tid; i < here * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), dd = i % (D / 4) * 4;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * ROWS + r]);
-    float lsum = 0.f, osum = 0.f;
+    float lsum = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (M > -INFINITY) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(sm_m[w * ROWS + r] - M);
+        const float f = ex2(sm_m[w * ROWS + r] - M);
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + r) * kPitch + at(dd));
         lsum += sm_l[w * ROWS + r] * f;
-        osum += sm_o[(w * ROWS + r) * kPitch + dd] * f;
+        sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
       }
     }
-    if (p.cluster > 1) {
-      cl_o[i] = osum;
-      if (dd == 0) {
-        cl_ml[2 * r] = M;
-        cl_ml[2 * r + 1] = lsum;
-      }
-    } else if (n_splits == 1) {
-      p.out[out_row(r) * D + dd] = round_bits<BF16>(lsum > 0.f ? osum / lsum : 0.f);
+    if (p.cluster > 1 || !whole) {
+      float* po = p.cluster > 1 ? cl_o + r * D + dd : p.part_o + (slot + r) * D + dd;
+      *reinterpret_cast<float4*>(po) = sum;
+      if (dd == 0) *reinterpret_cast<float2*>(p.cluster > 1 ? cl_ml + 2 * r : p.part_ml + 2 * (slot + r)) = make_float2(M, lsum);
     } else {
-      const int64_t slot = out_row(r) * p.splits + split;
-      p.part_o[slot * D + dd] = osum;
-      if (dd == 0) {
-        p.part_ml[2 * slot] = M;
-        p.part_ml[2 * slot + 1] = lsum;
-      }
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      *reinterpret_cast<uint2*>(p.out + out_row(r) * D + dd) = make_uint2(round_pair<BF16>(sum.x * inv, sum.y * inv), round_pair<BF16>(sum.z * inv, sum.w * inv));
     }
   }
   if (p.cluster > 1) {
     cluster_arrive();
     cluster_wait();
     const uint32_t lo = (uint32_t)__cvta_generic_to_shared(cl_o), lml = (uint32_t)__cvta_generic_to_shared(cl_ml);
-    for (int i = split * kThreads + tid; i < here * D; i += p.cluster * kThreads) {
+    for (int i = blockIdx.x * kThreads + tid; i < here * D; i += p.cluster * kThreads) {
       const int r = i / D, dd = i - r * D;
       float pm[8], pl[8], po[8], M = -INFINITY;
 #pragma unroll
@@ -460,42 +651,79 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kv8_kernel(const Kv8Args
           osum += po[c] * f;
         }
       }
-      p.out[out_row(r) * D + dd] = round_bits<BF16>(lsum > 0.f ? osum / lsum : 0.f);
+      p.out[out_row(r) * D + dd] = round_bits<BF16>(lsum == 0.f ? 0.f : osum / lsum);
     }
     cluster_arrive();                                  // nobody leaves while a peer may still read its partial
     cluster_wait();
+    return;
+  }
+  units_left -= unit_end - unit;
+  more = units_left > 0;
+  ++b;
+  unit = 0;
+  __syncthreads();                                     // (the merge has been read: its memory is the rings')
   }
 }
 
-// Merge of the splits that the workspace holds: a thread adds up four neighbouring outputs.
-template <bool BF16, int D>
-__global__ void __launch_bounds__(128) attn_decode_kv8_merge_kernel(const Kv8Args p) {
+// Merge of the sequences that several blocks have had a part of.  `each` warps (1 .. 16) add up a row's parts, every each-th one, and are
+// joined in shared memory; a lane has D / 32 neighbouring outputs.  (All parts in one thread's loop: one sequence of 131072 keys
+// in 256 parts took 100 us.)
+template <bool BF16, int D, int ROWS>
+__global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Args p, int blocks, int each) {
+  constexpr int W = D / 32;
+  __shared__ float sm_o[16][D];
+  __shared__ float2 sm_ml[16];
+  __shared__ int64_t scan[16];
   pdl_wait_then_trigger();
-  const int b = blockIdx.y, u = blockIdx.x * 128 + threadIdx.x, units = p.Sq * p.Hq * (D / 4);
-  const int n_splits = (max(0, min(p.seqlens[b], p.max_len)) + p.chunk - 1) / p.chunk;
-  if (n_splits <= 1 || u >= units) return;             // (one split: the result is there)
-  const int64_t row = (int64_t)b * p.Sq * p.Hq + u / (D / 4);
-  const int dd = u % (D / 4) * 4;
-  float M = -INFINITY, lsum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < n_splits; ++s) {                 // in split order
-    const int64_t slot = row * p.splits + s;
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + dd));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp & (each - 1);
+  const int b = blockIdx.y, r = blockIdx.x * ((int)(blockDim.x >> 5) / each) + warp / each;
+  // which blocks had a part
+  const int64_t before = sum_units(p, 0, b, scan), total = before + sum_units(p, b, p.B, scan);
+  const int64_t shares = min((int64_t)blocks, total);
+  const int first = (int)(((before + 1) * shares - 1) / total), last = (int)(((before + units_of(p, b)) * shares - 1) / total);
+  if (first == last) return;                           // (one: the result is there)
+  const bool on = r < p.Sq * p.Hq;
+  const int s = on ? r / p.Hq : 0, head = on ? r - s * p.Hq : 0, rep = p.Hq / p.Hkv, hkv = head / rep, tr = s * rep + head - hkv * rep;
+  const int64_t column = (int64_t)(hkv * p.tiles + tr / ROWS) * blocks;
+  float M = -INFINITY, lsum = 0.f, o[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) o[j] = 0.f;
+  auto join = [&](float2 ml, const float* v) {
     const float Mn = fmaxf(M, ml.x);
-    const float keep = M > -INFINITY ? exp2f(M - Mn) : 0.f, f = ml.x > -INFINITY ? exp2f(ml.x - Mn) : 0.f;
+    const float keep = M > -INFINITY ? ex2(M - Mn) : 0.f, f = ml.x > -INFINITY ? ex2(ml.x - Mn) : 0.f;
     M = Mn;
     lsum = lsum * keep + ml.y * f;
-    o[0] = o[0] * keep + a.x * f; o[1] = o[1] * keep + a.y * f;
-    o[2] = o[2] * keep + a.z * f; o[3] = o[3] * keep + a.w * f;
-  }
-  uint16_t e[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) e[j] = round_bits<BF16>(lsum > 0.f ? o[j] / lsum : 0.f);
-  *reinterpret_cast<uint2*>(p.out + row * D + dd) = make_uint2(e[0] | ((uint32_t)e[1] << 16), e[2] | ((uint32_t)e[3] << 16));
+    for (int j = 0; j < W; ++j) o[j] = o[j] * keep + v[j] * f;
+  };
+  if (on) {
+#pragma unroll 4
+    for (int k = first + part; k <= last; k += each) { // in the blocks' order
+      // (a block that begins in the middle of the sequence has it in its first slot)
+      const int64_t slot = ((column + k) * 2 + (k * total / shares > before ? 0 : 1)) * ROWS + tr % ROWS;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
+      float v[W];
+      if constexpr (W == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + lane * W));
+      else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(p.part_o + slot * D + lane * W));
+      join(ml, v);
+    }
+  }
+  if (each > 1) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) sm_o[warp][lane * W + j] = o[j];
+    if (lane == 0) sm_ml[warp] = make_float2(M, lsum);
+    __syncthreads();
+    if (part != 0 || !on) return;
+    for (int w = 1; w < each; ++w) join(sm_ml[warp + w], &sm_o[warp + w][lane * W]);
+  }
+  if (!on) return;
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  uint16_t* dst = p.out + ((int64_t)b * p.Sq * p.Hq + r) * D + lane * W;
+  if constexpr (W == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(round_pair<BF16>(o[0] * inv, o[1] * inv), round_pair<BF16>(o[2] * inv, o[3] * inv));
+  else *reinterpret_cast<uint32_t*>(dst) = round_pair<BF16>(o[0] * inv, o[1] * inv);
 }
 
-template <int D> constexpr int kv8_smem() { return kWarps * kRing * 2 * 16 * D; }
+template <int D> constexpr int kv8_smem() { return kWarps * kv8_ring<D>() * 2 * 16 * D; }
 
 // Clusters of `cluster` blocks of a kernel that can be resident at once (asked once per device and kernel).
 int max_active_clusters(const void* kern, int cluster, int smem) {
@@ -533,39 +761,37 @@ int launch(Kv8Args a, int B, void* workspace, cudaStream_t st) {
   static_assert(smem >= (kWarps * ROWS * (D + 4 + 2) + ROWS * (D + 2)) * 4, "the rings hold the merge tile");
   auto kern = attn_decode_kv8_kernel<D, INT8, BF16, ROWS>;
   a.tiles = (int)ceil_div((int64_t)a.Sq * (a.Hq / a.Hkv), ROWS);
-  const int64_t blocks = (int64_t)B * a.Hkv * a.tiles, slots = 2 * (int64_t)sm_count();
-  const int most = a.max_len > 0 ? a.max_len : 1;
-  int chunk = kStep;
-  while (chunk < most && blocks * ceil_div(most, chunk) > slots) chunk *= 2;
-  if (chunk > 2048 && most > 4096) chunk = 2048;       // (ragged lengths: the longest sequence would run alone at the end)
-  int splits = (int)ceil_div(most, chunk);
-  a.cluster = 1;
-  if (splits > 1 && (splits <= 8 || most <= kClusterMergeMaxLen)) {
-    const int c = splits < 8 ? splits : 8;
-    if (blocks <= max_active_clusters(reinterpret_cast<const void*>(kern), c, smem)) {
-      a.cluster = splits = c;
-      chunk = (int)ceil_div(ceil_div(most, c), kStep) * kStep;
-    }
-  }
-  const size_t rows = (size_t)B * a.Sq * a.Hq;
-  while (a.cluster == 1 && splits > 1 && rows * splits * (D + 2) * 4 > LLMQRT_WS_PARTIAL_BYTES) {
-    chunk *= 2;
-    splits = (int)ceil_div(most, chunk);
-  }
-  a.chunk = chunk;
-  a.splits = splits;
-  if (splits > 1 && a.cluster == 1) {
-    if (!workspace) return set_error(LLMQRT_ERR_WORKSPACE, "attn_decode_kv8: split keys need the workspace");
-    a.part_o = reinterpret_cast<float*>(ws_partials(workspace));
-    a.part_ml = a.part_o + rows * splits * D;
-  }
+  a.B = B;
+  const int64_t columns = (int64_t)a.Hkv * a.tiles;    // blocks' shares are of one KV head and row tile each
+  const int slots = std::max(1, max_active_clusters(reinterpret_cast<const void*>(kern), 1, smem));
+  const int64_t units = ceil_div(a.max_len > 0 ? a.max_len : 1, kStep);
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
-  if (int rc = launch_chained(kern, dim3((unsigned)splits, (unsigned)(a.Hkv * a.tiles), (unsigned)B), dim3(kThreads), smem, st, a.cluster, a))
-    return rc;
+  // Few sequences that are not long: up to eight blocks for each, a cluster that merges their parts.  Otherwise all blocks that fit at
+  // once share the keys out evenly, whatever the lengths, and sequences with several parts are merged by a second kernel.
+  const int cluster = (int)std::min<int64_t>(8, units);
+  if (cluster > 1 && a.max_len <= kClusterMergeMaxLen && B * columns <= max_active_clusters(reinterpret_cast<const void*>(kern), cluster, smem)) {
+    a.cluster = cluster;
+    if (int rc = launch_chained(kern, dim3((unsigned)cluster, (unsigned)columns, (unsigned)B), dim3(kThreads), smem, st, cluster, a)) return rc;
+    return check_launch("attn_decode_kv8");
+  }
+  a.cluster = 1;
+  // (one wave of blocks; where a column has fewer than four of them, up to four waves, the last of which is rarely full)
+  const int64_t waves = columns * 4 <= slots ? 1 : 4;
+  const int blocks = (int)std::min(std::max<int64_t>(1, waves * slots / columns), B * units);
+  if (blocks > 1 && !workspace) return set_error(LLMQRT_ERR_WORKSPACE, "attn_decode_kv8: split keys need the workspace");
+  const size_t rows = (size_t)columns * blocks * 2 * ROWS;
+  if (blocks > 1 && rows * (D + 2) * 4 > LLMQRT_WS_PARTIAL_BYTES)
+    return set_error(LLMQRT_ERR_UNSUPPORTED, "attn_decode_kv8: the blocks' partial results do not fit the workspace");
+  a.part_o = blocks > 1 ? reinterpret_cast<float*>(ws_partials(workspace)) : nullptr;
+  a.part_ml = a.part_o + rows * D;
+  if (int rc = launch_chained(kern, dim3((unsigned)blocks, (unsigned)columns, 1), dim3(kThreads), smem, st, 1, a)) return rc;
   if (int rc = check_launch("attn_decode_kv8")) return rc;
-  if (splits == 1 || a.cluster > 1) return LLMQRT_OK;
-  const int units = a.Sq * a.Hq * (D / 4);
-  if (int rc = launch_chained(attn_decode_kv8_merge_kernel<BF16, D>, dim3((unsigned)ceil_div(units, 128), (unsigned)B), dim3(128), 0, st, 1, a))
+  if (blocks == 1) return LLMQRT_OK;
+  int each = 1;
+  while (each < 16 && each * 4 * B < blocks) each *= 2;
+  const int warps = each < 4 ? 4 : each;
+  if (int rc = launch_chained(attn_decode_kv8_merge_kernel<BF16, D, ROWS>, dim3((unsigned)ceil_div(a.Sq * a.Hq, warps / each), (unsigned)B),
+                              dim3(32 * (unsigned)warps), 0, st, 1, a, blocks, each))
     return rc;
   return check_launch("attn_decode_kv8_merge");
 }

@@ -478,6 +478,38 @@ def test_attend_does_not_read_behind_the_last_key():
     assert bits_equal(attn_decode_kv8(q, kc, vc, ks, vs, table, _i32([45]), 128), clean)
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,Sq,top", [([1, 0, 0, 2, 0], 4, 1, 1, 20000), ([0] * 300 + [1, 64, 65, 5000] + [0] * 9, 2, 1, 1, 9000),
+                                               ([3000] + [1] * 130 + [129], 8, 8, 1, 40000), ([200, 70, 0, 64], 256, 256, 1, 9000),
+                                               ([777, 64], 512, 256, 16, 9000), ([6000, 5, 6001], 32, 2, 16, 9000)])
+def test_attend_shares(lens, Hq, Hkv, Sq, top):
+    """Fewer keys than blocks, sequences without keys between others, heads that fill the machine by themselves."""
+    _check_attend(lens, 16, Hq, Hkv, 64, Sq, "int8", torch.float16, top=top, width=-(-top // 16))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(2, 1), (16, 2), (24, 2)])
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_attend_keeps_nan_with_the_rows_that_see_it(d, Hq, Hkv, dt):
+    """A NaN in a later token's value or key is not seen by the earlier ones; a NaN in a query stays in its row."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    g = _gen(15)
+    kc, vc, ks, vs = _cache(g, "e4m3", 8, Hkv, 16, d)
+    q = torch.randn(2, 4, Hq, d, generator=g, device="cuda").to(DT[dt])
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens = [40, 63]
+    clean = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32(lens), 64)
+    vc.view(torch.uint8)[2, 0, 6, 5] = 0x7F                   # sequence 0's key 38: its last two tokens see it
+    kc.view(torch.uint8)[7, Hkv - 1, 14, 3] = 0xFF            # sequence 1's key 62: the last token alone
+    q[1, 0, 1, 7] = float("nan")
+    out = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32(lens), 64)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    rep = Hq // Hkv
+    bad[0, 2:, :rep, 5] = True
+    bad[1, 3, -rep:] = True
+    bad[1, 0, 1] = True
+    assert torch.isnan(out[bad]).all() and bits_equal(torch.where(bad, torch.zeros_like(out), out), torch.where(bad, torch.zeros_like(out), clean))
+
+
 def test_attend_beyond_32_bits():
     """A cache whose pages lie more than 2^32 bytes apart."""
     from llmqrt_b200.paged_cache import attn_decode_kv8, kv8_append
