@@ -32,6 +32,8 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 16 * kWarps;
 template <int D> constexpr int kv8_ring() { return D == 128 ? 3 : 5; }  // stages of a warp, 16 keys each
 constexpr int kSpan = 4096;                            // keys whose page numbers and scales a block holds at a time
+constexpr int kSwitch = 4;                             // what another sequence costs a block, in units of kStep keys
+constexpr int kMaxBlocks = 1024;                       // that one KV head's keys are shared out to
 constexpr int kMaxPages = kSpan / 16 + 1;              // pages that these touch
 constexpr int kClusterMergeMaxLen = 8192;               // greatest bound whose splits a cluster merges although it would take more than eight
 constexpr float kLog2e = 1.4426950408889634f;
@@ -98,49 +100,80 @@ template <bool BF16> __device__ __forceinline__ uint16_t round_bits(float f) {
 
 // Units of kStep keys of a sequence; one without keys counts as one (its rows of zeros are written).
 __device__ __forceinline__ int units_of(const Kv8Args& p, int b) { return max(1, (max(0, min(p.seqlens[b], p.max_len)) + kStep - 1) / kStep); }
-// Their number over sequences [b0, b1), by the whole block; `scan` has a word for each of its warps.
-__device__ __forceinline__ int64_t sum_units(const Kv8Args& p, int b0, int b1, int64_t* scan) {
-  int64_t n = 0;
-  for (int b = b0 + (int)threadIdx.x; b < b1; b += blockDim.x) n += units_of(p, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scan[threadIdx.x >> 5] = n;
-  __syncthreads();
-  n = 0;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) n += scan[w];
-  return n;
+
+// Where share k of the line begins, and the share that a place lies in (64-bit divisions take 100 instructions).
+__device__ __forceinline__ int64_t share_begin(int k, int64_t total, int shares) {
+  if (total < (1 << 21)) return (int64_t)((uint32_t)k * (uint32_t)total / (uint32_t)shares);      // k <= 1024
+  return k * total / shares;
 }
-// The sequence that unit `u` of all lies in, and which of the sequence's it is.
-__device__ __forceinline__ int find_unit(const Kv8Args& p, int64_t u, int64_t* scan, int& unit) {
-  __shared__ int found[2];
-  int64_t before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n = b < p.B ? units_of(p, b) : 0;
-    int64_t s = n;
+__device__ __forceinline__ int share_of(int64_t place, int64_t total, int shares) {
+  if (total < (1 << 21)) return (int)((((uint32_t)place + 1) * (uint32_t)shares - 1) / (uint32_t)total);
+  return (int)(((place + 1) * shares - 1) / total);
+}
+
+// Sequences lie on a line one after the other, each kSwitch places for the work that it costs to begin one and then its units; shares
+// are pieces of the line.  Finds the block's piece and where it begins.  (In shared memory: the loop over the keys has no registers
+// to spare for what is wanted after it.)
+struct Share {
+  int64_t total;                                       // the line's length
+  int64_t at, end;                                     // what is left of the piece
+  int64_t before;                                      // the length of the sequences before b
+  int shares, b;
+  int unit, unit_end, n_units;                         // what the block has of b, and how many there are
+};
+__device__ __forceinline__ void find_share(const Kv8Args& p, Share& share) {
+  __shared__ int64_t scan[2][kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto weight = [&](int b) -> int64_t { return b < p.B ? units_of(p, b) + kSwitch : 0; };
+  int64_t own = weight(tid), up_to = own, rest = 0;
+  for (int b = tid + kThreads; b < p.B; b += kThreads) rest += weight(b);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += v;
-    }
-    __syncthreads();
-    if (lane == 31) scan[warp] = s;
-    __syncthreads();
-    int64_t base = before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += scan[w];
-      before += scan[w];
-    }
-    if (u >= base + s - n && u < base + s) {
-      found[0] = b;
-      found[1] = (int)(u - (base + s - n));
-    }
-    if (u < before) break;                             // (the whole block)
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, up_to, o);
+    if (lane >= o) up_to += v;
+    rest += __shfl_xor_sync(0xffffffffu, rest, o);
+  }
+  if (lane == 31) {
+    scan[0][warp] = up_to;
+    scan[1][warp] = rest;
   }
   __syncthreads();
-  unit = found[1];
-  return found[0];
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) total += scan[0][w] + scan[1][w];
+  const int shares = (int)min((int64_t)gridDim.x, total);
+  const int64_t first = share_begin((int)blockIdx.x, total, shares);
+  if (tid == 0) {
+    share.total = total;
+    share.shares = shares;
+    share.at = first;
+    share.end = (int)blockIdx.x < shares ? share_begin((int)blockIdx.x + 1, total, shares) : first;
+  }
+  int64_t before = 0;
+  for (int b0 = 0;;) {
+    int64_t base = before;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += scan[0][w];
+      before += scan[0][w];
+    }
+    if (first >= base + up_to - own && first < base + up_to) {
+      share.b = b0 + tid;
+      share.before = base + up_to - own;
+    }
+    b0 += kThreads;
+    if (first < before || b0 >= p.B) break;          // (the whole block)
+    own = up_to = weight(b0 + tid);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, up_to, o);
+      if (lane >= o) up_to += v;
+    }
+    __syncthreads();
+    if (lane == 31) scan[0][warp] = up_to;
+    __syncthreads();
+  }
+  __syncthreads();
 }
 
 // Where a 16-byte chunk of a key's or a value's row lies in its tile of 16 rows, so that the fragment loads below meet no bank
@@ -164,33 +197,41 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   constexpr bool REST = !BF16;                         // Q's and P's remainders take part
   constexpr int G = ROWS / 8;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float4 pages[kMaxPages];                  // number (bits; -1: none), key scale, value scale
+  constexpr int kQPitch = D + 8;
+  __shared__ int page_ids[kMaxPages];                  // -1: none
+  __shared__ float2 page_scales[kMaxPages];            // keys', values'
+  __shared__ __align__(16) uint16_t q_rows[(REST ? 2 : 1) * ROWS * kQPitch];      // Q's rows as fp16, and what that leaves over
+  __shared__ float q_scale[ROWS];
+  __shared__ int q_sees[ROWS];                         // keys that a row's token sees
   pdl_wait();
   pdl_trigger();
   const int hkv = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles;
   const int rep = p.Hq / p.Hkv, rows = p.Sq * rep;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  // The block's share: a cluster's blocks have a sequence's keys between them, otherwise every block of a KV head has as many units
-  // of kStep keys of all sequences together.
-  int b, unit;
-  int64_t units_left;
-  if (p.cluster > 1) {
-    b = blockIdx.z;
-    const int n = units_of(p, b), each = (n + p.cluster - 1) / p.cluster;
-    unit = min((int)blockIdx.x * each, n);
-    units_left = min(each, n - unit);
-  } else {
-    __shared__ int64_t scan[kWarps];
-    const int64_t total = sum_units(p, 0, p.B, scan), shares = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= shares) return;
-    const int64_t first = blockIdx.x * total / shares;
-    units_left = (blockIdx.x + 1) * total / shares - first;
-    b = find_unit(p, first, scan, unit);
-  }
-  for (bool more = true; more;) {
+  // The block's share: a cluster's blocks have a sequence's keys between them, otherwise the blocks of a KV head share out all
+  // sequences' keys.
+  __shared__ Share share;
+  if (p.cluster == 1) find_share(p, share);
+  do {
+  if (p.cluster == 1 && share.at >= share.end) return; // (more blocks than places)
+  const int b = p.cluster > 1 ? (int)blockIdx.z : share.b;
   const int L_raw = p.seqlens[b], L = max(0, min(L_raw, p.max_len)), n_units = units_of(p, b);
-  const int unit_end = (int)min((int64_t)n_units, unit + units_left);
-  const bool whole = unit == 0 && unit_end == n_units;
+  int unit, unit_end;
+  if (p.cluster > 1) {
+    const int each = (n_units + p.cluster - 1) / p.cluster;
+    unit = min((int)blockIdx.x * each, n_units);
+    unit_end = min(unit + each, n_units);
+  } else {
+    const int64_t begins = share.before + kSwitch;     // where b's units do
+    unit = (int)max((int64_t)0, share.at - begins);
+    unit_end = (int)max((int64_t)0, min((int64_t)n_units, share.end - begins));
+    if (tid == 0) {
+      share.unit = unit;
+      share.unit_end = unit_end;
+      share.n_units = n_units;
+    }
+  }
+  if (p.cluster > 1 || unit_end > unit) {
   const int key_begin = min(unit * kStep, L), key_end = min(L, unit_end * kStep);
 
   // ---- page numbers and scales of the keys from span_begin on ----
@@ -201,11 +242,65 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
     for (int i = tid; i < n; i += kThreads) {
       const int id = p.table[(int64_t)b * p.table_stride + page0 + i];
       const bool good = id >= 0 && id < p.pages;
-      pages[i] = make_float4(__int_as_float(good ? id : -1), good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f,
-                             good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f, 0.f);
+      page_ids[i] = good ? id : -1;
+      page_scales[i] = make_float2(good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f, good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f);
     }
     __syncthreads();
   };
+
+  // ---- Q, turned, as fp16: sixteen threads a row, which have pairs of elements half a head apart ----
+  // (Before the first tiles: behind them its loads take 4 us.  Every warp preparing its own fragments took 3 us of all warps' issue.)
+  constexpr int NP = D / 32;                           // pairs of a thread
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+#pragma unroll
+  for (int h = 0; h < G; ++h) {
+    const int r_here = h * 8 + (tid >> 4), r = tile * ROWS + r_here, i0 = NP * (tid & 15);
+    const bool on = r < rows;
+    const int s = on ? r / rep : 0, head = hkv * rep + (on ? r - s * rep : 0), angle = L_raw - p.Sq + s;
+    const uint16_t* src = p.q + (int64_t)b * p.q_batch_stride + (int64_t)s * p.q_token_stride + (int64_t)head * D + i0;
+    float lo[NP], hi[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i += 2) {
+      const float2 a = unpack_pair<T>(on ? *reinterpret_cast<const uint32_t*>(src + i) : 0u);
+      const float2 c = unpack_pair<T>(on ? *reinterpret_cast<const uint32_t*>(src + D / 2 + i) : 0u);
+      lo[i] = a.x; lo[i + 1] = a.y; hi[i] = c.x; hi[i + 1] = c.y;
+    }
+    if (p.cos_tab != nullptr && angle >= 0 && angle < p.table_rows) {
+#pragma unroll
+      for (int i = 0; i < NP; i += 2) {
+        const float2 c = *reinterpret_cast<const float2*>(p.cos_tab + (int64_t)angle * (D / 2) + i0 + i);
+        const float2 sn = *reinterpret_cast<const float2*>(p.sin_tab + (int64_t)angle * (D / 2) + i0 + i);
+        const float l0 = lo[i], l1 = lo[i + 1];
+        lo[i] = l0 * c.x - hi[i] * sn.x; hi[i] = l0 * sn.x + hi[i] * c.x;
+        lo[i + 1] = l1 * c.y - hi[i + 1] * sn.y; hi[i + 1] = l1 * sn.y + hi[i + 1] * c.y;
+      }
+    }
+    // fp16 keeps 11 bits between 2^-14 and 65504: the row's maximum goes to [2^13, 2^14)
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+#pragma unroll
+    for (int o_ = 1; o_ < 16; o_ <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o_));
+    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);      // (an infinity or a NaN stays what it is)
+    const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
+    uint16_t* row = q_rows + r_here * kQPitch + i0;
+#pragma unroll
+    for (int i = 0; i < NP; i += 2)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float x = (c ? hi[i] : lo[i]) * up, y = (c ? hi[i + 1] : lo[i + 1]) * up;
+        const uint32_t w = pack_half(x, y);
+        *reinterpret_cast<uint32_t*>(row + c * (D / 2) + i) = w;
+        if constexpr (REST) {
+          const float2 f = unpack_half(w);
+          *reinterpret_cast<uint32_t*>(row + ROWS * kQPitch + c * (D / 2) + i) = pack_half(x - f.x, y - f.y);
+        }
+      }
+    if ((tid & 15) == 0) {
+      q_scale[r_here] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale * (p.softcap != 0.f ? 1.f : kLog2e);
+      q_sees[r_here] = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
+    }
+  }
   load_pages();
 
   // ---- the ring's first stages ----
@@ -218,10 +313,10 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   auto issue = [&](int key0, int stage) {
     if (key0 < span_end) {
       const uint32_t base = ring + (uint32_t)(stage * STAGE);
-      const int id = __float_as_int(pages[(key0 >> shift) - page0].x);
-      const int64_t at = (int64_t)max(id, 0) * p.page_stride + (int64_t)hkv * p.head_stride + (int64_t)(key0 & (p.page - 1)) * D + lane * 16;
-      const uint8_t* ks = p.k_cache + at;
-      const uint8_t* vs = p.v_cache + at;
+      const int id = page_ids[(key0 >> shift) - page0];
+      const int64_t from = (int64_t)max(id, 0) * p.page_stride + (int64_t)hkv * p.head_stride + (int64_t)(key0 & (p.page - 1)) * D + lane * 16;
+      const uint8_t* ks = p.k_cache + from;
+      const uint8_t* vs = p.v_cache + from;
       const uint32_t kd = base + k_dst, v0 = base + TILE + v_dst0, v1 = base + TILE + v_dst1;
       if (id >= 0 && key0 + 16 <= span_end) {
         cp_async_16<0>(kd, ks);
@@ -256,85 +351,29 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   };
   issue_first();
 
-  // ---- Q: rows g and g + 8 of the tile; register 2i, 2i + 1 of a piece are the MMA's k slots 2t and 2t + 8 of step i ----
-  uint32_t qa[G][NJ][8], qr[G][NJ][8];                 // fp16 and what it leaves over
+  // ---- its fragments: row g; registers 2i, 2i + 1 of a piece are the MMA's k slots 2t and 2t + 8 of step i ----
+  uint32_t qa[G][NJ][8], qr[G][NJ][8];
   float scale_q[G][2];                                 // of rows 2t and 2t + 1, which the lane has scores of
-  int sees[G][2];                                      // keys that these rows' tokens see
+  int sees[G][2];
 #pragma unroll
   for (int h = 0; h < G; ++h) {
-    const int r = tile * ROWS + h * 8 + g;
-    const bool on = r < rows;
-    const int s = on ? r / rep : 0, head = hkv * rep + (on ? r - s * rep : 0);
-    const int sees_g = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
-    const int angle = L_raw - p.Sq + s;
-    const bool rotate = p.cos_tab != nullptr && angle >= 0 && angle < p.table_rows;
-    const uint16_t* src = p.q + (int64_t)b * p.q_batch_stride + (int64_t)s * p.q_token_stride + (int64_t)head * D;
-    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    float x[NJ][16];                                   // this lane's elements 16 (4j + t) .. + 15
-    auto piece = [&](int d0, float (&y)[16]) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 v = on ? *reinterpret_cast<const uint4*>(src + d0 + 8 * i) : make_uint4(0, 0, 0, 0);
-        const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = unpack_pair<T>(vw[e]);
-          y[8 * i + 2 * e] = a.x; y[8 * i + 2 * e + 1] = a.y;
-        }
-      }
-    };
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) piece(16 * (4 * j + t), x[j]);
-    if (rotate) {                                      // pairs lie half a head apart: with d = 128 in the lane's own two pieces
-      const int i0 = D == 128 ? 16 * t : 16 * (t & 1);
-      const float4* cr = reinterpret_cast<const float4*>(p.cos_tab + (int64_t)angle * (D / 2) + i0);
-      const float4* sr = reinterpret_cast<const float4*>(p.sin_tab + (int64_t)angle * (D / 2) + i0);
-      float other[16];
-      if constexpr (D == 64) piece((16 * t + 32) % 64, other);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 c4 = __ldg(cr + k), s4 = __ldg(sr + k);
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (D == 128) {
-            const float lo = x[0][4 * k + e], hi = x[1][4 * k + e];
-            x[0][4 * k + e] = lo * c[e] - hi * sn[e];
-            x[1][4 * k + e] = lo * sn[e] + hi * c[e];
-          } else {
-            const float own = x[0][4 * k + e], far = other[4 * k + e];
-            x[0][4 * k + e] = t < 2 ? own * c[e] - far * sn[e] : far * sn[e] + own * c[e];
-          }
-        }
-      }
-    }
-    // fp16 keeps 11 bits between 2^-14 and 65504: the row's maximum goes to [2^13, 2^14)
-    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[j][e]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);      // (an infinity or a NaN stays what it is)
-    const float up = __uint_as_float((uint32_t)(13 - ex + 127) << 23);
-    const float scale_g = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale * (p.softcap != 0.f ? 1.f : kLog2e);
+      for (int i = 0; i < 8; i += 4) {
+        const uint16_t* src = q_rows + (h * 8 + g) * kQPitch + 16 * (4 * j + t) + 2 * i;
+        const uint4 v = *reinterpret_cast<const uint4*>(src);
+        qa[h][j][i] = v.x; qa[h][j][i + 1] = v.y; qa[h][j][i + 2] = v.z; qa[h][j][i + 3] = v.w;
+        if constexpr (REST) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + ROWS * kQPitch);
+          qr[h][j][i] = u.x; qr[h][j][i + 1] = u.y; qr[h][j][i + 2] = u.z; qr[h][j][i + 3] = u.w;
+        }
+      }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      scale_q[h][c] = __shfl_sync(0xffffffffu, scale_g, 4 * (2 * t + c));
-      sees[h][c] = __shfl_sync(0xffffffffu, sees_g, 4 * (2 * t + c));
+      scale_q[h][c] = q_scale[h * 8 + 2 * t + c];
+      sees[h][c] = q_sees[h * 8 + 2 * t + c];
     }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = x[j][2 * e] * up, c = x[j][2 * e + 1] * up;
-        qa[h][j][e] = pack_half(a, c);
-        if constexpr (REST) {
-          const float2 f = unpack_half(qa[h][j][e]);
-          qr[h][j][e] = pack_half(a - f.x, c - f.y);
-        }
-      }
   }
 
   float o[NE / 2][G][4];                               // columns 2e and 2e + 1 of the lane's NE, rows 2t and 2t + 1 each
@@ -369,9 +408,9 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
       __syncwarp();
       const uint32_t st = ring + (uint32_t)((it % kRing) * STAGE);
       const int pi = (key0 >> shift) - page0;
-      const float4 info = pages[pi];
-      const float ks = info.y, vs = info.z;
-      const bool good = __float_as_int(info.x) >= 0;
+      const float2 info = page_scales[pi];
+      const float ks = info.x, vs = info.y;
+      const bool good = page_ids[pi] >= 0;
 
       // ---- S^T = K Q^T: this lane gets keys g and g + 8 of rows 2t and 2t + 1 ----
       float s_acc[G][NJ][4];
@@ -453,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
             }
           }
       }
-      const float share = vs * v_inv;
+      const float v_share = vs * v_inv;
 #pragma unroll
       for (int h = 0; h < G; ++h)
 #pragma unroll
@@ -462,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
           for (int c = 0; c < 2; ++c) {
             const float e = ex2(pv[h][kb][c] - m_run[h][c]);
             l_run[h][c] += e;
-            pv[h][kb][c] = e * share;
+            pv[h][kb][c] = e * v_share;
           }
       uint32_t pa[G][2], pr[G][2];                       // of row g: keys 2t, 2t + 1 and 2t + 8, 2t + 9
 #pragma unroll
@@ -565,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   // A lane has NE neighbouring columns of two rows; every other lane's have their quarters of 32 bytes the other way round, so
   // that eight lanes' 16 bytes meet no bank twice.
   constexpr int kPitch = D + 4;
-  auto at = [](int dd) { return dd ^ ((dd / NE & 1) << 2); };
+  auto column = [](int dd) { return dd ^ ((dd / NE & 1) << 2); };
   float* sm_o = reinterpret_cast<float*>(smem);        // [kWarps][ROWS][kPitch]
   float* sm_m = sm_o + kWarps * ROWS * kPitch;         // [kWarps][ROWS]
   float* sm_l = sm_m + kWarps * ROWS;
@@ -586,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
       float* row = sm_o + (warp * ROWS + r) * kPitch;
 #pragma unroll
       for (int e = 0; e < NE / 2; e += 2)
-        *reinterpret_cast<float4*>(row + at(NE * g + 2 * e)) =
+        *reinterpret_cast<float4*>(row + column(NE * g + 2 * e)) =
             make_float4(unlift * o[e][h][c], unlift * o[e][h][c + 2], unlift * o[e + 1][h][c], unlift * o[e + 1][h][c + 2]);
     }
   __syncthreads();
@@ -595,8 +634,9 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
     const int rr = tile * ROWS + r, s = rr / rep;
     return ((int64_t)b * p.Sq + s) * p.Hq + hkv * rep + (rr - s * rep);
   };
-  // (a block's first segment goes to its first slot, its last one to the second)
-  const int64_t slot = (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (unit > 0 ? 0 : 1)) * ROWS;
+  const bool whole = p.cluster == 1 && share.unit == 0 && share.unit_end == share.n_units;
+  // A part of a sequence goes to the workspace: one begun in the middle to the block's first slot, one begun at the start to the second.
+  const int64_t slot = (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (p.cluster == 1 && share.unit > 0 ? 0 : 1)) * ROWS;
   for (int i = tid; i < here * (D / 4); i += kThreads) {
     const int r = i / (D / 4), dd = i % (D / 4) * 4;
     float M = -INFINITY;
@@ -608,18 +648,18 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = ex2(sm_m[w * ROWS + r] - M);
-        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + r) * kPitch + at(dd));
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * ROWS + r) * kPitch + column(dd));
         lsum += sm_l[w * ROWS + r] * f;
         sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
       }
     }
-    if (p.cluster > 1 || !whole) {
+    if (whole) {
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      *reinterpret_cast<uint2*>(p.out + out_row(r) * D + dd) = make_uint2(round_pair<BF16>(sum.x * inv, sum.y * inv), round_pair<BF16>(sum.z * inv, sum.w * inv));
+    } else {
       float* po = p.cluster > 1 ? cl_o + r * D + dd : p.part_o + (slot + r) * D + dd;
       *reinterpret_cast<float4*>(po) = sum;
       if (dd == 0) *reinterpret_cast<float2*>(p.cluster > 1 ? cl_ml + 2 * r : p.part_ml + 2 * (slot + r)) = make_float2(M, lsum);
-    } else {
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-      *reinterpret_cast<uint2*>(p.out + out_row(r) * D + dd) = make_uint2(round_pair<BF16>(sum.x * inv, sum.y * inv), round_pair<BF16>(sum.z * inv, sum.w * inv));
     }
   }
   if (p.cluster > 1) {
@@ -655,36 +695,62 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
     }
     cluster_arrive();                                  // nobody leaves while a peer may still read its partial
     cluster_wait();
-    return;
+    return;                                            // (a cluster's block has one sequence)
   }
-  units_left -= unit_end - unit;
-  more = units_left > 0;
-  ++b;
-  unit = 0;
-  __syncthreads();                                     // (the merge has been read: its memory is the rings')
   }
+  __syncthreads();                                     // (all has been read: the memory is the rings')
+  if (tid == 0) {
+    share.before += share.n_units + kSwitch;
+    share.at = share.before;
+    ++share.b;
+  }
+  __syncthreads();
+  } while (share.at < share.end);
 }
 
-// Merge of the sequences that several blocks have had a part of.  `each` warps (1 .. 16) add up a row's parts, every each-th one, and are
-// joined in shared memory; a lane has D / 32 neighbouring outputs.  (All parts in one thread's loop: one sequence of 131072 keys
-// in 256 parts took 100 us.)
+// Merge of the sequences that several blocks have had a part of.  `each` warps (1 .. 16) add up a row's parts, every each-th one, and
+// are joined in shared memory; a lane has D / 32 neighbouring outputs.  (In the main kernel, by the block that comes last, it took
+// 10 us a stage for 12 parts: one block has too few loads under way.)
 template <bool BF16, int D, int ROWS>
 __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Args p, int blocks, int each) {
-  constexpr int W = D / 32;
+  constexpr int W = D / 32, kBatch = 8;
   __shared__ float sm_o[16][D];
   __shared__ float2 sm_ml[16];
-  __shared__ int64_t scan[16];
+  __shared__ int64_t scan[2][16];
   pdl_wait_then_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp & (each - 1);
   const int b = blockIdx.y, r = blockIdx.x * ((int)(blockDim.x >> 5) / each) + warp / each;
   // which blocks had a part
-  const int64_t before = sum_units(p, 0, b, scan), total = before + sum_units(p, b, p.B, scan);
-  const int64_t shares = min((int64_t)blocks, total);
-  const int first = (int)(((before + 1) * shares - 1) / total), last = (int)(((before + units_of(p, b)) * shares - 1) / total);
+  int64_t before = 0, total = 0;
+  for (int i = threadIdx.x; i < p.B; i += blockDim.x) {
+    const int w = units_of(p, i) + kSwitch;
+    total += w;
+    before += i < b ? w : 0;
+  }
+  const int n_units = units_of(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) {
+    scan[0][warp] = total;
+    scan[1][warp] = before;
+  }
+  __syncthreads();
+  total = before = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+    total += scan[0][w];
+    before += scan[1][w];
+  }
+  const int shares = (int)min((int64_t)blocks, total);
+  const int64_t begins = before + kSwitch;
+  const int first = share_of(begins, total, shares), last = share_of(begins + n_units - 1, total, shares);
   if (first == last) return;                           // (one: the result is there)
   const bool on = r < p.Sq * p.Hq;
   const int s = on ? r / p.Hq : 0, head = on ? r - s * p.Hq : 0, rep = p.Hq / p.Hkv, hkv = head / rep, tr = s * rep + head - hkv * rep;
   const int64_t column = (int64_t)(hkv * p.tiles + tr / ROWS) * blocks;
+  const int in_middle = share_begin(first, total, shares) > begins ? 0 : 1;      // (the parts behind the first begin in the middle)
   float M = -INFINITY, lsum = 0.f, o[W];
 #pragma unroll
   for (int j = 0; j < W; ++j) o[j] = 0.f;
@@ -697,15 +763,22 @@ __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Arg
     for (int j = 0; j < W; ++j) o[j] = o[j] * keep + v[j] * f;
   };
   if (on) {
-#pragma unroll 4
-    for (int k = first + part; k <= last; k += each) { // in the blocks' order
-      // (a block that begins in the middle of the sequence has it in its first slot)
-      const int64_t slot = ((column + k) * 2 + (k * total / shares > before ? 0 : 1)) * ROWS + tr % ROWS;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
-      float v[W];
-      if constexpr (W == 4) *reinterpret_cast<float4*>(v) = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + lane * W));
-      else *reinterpret_cast<float2*>(v) = __ldcg(reinterpret_cast<const float2*>(p.part_o + slot * D + lane * W));
-      join(ml, v);
+    for (int k0 = first + part; k0 <= last; k0 += kBatch * each) {       // in the blocks' order
+      float2 ml[kBatch];
+      float v[kBatch][W];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int k = k0 + i * each;
+        if (k <= last) {
+          const int64_t slot = ((column + k) * 2 + (k == first ? in_middle : 0)) * ROWS + tr % ROWS;
+          ml[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
+          if constexpr (W == 4) *reinterpret_cast<float4*>(v[i]) = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + lane * W));
+          else *reinterpret_cast<float2*>(v[i]) = __ldcg(reinterpret_cast<const float2*>(p.part_o + slot * D + lane * W));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (k0 + i * each <= last) join(ml[i], v[i]);
     }
   }
   if (each > 1) {
@@ -777,19 +850,19 @@ int launch(Kv8Args a, int B, void* workspace, cudaStream_t st) {
   a.cluster = 1;
   // (one wave of blocks; where a column has fewer than four of them, up to four waves, the last of which is rarely full)
   const int64_t waves = columns * 4 <= slots ? 1 : 4;
-  const int blocks = (int)std::min(std::max<int64_t>(1, waves * slots / columns), B * units);
+  const int blocks = (int)std::min<int64_t>({std::max<int64_t>(1, waves * slots / columns), B * (units + kSwitch), kMaxBlocks});
   if (blocks > 1 && !workspace) return set_error(LLMQRT_ERR_WORKSPACE, "attn_decode_kv8: split keys need the workspace");
-  const size_t rows = (size_t)columns * blocks * 2 * ROWS;
-  if (blocks > 1 && rows * (D + 2) * 4 > LLMQRT_WS_PARTIAL_BYTES)
+  const size_t slots_all = (size_t)columns * blocks * 2;
+  if (blocks > 1 && (slots_all * ROWS * (D + 2) * 4 > LLMQRT_WS_PARTIAL_BYTES ))
     return set_error(LLMQRT_ERR_UNSUPPORTED, "attn_decode_kv8: the blocks' partial results do not fit the workspace");
   a.part_o = blocks > 1 ? reinterpret_cast<float*>(ws_partials(workspace)) : nullptr;
-  a.part_ml = a.part_o + rows * D;
+  a.part_ml = a.part_o + slots_all * ROWS * D;
   if (int rc = launch_chained(kern, dim3((unsigned)blocks, (unsigned)columns, 1), dim3(kThreads), smem, st, 1, a)) return rc;
   if (int rc = check_launch("attn_decode_kv8")) return rc;
   if (blocks == 1) return LLMQRT_OK;
-  int each = 1;
-  while (each < 16 && each * 4 * B < blocks) each *= 2;
-  const int warps = each < 4 ? 4 : each;
+  int each = 1;                                        // warps a row: eight parts each, one batch of loads, where the parts are that many
+  while (each < 16 && each * 8 * B < blocks) each *= 2;
+  const int warps = std::max(4, each);
   if (int rc = launch_chained(attn_decode_kv8_merge_kernel<BF16, D, ROWS>, dim3((unsigned)ceil_div(a.Sq * a.Hq, warps / each), (unsigned)B),
                               dim3(32 * (unsigned)warps), 0, st, 1, a, blocks, each))
     return rc;
