@@ -6,19 +6,25 @@
 // HBM-bound: each code is read once, half the bytes of a 16-bit cache, so that what a key costs the schedulers counts:
 // at 6.5 TB/s an SM takes a key and value row of 128 every 11 cycles.  Warps stream 16 keys a step through rings of their own in
 // shared memory (cp.async, 16 keys always lie in one page), turn the codes into fp16, where both kinds are exact, and multiply
-// with warp-level MMAs, whose rows are the query heads that share the KV head.
-//   S = Q K^T : a lane's K fragment is 16 contiguous bytes of a key's row; Q is loaded with the same permutation of d.
-//   O += P V  : the fragment wants two keys a register: bytes of two rows are interleaved before they are converted.
+// with warp-level MMAs: keys (or columns of V) are the sixteen rows, the query heads that share the KV head the eight columns.
+//   S^T = K Q^T     : a lane's K fragment is 16 contiguous bytes of two keys' rows; Q is loaded with the same permutation of d.
+//   O^T += V^T P^T  : the fragment wants two keys a register: bytes of two rows are interleaved before they are converted.
+// (With the query rows as the sixteen, half of them idle, it took twice the MMAs and accumulators, three blocks an SM, and 64 us where
+// this takes 58.)
 // Scales stay out of the products: k_scale multiplies S; v_scale, over the greatest one of the pages so far (a second running
-// reference beside the softmax's maximum), multiplies P, which thus never leaves [0, 1], where fp16 rounds it as it rounds the result.
-// Q in fp16 is exact for fp16 and, its row multiplied by a power of two, for bf16.
-// With at most eight rows the MMA's other eight hold what the rounding of Q (rotated here) and of P to fp16 left over, so that an
-// fp16 result is off by its own rounding alone; with more rows these remainders take MMAs of their own (fp16 only: bf16's own
-// rounding is eight times as large).
+// reference beside the softmax's maximum), multiplies P.  Q in fp16 is exact for fp16 and, its row multiplied by a power of two, for
+// bf16.  For an fp16 result what the rounding of Q (rotated here) and of P to fp16 left over takes MMAs of its own, so that the
+// result is off by its own rounding alone; bf16's own rounding is eight times as large.
 //
-// Grid (splits, Hkv * row tiles, B).  A block merges its four warps in shared memory; splits of one sequence are merged by the
-// thread-block cluster that they form, or, where there are more than eight, by a second kernel from the workspace.
+// Grid.  Few short sequences: clusters of up to eight blocks, which have a sequence's keys between them and merge their parts through
+// each other's shared memory.  Otherwise (blocks, Hkv * row tiles): as many blocks as fit at once, each with an equal piece of all
+// sequences' keys laid end to end, whatever their lengths; sequences that several blocks have had a part of are merged from
+// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 52.)
 // Page numbers outside the cache and rows behind the last key are not read (zeros take their place) and get no weight.
+//
+// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 52 us (4.3 TB/s: beginning a sequence costs a
+// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 34 us
+// (4.0 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 201 us (5.9 TB/s).
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -32,10 +38,10 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 16 * kWarps;
 template <int D> constexpr int kv8_ring() { return D == 128 ? 3 : 5; }  // stages of a warp, 16 keys each
 constexpr int kSpan = 4096;                            // keys whose page numbers and scales a block holds at a time
-constexpr int kSwitch = 4;                             // what another sequence costs a block, in units of kStep keys
+constexpr int kSwitch = 6;                             // what another sequence costs a block, in units of kStep keys (4: 54, 6 to 10: 51.6, 16: 52.5 us)
 constexpr int kMaxBlocks = 1024;                       // that one KV head's keys are shared out to
 constexpr int kMaxPages = kSpan / 16 + 1;              // pages that these touch
-constexpr int kClusterMergeMaxLen = 8192;               // greatest bound whose splits a cluster merges although it would take more than eight
+constexpr int kClusterMergeMaxLen = 8192;              // greatest bound on the lengths for which a sequence gets one cluster
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv8Args {
@@ -237,43 +243,58 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   // ---- page numbers and scales of the keys from span_begin on ----
   const int shift = __ffs(p.page) - 1;
   int span_begin = key_begin, span_end = min(key_end, key_begin + kSpan), page0 = key_begin >> shift;
-  auto load_pages = [&]() {
-    const int n = span_end > span_begin ? ((span_end - 1) >> shift) - page0 + 1 : 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const int id = p.table[(int64_t)b * p.table_stride + page0 + i];
-      const bool good = id >= 0 && id < p.pages;
-      page_ids[i] = good ? id : -1;
-      page_scales[i] = make_float2(good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f, good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f);
+  auto span_pages = [&]() { return span_end > span_begin ? ((span_end - 1) >> shift) - page0 + 1 : 0; };
+  auto page_id = [&](int i) { return i < span_pages() ? p.table[(int64_t)b * p.table_stride + page0 + i] : -1; };
+  auto page_scale = [&](int id) {
+    const bool good = id >= 0 && id < p.pages;
+    return make_float2(good ? p.k_scale[(int64_t)id * p.Hkv + hkv] : 0.f, good ? p.v_scale[(int64_t)id * p.Hkv + hkv] : 0.f);
+  };
+  auto keep_page = [&](int i, int id, float2 scales) {
+    page_ids[i] = id >= 0 && id < p.pages ? id : -1;
+    page_scales[i] = scales;
+  };
+  auto load_pages = [&](int from) {
+    for (int i = from; i < span_pages(); i += kThreads) {
+      const int id = page_id(i);
+      keep_page(i, id, page_scale(id));
     }
     __syncthreads();
   };
+  const int first_id = page_id(tid);
 
   // ---- Q, turned, as fp16: sixteen threads a row, which have pairs of elements half a head apart ----
-  // (Before the first tiles: behind them its loads take 4 us.  Every warp preparing its own fragments took 3 us of all warps' issue.)
+  // (Asked for before the first tiles, behind which the loads would take 4 us, and beside the pages' scales.  Every warp preparing its own fragments took 3 us of all warps' issue.)
   constexpr int NP = D / 32;                           // pairs of a thread
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  uint32_t q_lo[G][NP / 2], q_hi[G][NP / 2];
+  float2 q_cos[G][NP / 2], q_sin[G][NP / 2];
 #pragma unroll
   for (int h = 0; h < G; ++h) {
-    const int r_here = h * 8 + (tid >> 4), r = tile * ROWS + r_here, i0 = NP * (tid & 15);
+    const int r = tile * ROWS + h * 8 + (tid >> 4), i0 = NP * (tid & 15);
     const bool on = r < rows;
     const int s = on ? r / rep : 0, head = hkv * rep + (on ? r - s * rep : 0), angle = L_raw - p.Sq + s;
+    const bool turn = p.cos_tab != nullptr && angle >= 0 && angle < p.table_rows;
     const uint16_t* src = p.q + (int64_t)b * p.q_batch_stride + (int64_t)s * p.q_token_stride + (int64_t)head * D + i0;
+    const int64_t from = (int64_t)angle * (D / 2) + i0;
+#pragma unroll
+    for (int i = 0; i < NP / 2; ++i) {
+      q_lo[h][i] = on ? *reinterpret_cast<const uint32_t*>(src + 2 * i) : 0u;
+      q_hi[h][i] = on ? *reinterpret_cast<const uint32_t*>(src + D / 2 + 2 * i) : 0u;
+      q_cos[h][i] = turn ? *reinterpret_cast<const float2*>(p.cos_tab + from + 2 * i) : make_float2(1.f, 1.f);
+      q_sin[h][i] = turn ? *reinterpret_cast<const float2*>(p.sin_tab + from + 2 * i) : make_float2(0.f, 0.f);
+    }
+    if ((tid & 15) == 0) q_sees[h * 8 + (tid >> 4)] = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
+  }
+  const float2 first_scale = page_scale(first_id);
+#pragma unroll
+  for (int h = 0; h < G; ++h) {
+    const int r_here = h * 8 + (tid >> 4), i0 = NP * (tid & 15);
     float lo[NP], hi[NP];
 #pragma unroll
     for (int i = 0; i < NP; i += 2) {
-      const float2 a = unpack_pair<T>(on ? *reinterpret_cast<const uint32_t*>(src + i) : 0u);
-      const float2 c = unpack_pair<T>(on ? *reinterpret_cast<const uint32_t*>(src + D / 2 + i) : 0u);
-      lo[i] = a.x; lo[i + 1] = a.y; hi[i] = c.x; hi[i + 1] = c.y;
-    }
-    if (p.cos_tab != nullptr && angle >= 0 && angle < p.table_rows) {
-#pragma unroll
-      for (int i = 0; i < NP; i += 2) {
-        const float2 c = *reinterpret_cast<const float2*>(p.cos_tab + (int64_t)angle * (D / 2) + i0 + i);
-        const float2 sn = *reinterpret_cast<const float2*>(p.sin_tab + (int64_t)angle * (D / 2) + i0 + i);
-        const float l0 = lo[i], l1 = lo[i + 1];
-        lo[i] = l0 * c.x - hi[i] * sn.x; hi[i] = l0 * sn.x + hi[i] * c.x;
-        lo[i + 1] = l1 * c.y - hi[i + 1] * sn.y; hi[i + 1] = l1 * sn.y + hi[i + 1] * c.y;
-      }
+      const float2 a = unpack_pair<T>(q_lo[h][i / 2]), e = unpack_pair<T>(q_hi[h][i / 2]), c = q_cos[h][i / 2], sn = q_sin[h][i / 2];
+      lo[i] = a.x * c.x - e.x * sn.x; hi[i] = a.x * sn.x + e.x * c.x;
+      lo[i + 1] = a.y * c.y - e.y * sn.y; hi[i + 1] = a.y * sn.y + e.y * c.y;
     }
     // fp16 keeps 11 bits between 2^-14 and 65504: the row's maximum goes to [2^13, 2^14)
     float top = 0.f;
@@ -296,12 +317,10 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
           *reinterpret_cast<uint32_t*>(row + ROWS * kQPitch + c * (D / 2) + i) = pack_half(x - f.x, y - f.y);
         }
       }
-    if ((tid & 15) == 0) {
-      q_scale[r_here] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale * (p.softcap != 0.f ? 1.f : kLog2e);
-      q_sees[r_here] = on ? min(L, L_raw - p.Sq + 1 + s) : 0;
-    }
+    if ((tid & 15) == 0) q_scale[r_here] = __uint_as_float((uint32_t)(ex - 13 + 127) << 23) * p.scale * (p.softcap != 0.f ? 1.f : kLog2e);
   }
-  load_pages();
+  if (tid < span_pages()) keep_page(tid, first_id, first_scale);
+  load_pages(tid + kThreads);
 
   // ---- the ring's first stages ----
   // A lane's pieces of a tile are 512 bytes apart in both memories; their swizzle is one of two.
@@ -596,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
     span_begin = span_end;
     span_end = min(key_end, span_begin + kSpan);
     page0 = span_begin >> shift;
-    load_pages();
+    load_pages(tid);
     issue_first();
   }
 
@@ -787,7 +806,21 @@ __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Arg
     if (lane == 0) sm_ml[warp] = make_float2(M, lsum);
     __syncthreads();
     if (part != 0 || !on) return;
-    for (int w = 1; w < each; ++w) join(sm_ml[warp + w], &sm_o[warp + w][lane * W]);
+    const float2 mine = lane < each ? sm_ml[warp + lane] : make_float2(-INFINITY, 0.f);
+    M = mine.x;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    const float f_mine = mine.x > -INFINITY ? ex2(mine.x - M) : 0.f;
+    lsum = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = 0.f;
+    for (int w = 0; w < each; ++w) {
+      const float f = __shfl_sync(0xffffffffu, f_mine, w);
+      lsum += __shfl_sync(0xffffffffu, mine.y, w) * f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) o[j] += sm_o[warp + w][lane * W + j] * f;
+    }
   }
   if (!on) return;
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
