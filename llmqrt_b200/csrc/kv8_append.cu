@@ -34,12 +34,14 @@ struct AppendArgs {
   int T, Hkv, page, table_rows, window;
 };
 
-template <typename T, int D, bool INT8>
+// TEAM: warps that share a run, 1 or all of the block's.
+template <typename T, int D, bool INT8, int TEAM>
 __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
-  constexpr int kLanes = D / 16, kRows = 32 / kLanes;  // lanes of a row, rows a warp takes at once
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes * TEAM;             // lanes of a row, rows that are taken at once
+  __shared__ float tops[2][kWarps];
   pdl_wait_then_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, kind = blockIdx.z;
-  const int piece = lane % kLanes, sub = lane / kLanes;
+  const int piece = lane % kLanes, sub = lane / kLanes + (TEAM > 1 ? warp * (32 / kLanes) : 0);
   const int w0 = blockIdx.x * p.window, w1 = min(p.T, w0 + p.window);
   const int shift = __ffs(p.page) - 1;
   // the runs that begin in the window: one bit a token (a window has at most 32)
@@ -50,7 +52,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
   }
   unsigned runs = __ballot_sync(0xffffffffu, begins);
   for (int nth = 0; runs; runs &= runs - 1, ++nth) {
-    if (nth % kWarps != warp) continue;
+    if (TEAM == 1 && nth % kWarps != warp) continue;
     const int t0 = w0 + __ffs(runs) - 1;
     const int64_t s0 = p.slots[t0];
     const int row0 = (int)(s0 & (p.page - 1));
@@ -97,6 +99,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
       }
     };
     float top = 0.f;
+#pragma unroll 4
     for (int i = sub; i < n; i += kRows) {
       float x[16];
       fetch(i, x);
@@ -105,6 +108,12 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
     }
     top = warp_max(top);
     const float was = row0 > 0 ? *scale : 0.f;
+    if constexpr (TEAM > 1) {                          // (two sets in turn: one barrier a run is enough, and none reads the old scale behind it)
+      if (lane == 0) tops[nth & 1][warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) top = fmaxf(top, tops[nth & 1][w]);
+    }
     const float now = fmaxf(was, kv8_scale<INT8>(top)), inv = __fdiv_rn(1.f, now);
     // lane `piece` of a row holds elements 8 piece .. + 7 and D / 2 further: two 8-byte stores
     for (int i = sub; i < n; i += kRows) {
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
         }
       }
       __syncwarp();                                    // (every lane has read the old scale)
-      if (lane == 0) *scale = now;
+      if (TEAM > 1 ? threadIdx.x == 0 : lane == 0) *scale = now;
     }
   }
 }
@@ -168,14 +177,17 @@ extern "C" int llmqrt_kv8_append(void* k_cache, void* v_cache, float* k_scale, f
   a.slots = slots; a.cos_tab = cos_table; a.sin_tab = sin_table; a.positions = positions;
   a.num_slots = pages * page;
   a.T = (int)T; a.Hkv = (int)Hkv; a.page = (int)page; a.table_rows = (int)table_rows;
-  a.window = T <= 2048 ? kWarps : 32;
+  // (at 64 tokens a warp a run)
+  const bool team = T > 2048;
+  a.window = team ? 32 : kWarps;
   const dim3 grid((unsigned)ceil_div(T, a.window), (unsigned)Hkv, 2);
   auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
   const bool i8 = cache_type == LLMQRT_I8;
   auto pick = [&](auto tag) {
     using T_ = decltype(tag);
-    return d == 128 ? (i8 ? go(kv8_append_kernel<T_, 128, true>) : go(kv8_append_kernel<T_, 128, false>))
-                    : (i8 ? go(kv8_append_kernel<T_, 64, true>) : go(kv8_append_kernel<T_, 64, false>));
+#define LLMQRT_APPEND(D_, I_) (team ? go(kv8_append_kernel<T_, D_, I_, kWarps>) : go(kv8_append_kernel<T_, D_, I_, 1>))
+    return d == 128 ? (i8 ? LLMQRT_APPEND(128, true) : LLMQRT_APPEND(128, false)) : (i8 ? LLMQRT_APPEND(64, true) : LLMQRT_APPEND(64, false));
+#undef LLMQRT_APPEND
   };
   if (int rc = dtype == LLMQRT_F16 ? pick(__half()) : pick(__nv_bfloat16())) return rc;
   return check_launch("kv8_append");

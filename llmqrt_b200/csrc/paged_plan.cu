@@ -32,7 +32,7 @@ struct PlanArgs {
 };
 
 // Exclusive sum over the block's threads in thread order; the total comes back in `total`.
-__device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_sums, int64_t& total) {
+template <int THREADS> __device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_sums, int64_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t s = v;
 #pragma unroll
@@ -42,7 +42,7 @@ __device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_
   }
   if (lane == 31) warp_sums[warp] = s;
   __syncthreads();
-  int64_t w = lane < kPlanThreads / 32 ? warp_sums[lane] : 0;
+  int64_t w = lane < THREADS / 32 ? warp_sums[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t n = __shfl_up_sync(0xffffffffu, w, o);
@@ -54,32 +54,34 @@ __device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_
   return s - v + (warp > 0 ? before : 0);
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(PlanArgs p) {
+template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kernel(PlanArgs p) {
   extern __shared__ int32_t plan_smem[];
-  __shared__ int64_t warp_sums[kPlanThreads / 32];
+  __shared__ int64_t warp_sums[THREADS / 32];
   int32_t* cu_s = plan_smem;                           // [B] first token of the request
   int32_t* ctx_s = cu_s + p.B;                         // [B] its context
   int32_t* off_s = ctx_s + p.B;                        // [B] its first page's place below the stack's top; -1: it gets nothing
   const int cl = gridDim.x, rank = blockIdx.x;
   pdl_wait_then_trigger();
   const int64_t count = min(max(*p.free_count, 0), p.pool);
-  int64_t tokens = 0, wanted = 0, taken = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+  __shared__ int32_t taken;
+  if (threadIdx.x == 0) taken = 0;
+  __syncthreads();
+  int64_t tokens = 0, wanted = 0;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
     const int b = b0 + threadIdx.x;
     const bool in = b < p.B;
     const int64_t ctx = in ? max(p.context[b], 0) : 0, n = in ? max(p.fresh[b], 0) : 0;
     const int64_t have = (ctx + p.page - 1) / p.page, all = (ctx + n + p.page - 1) / p.page;
     int64_t sum;
-    const int64_t cu = tokens + block_exclusive_sum(n, warp_sums, sum);
+    const int64_t cu = tokens + block_exclusive_sum<THREADS>(n, warp_sums, sum);
     tokens += sum;
     bool fits = cu + n <= p.max_tokens && all <= p.width;
     const int64_t need = fits ? all - have : 0;
-    const int64_t off = wanted + block_exclusive_sum(need, warp_sums, sum);
+    const int64_t off = wanted + block_exclusive_sum<THREADS>(need, warp_sums, sum);
     wanted += sum;
     fits = fits && (need == 0 || off + need <= count);
     // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
-    block_exclusive_sum(fits ? need : 0, warp_sums, sum);
-    taken += sum;
+    if (fits && need) atomicMax(&taken, (int32_t)(off + need));
     if (in) {
       cu_s[b] = (int32_t)min(cu, (int64_t)0x7fffffff);
       ctx_s[b] = (int32_t)ctx;
@@ -92,7 +94,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(PlanArgs p) {
     cluster_wait();
   }
   if (rank == 0) {
-    for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+    for (int b = threadIdx.x; b < p.B; b += THREADS) {
       const int32_t next = b + 1 < p.B ? cu_s[b + 1] : (int32_t)min(tokens, (int64_t)0x7fffffff);
       p.cu[b + 1] = next;
       p.seq[b] = ctx_s[b] + (off_s[b] >= 0 ? next - cu_s[b] : 0);
@@ -102,8 +104,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(PlanArgs p) {
       *p.free_left = (int32_t)(count - taken);
     }
   }
-  const int lane = threadIdx.x & 31, warps = cl * (kPlanThreads / 32);
-  for (int b = rank * (kPlanThreads / 32) + (threadIdx.x >> 5); b < p.B; b += warps) {
+  const int lane = threadIdx.x & 31, warps = cl * (THREADS / 32);
+  for (int b = rank * (THREADS / 32) + (threadIdx.x >> 5); b < p.B; b += warps) {
     const int off = off_s[b];
     if (off < 0) continue;
     const int n = (b + 1 < p.B ? cu_s[b + 1] : (int)tokens) - cu_s[b];
@@ -111,27 +113,48 @@ __global__ void __launch_bounds__(kPlanThreads) plan_step_kernel(PlanArgs p) {
     for (int j = lane; j < all - have; j += 32) p.table[(int64_t)b * p.table_stride + have + j] = p.free_pages[count - 1 - off - j];
   }
   const int shift = __ffs(p.page) - 1;
-  for (int64_t t = rank * kPlanThreads + threadIdx.x; t < p.max_tokens; t += cl * kPlanThreads) {
-    int64_t slot = -1;
-    int32_t position = 0;
-    if (t < tokens) {
-      int lo = 0, hi = p.B;                            // the last request whose first token is at most t
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cu_s[mid] <= t) lo = mid;
-        else hi = mid;
-      }
-      const int off = off_s[lo];
-      if (off >= 0) {
-        position = ctx_s[lo] + (int32_t)(t - cu_s[lo]);
-        const int have = (int)(((int64_t)ctx_s[lo] + p.page - 1) >> shift), j = position >> shift;
-        // (a page taken in this step is read from the stack: another block may write the table's entry)
-        const int id = j < have ? p.table[(int64_t)lo * p.table_stride + j] : p.free_pages[count - 1 - off - (j - have)];
-        if (id >= 0) slot = ((int64_t)id << shift) + (position & (p.page - 1));
+  // A warp has consecutive tokens, 32 kBatch at a time: a lane looks for its first one's request by bisection and goes on from there,
+  // and kBatch look-ups are under way at once.
+  constexpr int kBatch = 4;
+  const int64_t all_tokens = min(tokens, (int64_t)p.max_tokens);
+  const int64_t each = ((int64_t)p.max_tokens + warps * 32 * kBatch - 1) / (warps * 32 * kBatch) * (32 * kBatch);
+  const int64_t begin = (rank * (THREADS / 32) + (threadIdx.x >> 5)) * each, end = min(begin + each, (int64_t)p.max_tokens);
+  int lo = 0;                                          // the last request whose first token is at most t
+  if (begin + lane < all_tokens) {
+    int hi = p.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu_s[mid] <= begin + lane) lo = mid;
+      else hi = mid;
+    }
+  }
+  for (int64_t t0 = begin + lane; t0 < end; t0 += 32 * kBatch) {
+    int32_t position[kBatch];
+    int id[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t t = t0 + 32 * i;
+      position[i] = 0;
+      id[i] = -1;
+      if (t < all_tokens) {
+        while (lo + 1 < p.B && cu_s[lo + 1] <= t) ++lo;
+        const int off = off_s[lo];
+        if (off >= 0) {
+          position[i] = ctx_s[lo] + (int32_t)(t - cu_s[lo]);
+          const int have = (int)(((int64_t)ctx_s[lo] + p.page - 1) >> shift), j = position[i] >> shift;
+          // (a page taken in this step is read from the stack: another block may write the table's entry)
+          id[i] = j < have ? p.table[(int64_t)lo * p.table_stride + j] : p.free_pages[count - 1 - off - (j - have)];
+        }
       }
     }
-    p.slots[t] = slot;
-    p.positions[t] = position;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t t = t0 + 32 * i;
+      if (t < end) {
+        p.slots[t] = id[i] >= 0 ? ((int64_t)id[i] << shift) + (position[i] & (p.page - 1)) : -1;
+        p.positions[t] = position[i];
+      }
+    }
   }
 }
 
@@ -151,7 +174,7 @@ release_kernel(const uint8_t* __restrict__ done, int32_t* __restrict__ lens, con
     const bool go = b < B && done[b] != 0;
     const int64_t n = go ? min(((int64_t)max(lens[b], 0) + page - 1) / page, (int64_t)width) : 0;
     int64_t sum;
-    const int64_t at = count + block_exclusive_sum(n, warp_sums, sum);
+    const int64_t at = count + block_exclusive_sum<kPlanThreads>(n, warp_sums, sum);
     first[threadIdx.x] = (int32_t)min(at, (int64_t)pool);
     pages[threadIdx.x] = (int32_t)n;
     if (go) lens[b] = 0;
@@ -194,9 +217,10 @@ int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t*
   const int cluster = max_tokens > 16384 ? 8 : max_tokens > 2048 || B > 256 ? 4 : 1;
   PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
              (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
-  const int smem = (int)(3 * 4 * B);
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(plan_step_kernel), smem)) return rc;
-  if (int rc = launch_chained(plan_step_kernel, dim3((unsigned)cluster), dim3(kPlanThreads), (size_t)smem, (cudaStream_t)stream, cluster, p))
+  const int smem = (int)(3 * 4 * B), threads = cluster == 8 ? 2 * kPlanThreads : kPlanThreads;
+  auto kern = cluster == 8 ? plan_step_kernel<2 * kPlanThreads> : plan_step_kernel<kPlanThreads>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
+  if (int rc = launch_chained(kern, dim3((unsigned)cluster), dim3((unsigned)threads), (size_t)smem, (cudaStream_t)stream, cluster, p))
     return rc;
   return check_launch("plan_step");
 }
