@@ -23,7 +23,7 @@ template <bool INT8> __device__ __forceinline__ uint4 kv8_encode(const float (&x
   for (int i = 0; i < 4; ++i) {
     const float a = __fmul_rn(x[4 * i], inv), b = __fmul_rn(x[4 * i + 1], inv), c = __fmul_rn(x[4 * i + 2], inv), d = __fmul_rn(x[4 * i + 3], inv);
     if constexpr (INT8) {
-      auto r = [](float v) { return __float2int_rn(fminf(fmaxf(v == v ? v : 0.f, -127.f), 127.f)); };
+      auto r = [](float v) { return max(__float2int_rn(v), -127); };      // (the conversion saturates, NaN gives 0; the pack saturates at 127)
       w[i] = pack_sat_s8(r(a), r(b), r(c), r(d));
     } else {
       w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |

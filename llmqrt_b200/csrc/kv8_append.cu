@@ -56,22 +56,17 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
     const int t0 = w0 + __ffs(runs) - 1;
     const int64_t s0 = p.slots[t0];
     const int row0 = (int)(s0 & (p.page - 1));
-    // length of the run: to the end of the page, or as far as the slots follow one another
-    int n = 1;
-    while (n < p.page - row0) {
-      const int i = n + lane;
-      const bool on = i < p.page - row0 && t0 + i < p.T && p.slots[t0 + i] == s0 + i;
-      const unsigned gap = ~__ballot_sync(0xffffffffu, on);
-      n += gap ? __ffs(gap) - 1 : 32;
-      if (gap) break;
-    }
     const int64_t page = s0 >> shift;
     uint8_t* tile = p.cache[kind] + page * p.page_stride + (int64_t)head * p.head_stride;
     float* scale = p.scale[kind] + page * p.Hkv + head;
     const bool rotated = kind == 0 && p.cos_tab != nullptr;
-    auto fetch = [&](int i, float (&x)[16]) {
+    auto load = [&](int i, bool on, uint4& lo, uint4& hi, int& at) {
       const T* src = static_cast<const T*>(p.fresh[kind]) + (int64_t)(t0 + i) * p.token_stride[kind] + head * D + piece * 8;
-      const uint4 lo = *reinterpret_cast<const uint4*>(src), hi = *reinterpret_cast<const uint4*>(src + D / 2);
+      lo = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+      hi = on ? *reinterpret_cast<const uint4*>(src + D / 2) : make_uint4(0, 0, 0, 0);
+      at = on && rotated ? p.positions[t0 + i] : -1;
+    };
+    auto turn = [&](const uint4& lo, const uint4& hi, int at, float (&x)[16]) {
       const uint32_t a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -79,35 +74,62 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
         x[2 * j] = f.x; x[2 * j + 1] = f.y;
         x[8 + 2 * j] = g.x; x[8 + 2 * j + 1] = g.y;
       }
-      if (rotated) {
-        const int at = p.positions[t0 + i];
-        if (at >= 0 && at < p.table_rows) {            // (outside the table: not rotated)
-          const float* cr = p.cos_tab + (int64_t)at * (D / 2) + piece * 8;
-          const float* sr = p.sin_tab + (int64_t)at * (D / 2) + piece * 8;
+      if (at >= 0 && at < p.table_rows) {              // (outside the table: not rotated)
+        const float* cr = p.cos_tab + (int64_t)at * (D / 2) + piece * 8;
+        const float* sr = p.sin_tab + (int64_t)at * (D / 2) + piece * 8;
 #pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const float4 c = *reinterpret_cast<const float4*>(cr + j), s = *reinterpret_cast<const float4*>(sr + j);
-            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+        for (int j = 0; j < 8; j += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(cr + j), s = *reinterpret_cast<const float4*>(sr + j);
+          const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {              // (two products and their sum, each rounded: no contraction)
-              const float u = x[j + e], v = x[8 + j + e];
-              x[j + e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(v, sn[e]));
-              x[8 + j + e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(v, cs[e]));
-            }
+          for (int e = 0; e < 4; ++e) {                // (two products and their sum, each rounded: no contraction)
+            const float u = x[j + e], v = x[8 + j + e];
+            x[j + e] = __fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(v, sn[e]));
+            x[8 + j + e] = __fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(v, cs[e]));
           }
         }
       }
     };
+    auto fetch = [&](int i, float (&x)[16]) {
+      uint4 lo, hi;
+      int at;
+      load(i, true, lo, hi, at);
+      turn(lo, hi, at, x);
+    };
+    // The first rows are asked for before the run's length is known, and kept.
+    constexpr int kKeep = 2;
+    const int most = min(p.page - row0, p.T - t0);
+    const float was = row0 > 0 ? *scale : 0.f;
+    uint4 lo[kKeep], hi[kKeep];
+    int at[kKeep];
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) load(sub + k * kRows, sub + k * kRows < most, lo[k], hi[k], at[k]);
+    // length of the run: to the end of the page, or as far as the slots follow one another
+    int n = 1;
+    while (n < most) {
+      const int i = n + lane;
+      const bool on = i < most && p.slots[t0 + i] == s0 + i;
+      const unsigned gap = ~__ballot_sync(0xffffffffu, on);
+      n += gap ? __ffs(gap) - 1 : 32;
+      if (gap) break;
+    }
+    float kept[kKeep][16];
     float top = 0.f;
-#pragma unroll 4
-    for (int i = sub; i < n; i += kRows) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      if (sub + k * kRows >= n) continue;
+      turn(lo[k], hi[k], at[k], kept[k]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(kept[k][j]));
+    }
+#pragma unroll 2
+    for (int i = sub + kKeep * kRows; i < n; i += kRows) {
       float x[16];
       fetch(i, x);
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[j]));
     }
     top = warp_max(top);
-    const float was = row0 > 0 ? *scale : 0.f;
     if constexpr (TEAM > 1) {                          // (two sets in turn: one barrier a run is enough, and none reads the old scale behind it)
       if (lane == 0) tops[nth & 1][warp] = top;
       __syncthreads();
@@ -116,13 +138,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
     }
     const float now = fmaxf(was, kv8_scale<INT8>(top)), inv = __fdiv_rn(1.f, now);
     // lane `piece` of a row holds elements 8 piece .. + 7 and D / 2 further: two 8-byte stores
-    for (int i = sub; i < n; i += kRows) {
-      float x[16];
-      fetch(i, x);
+    auto store = [&](int i, const float (&x)[16]) {
       const uint4 c = kv8_encode<INT8>(x, inv);
       uint8_t* dst = tile + (int64_t)(row0 + i) * D + piece * 8;
       *reinterpret_cast<uint2*>(dst) = make_uint2(c.x, c.y);
       *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(c.z, c.w);
+    };
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (sub + k * kRows < n) store(sub + k * kRows, kept[k]);
+    for (int i = sub + kKeep * kRows; i < n; i += kRows) {
+      float x[16];
+      fetch(i, x);
+      store(i, x);
     }
     if (now != was) {
       if (row0 > 0) {

@@ -5,7 +5,7 @@
 // order of the requests; then every new token has a slot, page number * page + row, and a position.
 //
 // Latency-bound (a step of 64 requests touches 3 KB): one launch of at most eight blocks, a cluster.  Each of them adds up
-// all requests for itself -- two scans, the second over what the first lets through -- and keeps the sums in shared memory;
+// all requests for itself -- tokens and pages at once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory;
 // tokens and table rows are then dealt out, a token finding its request by bisection.  The stack's count and the lengths
 // may be updated in place: nothing is written before every block of the cluster has read them.
 #include "common.cuh"
@@ -31,36 +31,42 @@ struct PlanArgs {
   int B, width, pool, page, max_tokens;
 };
 
-// Exclusive sum over the block's threads in thread order; the total comes back in `total`.
-template <int THREADS> __device__ __forceinline__ int64_t block_exclusive_sum(int64_t v, int64_t* warp_sums, int64_t& total) {
+// Exclusive sums over the block's threads in thread order, of two values at once; the totals come back beside them.
+template <int THREADS> __device__ __forceinline__ void block_exclusive_sums(int64_t a, int64_t b, longlong2* warp_sums, longlong2& before, longlong2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t s = v;
+  int64_t s = a, r = b;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t n = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += n;
+    const int64_t m = __shfl_up_sync(0xffffffffu, s, o), n = __shfl_up_sync(0xffffffffu, r, o);
+    if (lane >= o) {
+      s += m;
+      r += n;
+    }
   }
-  if (lane == 31) warp_sums[warp] = s;
+  if (lane == 31) warp_sums[warp] = make_longlong2(s, r);
   __syncthreads();
-  int64_t w = lane < THREADS / 32 ? warp_sums[lane] : 0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t n = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += n;
+  before = make_longlong2(s - a, r - b);
+  total = make_longlong2(0, 0);
+#pragma unroll 8
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const longlong2 v = warp_sums[w];
+    if (w < warp) {
+      before.x += v.x;
+      before.y += v.y;
+    }
+    total.x += v.x;
+    total.y += v.y;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
   __syncthreads();                                     // (the words may be used again)
-  return s - v + (warp > 0 ? before : 0);
 }
 
 template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kernel(PlanArgs p) {
   extern __shared__ int32_t plan_smem[];
-  __shared__ int64_t warp_sums[THREADS / 32];
+  __shared__ longlong2 warp_sums[THREADS / 32];
   int32_t* cu_s = plan_smem;                           // [B] first token of the request
   int32_t* ctx_s = cu_s + p.B;                         // [B] its context
   int32_t* off_s = ctx_s + p.B;                        // [B] its first page's place below the stack's top; -1: it gets nothing
-  const int cl = gridDim.x, rank = blockIdx.x;
+  const int cl = gridDim.x, rank = blockIdx.x, shift = __ffs(p.page) - 1;
   pdl_wait_then_trigger();
   const int64_t count = min(max(*p.free_count, 0), p.pool);
   __shared__ int32_t taken;
@@ -71,14 +77,22 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     const int b = b0 + threadIdx.x;
     const bool in = b < p.B;
     const int64_t ctx = in ? max(p.context[b], 0) : 0, n = in ? max(p.fresh[b], 0) : 0;
-    const int64_t have = (ctx + p.page - 1) / p.page, all = (ctx + n + p.page - 1) / p.page;
-    int64_t sum;
-    const int64_t cu = tokens + block_exclusive_sum<THREADS>(n, warp_sums, sum);
-    tokens += sum;
-    bool fits = cu + n <= p.max_tokens && all <= p.width;
-    const int64_t need = fits ? all - have : 0;
-    const int64_t off = wanted + block_exclusive_sum<THREADS>(need, warp_sums, sum);
-    wanted += sum;
+    const int64_t have = (ctx + p.page - 1) >> shift, all = (ctx + n + p.page - 1) >> shift;
+    // (where no request is turned down for its tokens, the pages' sum need not wait for the tokens')
+    bool fits = all <= p.width;
+    longlong2 before, sum, sum_again;
+    block_exclusive_sums<THREADS>(n, fits ? all - have : 0, warp_sums, before, sum);
+    const int64_t cu = tokens + before.x;
+    int64_t need = fits ? all - have : 0, off = wanted + before.y, sum_pages = sum.y;
+    if (tokens + sum.x > p.max_tokens) {
+      fits = fits && cu + n <= p.max_tokens;
+      need = fits ? all - have : 0;
+      block_exclusive_sums<THREADS>(need, 0, warp_sums, before, sum_again);
+      off = wanted + before.x;
+      sum_pages = sum_again.x;
+    }
+    tokens += sum.x;
+    wanted += sum_pages;
     fits = fits && (need == 0 || off + need <= count);
     // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
     if (fits && need) atomicMax(&taken, (int32_t)(off + need));
@@ -109,10 +123,9 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     const int off = off_s[b];
     if (off < 0) continue;
     const int n = (b + 1 < p.B ? cu_s[b + 1] : (int)tokens) - cu_s[b];
-    const int have = (int)(((int64_t)ctx_s[b] + p.page - 1) / p.page), all = (int)(((int64_t)ctx_s[b] + n + p.page - 1) / p.page);
+    const int have = (int)(((int64_t)ctx_s[b] + p.page - 1) >> shift), all = (int)(((int64_t)ctx_s[b] + n + p.page - 1) >> shift);
     for (int j = lane; j < all - have; j += 32) p.table[(int64_t)b * p.table_stride + have + j] = p.free_pages[count - 1 - off - j];
   }
-  const int shift = __ffs(p.page) - 1;
   // A warp has consecutive tokens, 32 kBatch at a time: a lane looks for its first one's request by bisection and goes on from there,
   // and kBatch look-ups are under way at once.
   constexpr int kBatch = 4;
@@ -164,21 +177,23 @@ __global__ void __launch_bounds__(kPlanThreads)
 release_kernel(const uint8_t* __restrict__ done, int32_t* __restrict__ lens, const int32_t* __restrict__ table,
                int64_t table_stride, int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count, int B, int width, int pool,
                int page) {
-  __shared__ int64_t warp_sums[kPlanThreads / 32];
+  __shared__ longlong2 warp_sums[kPlanThreads / 32];
   __shared__ int32_t first[kPlanThreads];
   __shared__ int32_t pages[kPlanThreads];
   pdl_wait_then_trigger();
+  const int shift = __ffs(page) - 1;
   int64_t count = min(max(*free_count, 0), pool);
   for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
     const int b = b0 + threadIdx.x;
     const bool go = b < B && done[b] != 0;
-    const int64_t n = go ? min(((int64_t)max(lens[b], 0) + page - 1) / page, (int64_t)width) : 0;
-    int64_t sum;
-    const int64_t at = count + block_exclusive_sum<kPlanThreads>(n, warp_sums, sum);
+    const int64_t n = go ? min((int64_t)(((int64_t)max(lens[b], 0) + page - 1) >> shift), (int64_t)width) : 0;
+    longlong2 before, sum;
+    block_exclusive_sums<kPlanThreads>(n, 0, warp_sums, before, sum);
+    const int64_t at = count + before.x;
     first[threadIdx.x] = (int32_t)min(at, (int64_t)pool);
     pages[threadIdx.x] = (int32_t)n;
     if (go) lens[b] = 0;
-    count = min(count + sum, (int64_t)pool);
+    count = min(count + (int64_t)sum.x, (int64_t)pool);
     __syncthreads();
     for (int r = threadIdx.x >> 5; r < min(kPlanThreads, B - b0); r += kPlanThreads / 32)
       for (int j = threadIdx.x & 31; j < pages[r]; j += 32)
