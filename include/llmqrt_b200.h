@@ -321,7 +321,7 @@ int llmqrt_attn_decode_step(const void* q, int64_t q_batch_stride, const void* k
 int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t* block_table, int64_t table_stride,
                      const int32_t* free_pages, const int32_t* free_count, int32_t* free_left, int32_t* seq_lens, int32_t* cu_new,
                      int64_t* slots, int32_t* positions, int64_t B, int64_t width, int64_t pool, int64_t page, int64_t max_tokens,
-                     llmqrt_stream_t stream);
+                     void* workspace, llmqrt_stream_t stream);
 
 /* The pages of the requests with done[b] != 0 go back onto the stack (which has room for `pool`) and their lengths become 0. */
 int llmqrt_release_pages(const uint8_t* done, int32_t* lens, const int32_t* block_table, int64_t table_stride, int32_t* free_pages,

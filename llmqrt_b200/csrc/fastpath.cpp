@@ -1146,7 +1146,8 @@ FAST_FN(plan_step) {
   Tensor positions = empty(ctx, {max_tokens}, at::kInt);
   auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(mptr(t)); };
   check(llmqrt_plan_step(i32(ctx), i32(fresh), i32(table), table_stride(table), i32(pages), i32(count), i32(left), i32(seq), i32(cu),
-                         static_cast<int64_t*>(mptr(slots)), i32(positions), B, table.size(1), pages.size(0), page, max_tokens, c.stream));
+                         static_cast<int64_t*>(mptr(slots)), i32(positions), B, table.size(1), pages.size(0), page, max_tokens, c.workspace(),
+                         c.stream));
   gil.done();
   return wrap_tuple(seq, cu, slots, positions);
   FAST_END

@@ -4,10 +4,13 @@
 // table, and is to get new[b] more.  The pages that this takes come from the top of a stack of free page numbers, in the
 // order of the requests; then every new token has a slot, page number * page + row, and a position.
 //
-// Latency-bound (a step of 64 requests touches 3 KB): one launch of at most eight blocks, a cluster.  Each of them adds up
+// Latency-bound (a step of 64 requests touches 3 KB): one launch, of one block, or where tokens are many of one for each 1024, of them
+// (a cluster of eight blocks took 13 us for 131072: their instructions, not their look-ups).  Each adds up
 // all requests for itself -- tokens and pages at once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory;
-// tokens and table rows are then dealt out, a token finding its request by bisection.  The stack's count and the lengths
-// may be updated in place: nothing is written before every block of the cluster has read them.
+// tokens and pages are then dealt out, each finding its request by bisection.  The stack's count and the lengths may be updated
+// in place: the last block to have read them writes them.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace llmqrt {
@@ -28,6 +31,7 @@ struct PlanArgs {
   int32_t* cu;                     // [B + 1]
   int64_t* slots;                  // [max_tokens]
   int32_t* positions;              // [max_tokens]
+  int* counter;                    // zero between calls; with several blocks
   int B, width, pool, page, max_tokens;
 };
 
@@ -64,8 +68,8 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
   extern __shared__ int32_t plan_smem[];
   __shared__ longlong2 warp_sums[THREADS / 32];
   int32_t* cu_s = plan_smem;                           // [B] first token of the request
-  int32_t* ctx_s = cu_s + p.B;                         // [B] its context
-  int32_t* off_s = ctx_s + p.B;                        // [B] its first page's place below the stack's top; -1: it gets nothing
+  int32_t* ctx_s = cu_s + p.B;                         // [B] its context; one that gets nothing: ~context
+  int32_t* off_s = ctx_s + p.B;                        // [B] its first new page's place below the stack's top (pages wanted before it)
   const int cl = gridDim.x, rank = blockIdx.x, shift = __ffs(p.page) - 1;
   pdl_wait_then_trigger();
   const int64_t count = min(max(*p.free_count, 0), p.pool);
@@ -98,20 +102,26 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     if (fits && need) atomicMax(&taken, (int32_t)(off + need));
     if (in) {
       cu_s[b] = (int32_t)min(cu, (int64_t)0x7fffffff);
-      ctx_s[b] = (int32_t)ctx;
-      off_s[b] = !fits ? -1 : need ? (int32_t)off : 0;
+      ctx_s[b] = fits ? (int32_t)ctx : ~(int32_t)ctx;
+      off_s[b] = (int32_t)min(off, (int64_t)0x7fffffff);
     }
   }
   __syncthreads();
-  if (cl > 1) {                                        // every block has read the lengths and the count
-    cluster_arrive();
-    cluster_wait();
+  bool last = cl == 1;
+  if (cl > 1) {
+    if (threadIdx.x == 0) {
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.counter) : "memory");
+      last = before == cl - 1;
+      if (last) *p.counter = 0;                        // as the next call wants it
+    }
+    last = __syncthreads_or(last);
   }
-  if (rank == 0) {
+  if (last) {                                          // every block has read the lengths and the count
     for (int b = threadIdx.x; b < p.B; b += THREADS) {
       const int32_t next = b + 1 < p.B ? cu_s[b + 1] : (int32_t)min(tokens, (int64_t)0x7fffffff);
       p.cu[b + 1] = next;
-      p.seq[b] = ctx_s[b] + (off_s[b] >= 0 ? next - cu_s[b] : 0);
+      p.seq[b] = ctx_s[b] >= 0 ? ctx_s[b] + next - cu_s[b] : ~ctx_s[b];
     }
     if (threadIdx.x == 0) {
       p.cu[0] = 0;
@@ -119,28 +129,22 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     }
   }
   const int lane = threadIdx.x & 31, warps = cl * (THREADS / 32);
-  for (int b = rank * (THREADS / 32) + (threadIdx.x >> 5); b < p.B; b += warps) {
-    const int off = off_s[b];
-    if (off < 0) continue;
-    const int n = (b + 1 < p.B ? cu_s[b + 1] : (int)tokens) - cu_s[b];
-    const int have = (int)(((int64_t)ctx_s[b] + p.page - 1) >> shift), all = (int)(((int64_t)ctx_s[b] + n + p.page - 1) >> shift);
-    for (int j = lane; j < all - have; j += 32) p.table[(int64_t)b * p.table_stride + have + j] = p.free_pages[count - 1 - off - j];
-  }
+  auto last_at_most = [&](const int32_t* first, int64_t i) {             // the last request whose first token, or page, is at most i
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
   // A warp has consecutive tokens, 32 kBatch at a time: a lane looks for its first one's request by bisection and goes on from there,
   // and kBatch look-ups are under way at once.
   constexpr int kBatch = 4;
   const int64_t all_tokens = min(tokens, (int64_t)p.max_tokens);
   const int64_t each = ((int64_t)p.max_tokens + warps * 32 * kBatch - 1) / (warps * 32 * kBatch) * (32 * kBatch);
   const int64_t begin = (rank * (THREADS / 32) + (threadIdx.x >> 5)) * each, end = min(begin + each, (int64_t)p.max_tokens);
-  int lo = 0;                                          // the last request whose first token is at most t
-  if (begin + lane < all_tokens) {
-    int hi = p.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu_s[mid] <= begin + lane) lo = mid;
-      else hi = mid;
-    }
-  }
+  int lo = begin + lane < all_tokens ? last_at_most(cu_s, begin + lane) : 0;
   for (int64_t t0 = begin + lane; t0 < end; t0 += 32 * kBatch) {
     int32_t position[kBatch];
     int id[kBatch];
@@ -151,12 +155,12 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
       id[i] = -1;
       if (t < all_tokens) {
         while (lo + 1 < p.B && cu_s[lo + 1] <= t) ++lo;
-        const int off = off_s[lo];
-        if (off >= 0) {
-          position[i] = ctx_s[lo] + (int32_t)(t - cu_s[lo]);
-          const int have = (int)(((int64_t)ctx_s[lo] + p.page - 1) >> shift), j = position[i] >> shift;
+        const int ctx = ctx_s[lo];
+        if (ctx >= 0) {
+          position[i] = ctx + (int32_t)(t - cu_s[lo]);
+          const int have = (int)(((int64_t)ctx + p.page - 1) >> shift), j = position[i] >> shift;
           // (a page taken in this step is read from the stack: another block may write the table's entry)
-          id[i] = j < have ? p.table[(int64_t)lo * p.table_stride + j] : p.free_pages[count - 1 - off - (j - have)];
+          id[i] = j < have ? p.table[(int64_t)lo * p.table_stride + j] : p.free_pages[count - 1 - off_s[lo] - (j - have)];
         }
       }
     }
@@ -168,6 +172,10 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
         p.positions[t] = position[i];
       }
     }
+  }
+  for (int i = rank * THREADS + threadIdx.x; i < taken; i += cl * THREADS) {
+    const int b = last_at_most(off_s, i), have = (int)(((int64_t)ctx_s[b] + p.page - 1) >> shift);
+    p.table[(int64_t)b * p.table_stride + have + i - off_s[b]] = p.free_pages[count - 1 - i];
   }
 }
 
@@ -224,19 +232,21 @@ extern "C" {
 int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t* block_table, int64_t table_stride,
                      const int32_t* free_pages, const int32_t* free_count, int32_t* free_left, int32_t* seq_lens, int32_t* cu_new,
                      int64_t* slots, int32_t* positions, int64_t B, int64_t width, int64_t pool, int64_t page, int64_t max_tokens,
-                     llmqrt_stream_t stream) {
+                     void* workspace, llmqrt_stream_t stream) {
   if (int rc = check_table("plan_step", block_table, table_stride, free_pages, free_count, B, width, pool, page)) return rc;
   LLMQRT_REQUIRE(max_tokens >= 0 && max_tokens < 0x7fffffffll, "plan_step: bad max_tokens");
   LLMQRT_REQUIRE(free_left && cu_new && (B == 0 || (context && new_tokens && seq_lens)) && (max_tokens == 0 || (slots && positions)),
                  "plan_step: null pointer");
-  const int cluster = max_tokens > 16384 ? 8 : max_tokens > 2048 || B > 256 ? 4 : 1;
+  // (a decode step wants few warps that wait for one another, a large one many look-ups under way)
+  const bool few = max_tokens <= 256 && B <= 128;
+  const int blocks = few ? 1 : (int)std::min<int64_t>(128, std::max<int64_t>(1, ceil_div(std::max(max_tokens, 4 * B), 1024)));
+  LLMQRT_REQUIRE(blocks == 1 || workspace, "plan_step: null workspace");
   PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
-             (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
-  const int smem = (int)(3 * 4 * B), threads = cluster == 8 ? 2 * kPlanThreads : kPlanThreads;
-  auto kern = cluster == 8 ? plan_step_kernel<2 * kPlanThreads> : plan_step_kernel<kPlanThreads>;
+             blocks > 1 ? ws_counters(workspace) : nullptr, (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
+  const int smem = (int)(3 * 4 * B), threads = few ? 128 : kPlanThreads;
+  auto kern = few ? plan_step_kernel<128> : plan_step_kernel<kPlanThreads>;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
-  if (int rc = launch_chained(kern, dim3((unsigned)cluster), dim3((unsigned)threads), (size_t)smem, (cudaStream_t)stream, cluster, p))
-    return rc;
+  if (int rc = launch_chained(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)smem, (cudaStream_t)stream, 1, p)) return rc;
   return check_launch("plan_step");
 }
 

@@ -112,7 +112,7 @@ def test_the_library_refuses():
     from llmqrt_b200 import _lib
 
     def plan(B=1, width=1, pool=1, page=16, most=1, p=64):
-        return _status("llmqrt_plan_step", p, p, p, width, p, p, p, p, p, p, p, B, width, pool, page, most, None)
+        return _status("llmqrt_plan_step", p, p, p, width, p, p, p, p, p, p, p, B, width, pool, page, most, None, None)
     for kw in (dict(page=8), dict(page=48), dict(page=256), dict(B=8193), dict(B=-1), dict(width=2 ** 28), dict(most=-1), dict(p=None)):
         assert plan(**kw) == -1, kw
 
