@@ -6,19 +6,24 @@
 // A page's scale thus only grows while it fills, and a page whose first row is written starts afresh.  Rows behind the run
 // stay as they were.  Keys are rotated first, if tables are given; nothing is rounded in between.
 //
-// A warp does one run of one head, of the keys or of the values: eight lanes (d = 64: four) hold a row, sixteen elements
-// each -- eight and the eight half a head away, the rotation's pairs -- so that two 16-byte loads fetch them and one
-// pass over the run finds the maximum, a second (whose reads come from L1) the codes.  No other warp touches
+// A team of warps does one run of one head, of the keys or of the values: eight lanes (d = 64: four) hold a row, sixteen elements
+// each -- eight and the eight half a head away, the rotation's pairs.  The first rows are asked for before the run's length is known
+// and stay in registers; those behind them are read once for the maximum and again (from L1) for their codes.  Nobody else touches
 // these codes or their scale, so there are no atomics and the result is the same on every run.
 //
-// A block looks for runs in a window of the call's tokens, one window for each head, keys and values; its warps take the runs
-// in turn.  Windows are short where the call is small: a decode step's tokens are runs of their own, each wants a warp.
+// A block looks for runs in a window of the call's tokens, one window for each head, keys and values.  A decode step's tokens are runs
+// of their own: a warp each, four to a window.  Of many tokens a window has 32, and the block's two warps take each run together.
+//
+// Bound by its chain of loads (slots, rows and positions, angles) and by 20 instructions an element, at half of what the schedulers
+// could issue: 17600 tokens of 4 heads of 128 take 17 us with their rows in L2 and 23 without, 54 MB at 2.5 TB/s of 6.5.
+// (A warp a run: 33 us; four warps: 18; eight: 26, as what a run costs before its rows is paid by each of them.)
 #include "kv8.cuh"
 
 namespace llmqrt {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;                              // a warp a run
+constexpr int kTeam = 2;                               // that share a run
 
 struct AppendArgs {
   uint8_t* cache[2];               // keys, values: [pages, Hkv, page, d]
@@ -34,11 +39,11 @@ struct AppendArgs {
   int T, Hkv, page, table_rows, window;
 };
 
-// TEAM: warps that share a run, 1 or all of the block's.
+// TEAM: warps that share a run: 1, or all of the block's.
 template <typename T, int D, bool INT8, int TEAM>
-__global__ void __launch_bounds__(kWarps * 32) kv8_append_kernel(AppendArgs p) {
+__global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ? 20 / TEAM : 5) kv8_append_kernel(AppendArgs p) {
   constexpr int kLanes = D / 16, kRows = 32 / kLanes * TEAM;             // lanes of a row, rows that are taken at once
-  __shared__ float tops[2][kWarps];
+  __shared__ float tops[2][TEAM];
   pdl_wait_then_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, kind = blockIdx.z;
   const int piece = lane % kLanes, sub = lane / kLanes + (TEAM > 1 ? warp * (32 / kLanes) : 0);
@@ -205,15 +210,15 @@ extern "C" int llmqrt_kv8_append(void* k_cache, void* v_cache, float* k_scale, f
   a.slots = slots; a.cos_tab = cos_table; a.sin_tab = sin_table; a.positions = positions;
   a.num_slots = pages * page;
   a.T = (int)T; a.Hkv = (int)Hkv; a.page = (int)page; a.table_rows = (int)table_rows;
-  // (at 64 tokens a warp a run)
+  // (64 tokens of a decode step: 2.6 us with a warp each)
   const bool team = T > 2048;
   a.window = team ? 32 : kWarps;
   const dim3 grid((unsigned)ceil_div(T, a.window), (unsigned)Hkv, 2);
-  auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
+  auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(team ? kTeam * 32 : kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
   const bool i8 = cache_type == LLMQRT_I8;
   auto pick = [&](auto tag) {
     using T_ = decltype(tag);
-#define LLMQRT_APPEND(D_, I_) (team ? go(kv8_append_kernel<T_, D_, I_, kWarps>) : go(kv8_append_kernel<T_, D_, I_, 1>))
+#define LLMQRT_APPEND(D_, I_) (team ? go(kv8_append_kernel<T_, D_, I_, kTeam>) : go(kv8_append_kernel<T_, D_, I_, 1>))
     return d == 128 ? (i8 ? LLMQRT_APPEND(128, true) : LLMQRT_APPEND(128, false)) : (i8 ? LLMQRT_APPEND(64, true) : LLMQRT_APPEND(64, false));
 #undef LLMQRT_APPEND
   };

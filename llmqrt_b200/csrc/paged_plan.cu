@@ -4,11 +4,12 @@
 // table, and is to get new[b] more.  The pages that this takes come from the top of a stack of free page numbers, in the
 // order of the requests; then every new token has a slot, page number * page + row, and a position.
 //
-// Latency-bound (a step of 64 requests touches 3 KB): one launch, of one block, or where tokens are many of one for each 1024, of them
-// (a cluster of eight blocks took 13 us for 131072: their instructions, not their look-ups).  Each adds up
-// all requests for itself -- tokens and pages at once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory;
-// tokens and pages are then dealt out, each finding its request by bisection.  The stack's count and the lengths may be updated
-// in place: the last block to have read them writes them.
+// Latency-bound (a step of 64 requests touches 3 KB): one launch.  Each block adds up all requests for itself -- tokens and pages at
+// once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory; tokens and pages are then
+// dealt out, each finding its request by bisection.  The stack's count and the lengths may be updated in place: the last block to
+// have read them writes them.
+// On the GPU 5.6 us for 64 requests of one token (four warps, which wait for one another less than sixteen) and 5.8 us for 131072
+// tokens of 333 requests, 128 blocks (a cluster of eight, which the instructions of a token bound: 13 us).
 #include <algorithm>
 
 #include "common.cuh"
