@@ -522,6 +522,13 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
             l_run[h][c] += e;
             pv[h][kb][c] = e * v_share;
           }
+      if (key0 + 16 > sees_all) {                        // (whatever the scale of a page that the row does not see)
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key0 + 8 * (i >> 1) + g >= sees[h][i & 1]) pv[h][i >> 1][i & 1] = 0.f;
+      }
       uint32_t pa[G][2], pr[G][2];                       // of row g: keys 2t, 2t + 1 and 2t + 8, 2t + 9
 #pragma unroll
       for (int h = 0; h < G; ++h)
@@ -943,7 +950,7 @@ extern "C" int llmqrt_attn_decode_kv8(const void* q, int64_t q_batch_stride, int
   a.table_rows = (int)table_rows; a.out = static_cast<uint16_t*>(out);
   a.Sq = (int)Sq; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.pages = (int)pages; a.page = (int)page;
   const int64_t most = max_seqlen < width * page ? max_seqlen : width * page;
-  LLMQRT_REQUIRE(most <= 0x7ffffff0ll, "attn_decode_kv8: sequences too long");
+  LLMQRT_REQUIRE(most <= 0x7fff0000ll, "attn_decode_kv8: sequences too long");      // (keys a few steps ahead are 32-bit numbers)
   a.max_len = pages == 0 ? 0 : (int)most;
   a.scale = 1.0f / sqrtf((float)d);
   a.softcap = softcap;

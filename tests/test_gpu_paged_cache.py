@@ -510,6 +510,19 @@ def test_attend_keeps_nan_with_the_rows_that_see_it(d, Hq, Hkv, dt):
     assert torch.isnan(out[bad]).all() and bits_equal(torch.where(bad, torch.zeros_like(out), out), torch.where(bad, torch.zeros_like(out), clean))
 
 
+def test_attend_keeps_a_bad_scale_with_the_rows_that_see_it():
+    """A page whose scales are NaN and that only the last token sees."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    g = _gen(16)
+    kc, vc, ks, vs = _cache(g, "int8", 4, 2, 16, 64)
+    q = torch.randn(1, 3, 8, 64, generator=g, device="cuda").half()
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    clean = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32([49]), 64)
+    ks[3], vs[3] = float("nan"), float("nan")
+    out = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32([49]), 64)
+    assert torch.isnan(out[0, 2]).all() and bits_equal(out[0, :2], clean[0, :2])
+
+
 def test_attend_beyond_32_bits():
     """A cache whose pages lie more than 2^32 bytes apart."""
     from llmqrt_b200.paged_cache import attn_decode_kv8, kv8_append
