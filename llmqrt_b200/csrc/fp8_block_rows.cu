@@ -10,6 +10,9 @@
 // and t = h * w, a product of two 16-bit values and therefore exact in fp32, y = t / sqrt(mean(h^2) + eps): the root divides
 // the group's maximum like every element of it and cancels, q = e4m3(t * (448 / max |t|)), and only the scale carries it.
 // (glue.cu's norm rounds to T twice on the way, as the reference's does; its int8 scale is one per row.)
+//
+// HBM-bound where rows are many: 8191 rows of 3584 with a residual take 37.7 us, 5.5 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us
+// of the GPU, the call 7 with its three allocations.
 #include "common.cuh"
 
 namespace llmqrt {

@@ -7,16 +7,17 @@
 // stay as they were.  Keys are rotated first, if tables are given; nothing is rounded in between.
 //
 // A team of warps does one run of one head, of the keys or of the values: eight lanes (d = 64: four) hold a row, sixteen elements
-// each -- eight and the eight half a head away, the rotation's pairs.  The first rows are asked for before the run's length is known
-// and stay in registers; those behind them are read once for the maximum and again (from L1) for their codes.  Nobody else touches
-// these codes or their scale, so there are no atomics and the result is the same on every run.
+// each -- eight and the eight half a head away, the rotation's pairs.  The first rows (four a lane where teams share a run) are asked
+// for before the run's length is known and stay in registers as they came; those behind them are read once for the maximum and
+// again (from L1) for their codes.  Nobody else touches these codes or their scale, so there are no atomics and the result is the same
+// on every run.
 //
 // A block looks for runs in a window of the call's tokens, one window for each head, keys and values.  A decode step's tokens are runs
 // of their own: a warp each, four to a window.  Of many tokens a window has 32, and the block's two warps take each run together.
 //
-// Bound by its chain of loads (slots, rows and positions, angles) and by 20 instructions an element, at half of what the schedulers
-// could issue: 17600 tokens of 4 heads of 128 take 17 us with their rows in L2 and 23 without, 54 MB at 2.5 TB/s of 6.5.
-// (A warp a run: 33 us; four warps: 18; eight: 26, as what a run costs before its rows is paid by each of them.)
+// Bound by its chain of loads (slots, rows and positions, angles; 18 warps an SM) and 17 instructions an element, at half of what the
+// schedulers could issue: 17600 tokens of 4 heads of 128 take 17 us with their rows in L2 and 21 without, 58 MB at 2.7 TB/s of 6.5.
+// (A warp a run: 33 us; four warps: 18 and 24; eight: 26, as what a run costs before its rows is paid by each of them.)
 #include "kv8.cuh"
 
 namespace llmqrt {
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
       turn(lo, hi, at, x);
     };
     // The first rows are asked for before the run's length is known, and kept.
-    constexpr int kKeep = 2;
+    constexpr int kKeep = TEAM == 1 ? 1 : 4;
     const int most = min(p.page - row0, p.T - t0);
     const float was = row0 > 0 ? *scale : 0.f;
     uint4 lo[kKeep], hi[kKeep];
@@ -118,14 +119,14 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
       n += gap ? __ffs(gap) - 1 : 32;
       if (gap) break;
     }
-    float kept[kKeep][16];
     float top = 0.f;
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
       if (sub + k * kRows >= n) continue;
-      turn(lo[k], hi[k], at[k], kept[k]);
+      float x[16];
+      turn(lo[k], hi[k], at[k], x);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(kept[k][j]));
+      for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[j]));
     }
 #pragma unroll 2
     for (int i = sub + kKeep * kRows; i < n; i += kRows) {
@@ -151,7 +152,11 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
     };
 #pragma unroll
     for (int k = 0; k < kKeep; ++k)
-      if (sub + k * kRows < n) store(sub + k * kRows, kept[k]);
+      if (sub + k * kRows < n) {                       // (turned once more: as fp32 they would take twice the registers)
+        float x[16];
+        turn(lo[k], hi[k], at[k], x);
+        store(sub + k * kRows, x);
+      }
     for (int i = sub + kKeep * kRows; i < n; i += kRows) {
       float x[16];
       fetch(i, x);
