@@ -16,6 +16,8 @@
 //   block_split_kernel  few tokens: weights are the 128-lane operand (128 rows: one row of scales), the tokens the 16 .. 128
 //                       columns, and the reduction is shared out to a cluster, whose CTAs add their sums up through
 //                       distributed shared memory in rank order.
+// Measured: 64 x 37888 x 3584 29 us (HBM alone 21.5), 1 x 4864 x 896 5.3 us; 4096 x 3584 x 18944 295 us, 1.9 PFLOP/s, where the
+// tensor cores alone take 180 at the rate that the board's 1000 W leave them: every K block's sums pass through registers.
 // All waits are bounded as in gemm_tc.cu.
 #include "gemm_w8a8.cuh"
 #include "tc_tiles.cuh"
@@ -63,7 +65,11 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster
 __device__ __forceinline__ void load_now(const float* p, float& v) { asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p)); }
 
 // ---- few tokens --------------------------------------------------------------------------------------
-constexpr int kSplitThreads = 192;                     // TMA warp, MMA warp, four epilogue warps
+// TMA warp, MMA warp, and four epilogue warps for each 32 tokens: with four for all of them they bound 128 tokens, 1370 cycles a
+// K block whose weights come in 700 (37888 x 3584: 44.2 us, now 37.1; 64 tokens 30.4 and 29.3).  What is left grows with the
+// activations, which each tile of 128 weight rows fetches from L2 again: with the weights 7 TB/s (one token: 25.1 us, 5.4 TB/s).
+template <int BN> constexpr int split_groups() { return BN <= 32 ? 1 : BN / 32; }
+template <int BN> constexpr int split_threads() { return 64 + 128 * split_groups<BN>(); }
 constexpr int kSplitBufs = 4;                          // accumulators of BN columns
 template <int BN> constexpr int split_stage_bytes() { return (kBM + BN) * kRowBytes; }
 template <int BN> constexpr int split_stages() {
@@ -77,11 +83,11 @@ __device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[32]) { tc
 __device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[16]) { tc::tmem_ld_32x16(taddr, r); }
 
 template <int BN>
-__global__ void __launch_bounds__(kSplitThreads, 1)
+__global__ void __launch_bounds__(split_threads<BN>(), 1)
 block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const BlockParams prm) {
   constexpr int kStages = split_stages<BN>(), kStageBytes = split_stage_bytes<BN>();
-  constexpr int kPer = BN < 32 ? 1 : BN / 32;          // token scales a lane fetches
-  constexpr int kChunk = BN < 32 ? BN : 32;            // columns a tcgen05.ld takes
+  constexpr int kCols = BN < 32 ? BN : 32;             // columns (tokens) of an epilogue warp
+  constexpr int kGroups = split_groups<BN>(), kEpilogues = 4 * kGroups;
   static_assert(kStages * kStageBytes >= BN * kBM * 4, "the ring holds the partial sums");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -89,7 +95,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   __shared__ __align__(8) uint64_t bar_empty[kStages];
   __shared__ __align__(8) uint64_t bar_acc_full[kSplitBufs];
   __shared__ __align__(8) uint64_t bar_acc_empty[kSplitBufs];
-  __shared__ __align__(16) float scales[4][2][BN];     // each epilogue warp's own: the tokens' scales of a K block
+  __shared__ __align__(16) float scales[kEpilogues][2][kCols];           // each epilogue warp's own: the tokens' scales of a K block
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -105,7 +111,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     }
     for (int b = 0; b < kSplitBufs; ++b) {
       tc::mbar_init(tc::smem_u32(&bar_acc_full[b]), 1);
-      tc::mbar_init(tc::smem_u32(&bar_acc_empty[b]), 4);
+      tc::mbar_init(tc::smem_u32(&bar_acc_empty[b]), kEpilogues);
     }
     tc::mbar_fence_init();
     tc::tma_prefetch_descriptor(&tm_w);
@@ -129,8 +135,8 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   const int kb_begin = (int)((int64_t)rank * prm.k_blocks / S);
   const int kb_count = (int)((int64_t)(rank + 1) * prm.k_blocks / S) - kb_begin;
 
-  F2 acc[BN / 2];                                      // epilogue: row quad * 32 + lane of the tile, all tokens
-  const int quad = warp & 3, wrow = quad * 32 + lane;
+  F2 acc[kCols / 2];                                   // epilogue: row quad * 32 + lane of the tile, tokens from c_begin on
+  const int quad = warp & 3, wrow = quad * 32 + lane, c_begin = (warp - 2) / 4 * kCols;
   const float* a_scale = prm.a_scale;
 
   if (warp == 0) {
@@ -208,66 +214,50 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
       const int tp = tile / prm.tiles_q, tq = tile % prm.tiles_q;
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) acc[i] = f2(0.f, 0.f);
+      for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
+      // (tokens behind the last one: any valid scale, their columns are not written)
       const float* ws = prm.w_scale + (int64_t)tp * prm.k_blocks + kb_begin;
-      const float* as[kPer];
-      float next[kPer], w_next;
+      const float* as = a_scale + (int64_t)min(tq * BN + c_begin + lane, prm.M - 1) * prm.k_blocks + kb_begin;
+      float next, w_next;
       load_now(ws, w_next);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {                 // (tokens behind the last one: any valid scale, their columns are not written)
-        as[i] = a_scale + (int64_t)min(tq * BN + i * 32 + lane, prm.M - 1) * prm.k_blocks + kb_begin;
-        load_now(as[i], next[i]);
-      }
+      load_now(as, next);
 #pragma unroll 1
       for (int it = 0; it < kb_count; ++it) {
         float* mine = scales[warp - 2][it & 1];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (BN >= 32 || lane < BN) mine[i * 32 + lane] = __fmul_rn(next[i], w_next);
+        if (kCols == 32 || lane < kCols) mine[lane] = __fmul_rn(next, w_next);
         const int ahead = min(it + 1, kb_count - 1);
         load_now(ws + ahead, w_next);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) load_now(as[i] + ahead, next[i]);
+        load_now(as + ahead, next);
         if (!ready) tc::mbar_wait_or_flag(tc::smem_u32(&bar_acc_full[buf]), acc_phase, abort_u32);
         __syncwarp();
         tc::fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN), empty = tc::smem_u32(&bar_acc_empty[buf]);
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + c_begin), empty = tc::smem_u32(&bar_acc_empty[buf]);
         if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
-        uint32_t r[2][kChunk];
-        ld_chunk(taddr, r[0]);
+        uint32_t v[kCols];
+        ld_chunk(taddr, v);
+        // (whether the next block's accumulator is complete is asked for ahead: the answer takes 100 cycles, be it yes)
+        ready = tc::mbar_test_wait(tc::smem_u32(&bar_acc_full[buf]), acc_phase);
+        tc::tmem_ld_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(empty);
 #pragma unroll
-        for (int c0 = 0; c0 < BN; c0 += kChunk) {
-          uint32_t(&v)[kChunk] = r[c0 / kChunk & 1];
-          // (whether the next block's accumulator is complete is asked for ahead: the answer takes 100 cycles, be it yes)
-          if (c0 + kChunk == BN) ready = tc::mbar_test_wait(tc::smem_u32(&bar_acc_full[buf]), acc_phase);
-          tc::tmem_ld_wait();
-          if (c0 + kChunk < BN) {
-            ld_chunk(taddr + (uint32_t)(c0 + kChunk), r[(c0 / kChunk + 1) & 1]);
-          } else {
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(empty);
-          }
-#pragma unroll
-          for (int c = 0; c < kChunk; c += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(mine + c0 + c);
-            F2& lo = acc[(c0 + c) / 2];
-            F2& hi = acc[(c0 + c) / 2 + 1];
-            lo = f2_fma(f2_of(v[c], v[c + 1]), f2(s.x, s.y), lo);
-            hi = f2_fma(f2_of(v[c + 2], v[c + 3]), f2(s.z, s.w), hi);
-          }
+        for (int c = 0; c < kCols; c += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(mine + c);
+          acc[c / 2] = f2_fma(f2_of(v[c], v[c + 1]), f2(s.x, s.y), acc[c / 2]);
+          acc[c / 2 + 1] = f2_fma(f2_of(v[c + 2], v[c + 3]), f2(s.z, s.w), acc[c / 2 + 1]);
         }
       }
       if (tc::warp_aborted(abort)) break;
       if (S == 1) {                                    // straight from registers: a warp writes 32 neighbours of a token's row
-        const int n = tp * kBM + wrow, tokens = min(BN, prm.M - tq * BN);
+        const int n = tp * kBM + wrow, m0 = tq * BN + c_begin, tokens = min(kCols, prm.M - m0);
         if (n < prm.N) {
           const float b = prm.bias ? load_as_f32(prm.bias, n, prm.bias_dtype) : 0.f;
 #pragma unroll
-          for (int i = 0; i < BN; ++i) {
+          for (int i = 0; i < kCols; ++i) {
             float lo, hi;
             f2_split(acc[i / 2], lo, hi);
-            if (i < tokens) store_from_f32(prm.out, (int64_t)(tq * BN + i) * prm.ldo + n, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, (i & 1 ? hi : lo) + b);
+            if (i < tokens) store_from_f32(prm.out, (int64_t)(m0 + i) * prm.ldo + n, prm.bf16 ? LLMQRT_BF16 : LLMQRT_F16, (i & 1 ? hi : lo) + b);
           }
         }
       }
@@ -282,10 +272,10 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     __syncthreads();
     if (warp >= 2) {
 #pragma unroll
-      for (int i = 0; i < BN; ++i) {
+      for (int i = 0; i < kCols; ++i) {
         float lo, hi;
         f2_split(acc[i / 2], lo, hi);
-        if (i < tokens) part[i * kBM + wrow] = i & 1 ? hi : lo;
+        if (c_begin + i < tokens) part[(c_begin + i) * kBM + wrow] = i & 1 ? hi : lo;
       }
     }
     cluster_sync_all();
@@ -295,7 +285,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
 #pragma unroll
       for (int j = 0; j < 4; ++j) b[j] = prm.bias && n + j < prm.N ? load_as_f32(prm.bias, n + j, prm.bias_dtype) : 0.f;
       const bool wide = n + 4 <= prm.N && prm.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 7) == 0;
-      for (int m = rank * tokens / S + warp - 2; m < m1; m += 4) {
+      for (int m = rank * tokens / S + warp - 2; m < m1; m += kEpilogues) {
         const uint32_t local = tc::smem_u32(part + m * kBM + lane * 4);
         float4 v[kMaxCluster];
 #pragma unroll
@@ -713,7 +703,7 @@ template <int BN> const int* split_clusters() {
   static const int none[kMaxCluster + 1] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return none;
-  std::call_once(once[dev], [dev] { ask_clusters(block_split_kernel<BN>, kSplitThreads, split_smem<BN>(), 1, kMaxCluster, known[dev]); });
+  std::call_once(once[dev], [dev] { ask_clusters(block_split_kernel<BN>, split_threads<BN>(), split_smem<BN>(), 1, kMaxCluster, known[dev]); });
   return known[dev];
 }
 template <int BN> int pair_clusters() {
@@ -785,7 +775,7 @@ int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), split_smem<BN>())) return rc;
   const int64_t grid = prm.splits > 1 ? tiles * prm.splits : std::min(tiles, (int64_t)sm_count());
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = config(kern, (int)grid, prm.splits, kSplitThreads, split_smem<BN>(), st, attr);
+  cudaLaunchConfig_t cfg = config(kern, (int)grid, prm.splits, split_threads<BN>(), split_smem<BN>(), st, attr);
   LLMQRT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, prm));
   return check_launch("fp8 block linear");
 }
