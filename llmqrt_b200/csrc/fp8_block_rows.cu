@@ -11,8 +11,11 @@
 // the group's maximum like every element of it and cancels, q = e4m3(t * (448 / max |t|)), and only the scale carries it.
 // (glue.cu's norm rounds to T twice on the way, as the reference's does; its int8 scale is one per row.)
 //
-// HBM-bound where rows are many: 8191 rows of 3584 with a residual take 37.7 us, 5.5 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us
-// of the GPU, the call 7 with its three allocations.
+// HBM-bound where rows are many, once a lane works out the factor of one of its units only and passes it on (the divisions, of all
+// of them in every lane, held the schedulers at 3/4 of their rate: 37.7 us): 8191 rows of 3584 with a residual take 33 us back to back
+// and 36 among others, 6.2 and 5.7 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us of the GPU, the call 7 with its three allocations.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace llmqrt {
@@ -43,6 +46,13 @@ template <typename T> __device__ __forceinline__ void unpack8(const uint4& v, fl
     f[2 * p] = x.x;
     f[2 * p + 1] = x.y;
   }
+}
+
+// Two sums, each rounded once to T.
+template <typename T> __device__ __forceinline__ uint32_t add_pairs(uint32_t a, uint32_t b) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2 s = __hadd2(*reinterpret_cast<const T2*>(&a), *reinterpret_cast<const T2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&s);
 }
 
 // Unit-slot i of the matrix: row i / (16 groups), unit i % (16 groups); slots behind a row's last unit are empty.
@@ -106,10 +116,7 @@ rmsnorm_fp8_block_kernel(const T* __restrict__ x, int64_t ldx, const T* __restri
         const uint32_t a[4] = {hv[k].x, hv[k].y, hv[k].z, hv[k].w}, b[4] = {rv[k].x, rv[k].y, rv[k].z, rv[k].w};
         uint32_t s[4];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float2 f = unpack_pair<T>(a[p]), g = unpack_pair<T>(b[p]);
-          s[p] = pack_pair<T>(f.x + g.x, f.y + g.y);
-        }
+        for (int p = 0; p < 4; ++p) s[p] = add_pairs<T>(a[p], b[p]);
         hv[k] = make_uint4(s[0], s[1], s[2], s[3]);
         const int u = threadIdx.x + k * blockDim.x;
         if (u < units) *reinterpret_cast<uint4*>(h_out + m * H + u * 8) = hv[k];
@@ -129,27 +136,32 @@ rmsnorm_fp8_block_kernel(const T* __restrict__ x, int64_t ldx, const T* __restri
   float ss = 0.f;
   for (int w = lane; w < U * nwarps; w += 32) ss += red[w];
   const float rstd = rsqrtf(warp_sum(ss) / (float)H + eps);
+  float t[U][8], top = 0.f;
+  const int mine = lane & (U - 1);                     // the unit whose group's factor and scale the lane works out
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const int u = threadIdx.x + k * blockDim.x;
-    if (!__any_sync(0xffffffffu, u < units)) break;    // (the whole warp)
-    float t[8], top = 0.f;
-    unpack8<T>(hv[k], t);
-    {
-      float w[8];
-      unpack8<T>(u < units ? *reinterpret_cast<const uint4*>(weight + u * 8) : make_uint4(0, 0, 0, 0), w);
+    float w[8], top_k = 0.f;
+    unpack8<T>(hv[k], t[k]);
+    unpack8<T>(u < units ? *reinterpret_cast<const uint4*>(weight + u * 8) : make_uint4(0, 0, 0, 0), w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        t[j] = __fmul_rn(t[j], w[j]);
-        top = fmaxf(top, fabsf(t[j]));
-      }
+    for (int j = 0; j < 8; ++j) {
+      t[k][j] = __fmul_rn(t[k][j], w[j]);
+      top_k = fmaxf(top_k, fabsf(t[k][j]));
     }
-    top = half_warp_max(top);
-    const float y = __fmul_rn(top, rstd);
-    const bool above = y >= kFloor;                    // (no: a row with an infinity or a NaN, or a group of next to nothing)
-    const float c = above ? __fdiv_rn(kE4m3Max, top) : __fmul_rn(rstd, kE4m3Max / kFloor);
-    if (u < units) *reinterpret_cast<uint2*>(q + m * H + u * 8) = to_e4m3x8(t, c);
-    if (u < units && u % kGroupUnits == 0) scale[m * groups + u / kGroupUnits] = __fdiv_rn(above ? y : kFloor, kE4m3Max);
+    top_k = half_warp_max(top_k);
+    if (k == mine) top = top_k;
+  }
+  const float y = __fmul_rn(top, rstd);
+  const bool above = y >= kFloor;                      // (no: a row with an infinity or a NaN, or a group of next to nothing)
+  const float c_mine = above ? __fdiv_rn(kE4m3Max, top) : __fmul_rn(rstd, kE4m3Max / kFloor);
+  const int in_group = lane & (kGroupUnits - 1), u_mine = (int)threadIdx.x - in_group + in_group * (int)blockDim.x;
+  if (in_group < U && u_mine < units) scale[m * groups + u_mine / kGroupUnits] = __fdiv_rn(above ? y : kFloor, kE4m3Max);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int u = threadIdx.x + k * blockDim.x;
+    const float c = __shfl_sync(0xffffffffu, c_mine, lane - mine + k);
+    if (u < units) *reinterpret_cast<uint2*>(q + m * H + u * 8) = to_e4m3x8(t[k], c);
   }
 }
 
