@@ -486,6 +486,27 @@ def test_attend_shares(lens, Hq, Hkv, Sq, top):
     _check_attend(lens, 16, Hq, Hkv, 64, Sq, "int8", torch.float16, top=top, width=-(-top // 16))
 
 
+def test_attend_many_sequences():
+    """So many sequences that their keys, laid end to end, pass what 32-bit products hold; all of them share the same pages."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    g = _gen(17)
+    B, n = 60000, 1900
+    kc, vc, ks, vs = _cache(g, "int8", 119, 1, 16, 64)
+    table = torch.randperm(119, generator=g, device="cuda").int().expand(B, 119)[:, :119]
+    table = table.contiguous()
+    lens = torch.randint(1, n + 1, (B,), generator=g, device="cuda").int()
+    lens[::3] = n
+    lens[[5, 4000, B - 2]] = 0
+    q = torch.randn(B, 2, 64, generator=g, device="cuda").half()
+    out = attn_decode_kv8(q, kc, vc, ks, vs, table, lens, 9000)
+    some = torch.cat([torch.arange(0, B, 997, device="cuda"), torch.tensor([5, 4000, B - 2, B - 1], device="cuda")])
+    want = _attend(q[some][:, None], kc, vc, ks, vs, table[some], lens[some].tolist(), 9000, 0.0, None, None)[:, 0]
+    assert rel_fro(out[some], want) < 2.0 ** -11 + 2.0 ** -16 and (out[[5, 4000, B - 2]] == 0).all()
+    # (what a call of a part of them gives, whose blocks cut the sequences elsewhere: each off by its own rounding, 2^-11)
+    parts = torch.cat([attn_decode_kv8(q[i:i + 7000], kc, vc, ks, vs, table[i:i + 7000], lens[i:i + 7000], n) for i in range(0, B, 7000)])
+    assert rel_fro(out, parts) < 2 * (2.0 ** -11 + 2.0 ** -16)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("Hq,Hkv", [(2, 1), (16, 2), (24, 2)])
 @pytest.mark.parametrize("dt", ["fp16", "bf16"])
