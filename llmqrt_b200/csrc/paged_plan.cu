@@ -8,8 +8,8 @@
 // once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory; tokens and pages are then
 // dealt out, each finding its request by bisection.  The stack's count and the lengths may be updated in place: the last block to
 // have read them writes them.
-// On the GPU 5.6 us for 64 requests of one token (four warps, which wait for one another less than sixteen) and 5.8 us for 131072
-// tokens of 333 requests, 128 blocks (a cluster of eight, which the instructions of a token bound: 13 us).
+// On the GPU 3.8 us for 64 requests of one token (four warps, which wait for one another less than sixteen: 5.6), 5.9 us for 131072
+// tokens of 333 requests, 128 blocks (a cluster of eight, which the instructions of a token bound: 13 us), 16 us for 8192 requests.
 #include <algorithm>
 
 #include "common.cuh"
@@ -52,20 +52,39 @@ template <int THREADS> __device__ __forceinline__ void block_exclusive_sums(int6
   __syncthreads();
   before = make_longlong2(s - a, r - b);
   total = make_longlong2(0, 0);
-#pragma unroll 8
-  for (int w = 0; w < THREADS / 32; ++w) {
-    const longlong2 v = warp_sums[w];
-    if (w < warp) {
-      before.x += v.x;
-      before.y += v.y;
+  if constexpr (THREADS <= 128) {
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      const longlong2 v = warp_sums[w];
+      if (w < warp) {
+        before.x += v.x;
+        before.y += v.y;
+      }
+      total.x += v.x;
+      total.y += v.y;
     }
-    total.x += v.x;
-    total.y += v.y;
+  } else {                                             // (32 words one after the other: 4 us with 32 warps at it)
+    longlong2 v = lane < THREADS / 32 ? warp_sums[lane] : make_longlong2(0, 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t m = __shfl_up_sync(0xffffffffu, v.x, o), n = __shfl_up_sync(0xffffffffu, v.y, o);
+      if (lane >= o) {
+        v.x += m;
+        v.y += n;
+      }
+    }
+    total = make_longlong2(__shfl_sync(0xffffffffu, v.x, 31), __shfl_sync(0xffffffffu, v.y, 31));
+    const int64_t m = __shfl_sync(0xffffffffu, v.x, (warp + 31) & 31), n = __shfl_sync(0xffffffffu, v.y, (warp + 31) & 31);
+    if (warp > 0) {
+      before.x += m;
+      before.y += n;
+    }
   }
   __syncthreads();                                     // (the words may be used again)
 }
 
-template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kernel(PlanArgs p) {
+// EACH: neighbouring requests that a thread adds up.
+template <int THREADS, int EACH> __global__ void __launch_bounds__(THREADS) plan_step_kernel(PlanArgs p) {
   extern __shared__ int32_t plan_smem[];
   __shared__ longlong2 warp_sums[THREADS / 32];
   int32_t* cu_s = plan_smem;                           // [B] first token of the request
@@ -78,33 +97,60 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
   if (threadIdx.x == 0) taken = 0;
   __syncthreads();
   int64_t tokens = 0, wanted = 0;
-  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
-    const int b = b0 + threadIdx.x;
-    const bool in = b < p.B;
-    const int64_t ctx = in ? max(p.context[b], 0) : 0, n = in ? max(p.fresh[b], 0) : 0;
-    const int64_t have = (ctx + p.page - 1) >> shift, all = (ctx + n + p.page - 1) >> shift;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS * EACH) {
+    const int b1 = b0 + (int)threadIdx.x * EACH;
+    int ctx[EACH], n[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      ctx[j] = b1 + j < p.B ? max(p.context[b1 + j], 0) : 0;
+      n[j] = b1 + j < p.B ? max(p.fresh[b1 + j], 0) : 0;
+    }
+    // pages that a request takes; -1: more than its row of the table has
+    auto pages_of = [&](int j) {
+      const int64_t have = ((int64_t)ctx[j] + p.page - 1) >> shift, all = ((int64_t)ctx[j] + n[j] + p.page - 1) >> shift;
+      return all <= p.width ? (int)(all - have) : -1;
+    };
+    int64_t my_tokens = 0, my_pages = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      my_tokens += n[j];
+      my_pages += max(pages_of(j), 0);
+    }
     // (where no request is turned down for its tokens, the pages' sum need not wait for the tokens')
-    bool fits = all <= p.width;
-    longlong2 before, sum, sum_again;
-    block_exclusive_sums<THREADS>(n, fits ? all - have : 0, warp_sums, before, sum);
-    const int64_t cu = tokens + before.x;
-    int64_t need = fits ? all - have : 0, off = wanted + before.y, sum_pages = sum.y;
-    if (tokens + sum.x > p.max_tokens) {
-      fits = fits && cu + n <= p.max_tokens;
-      need = fits ? all - have : 0;
-      block_exclusive_sums<THREADS>(need, 0, warp_sums, before, sum_again);
-      off = wanted + before.x;
+    longlong2 before, sum;
+    block_exclusive_sums<THREADS>(my_tokens, my_pages, warp_sums, before, sum);
+    int64_t cu = tokens + before.x, off = wanted + before.y, sum_pages = sum.y;
+    const bool too_many = tokens + sum.x > p.max_tokens;
+    if (too_many) {
+      my_pages = 0;
+      int64_t end = cu;
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        end += n[j];
+        if (end <= p.max_tokens) my_pages += max(pages_of(j), 0);
+      }
+      longlong2 before_again, sum_again;
+      block_exclusive_sums<THREADS>(my_pages, 0, warp_sums, before_again, sum_again);
+      off = wanted + before_again.x;
       sum_pages = sum_again.x;
     }
     tokens += sum.x;
     wanted += sum_pages;
-    fits = fits && (need == 0 || off + need <= count);
-    // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
-    if (fits && need) atomicMax(&taken, (int32_t)(off + need));
-    if (in) {
-      cu_s[b] = (int32_t)min(cu, (int64_t)0x7fffffff);
-      ctx_s[b] = fits ? (int32_t)ctx : ~(int32_t)ctx;
-      off_s[b] = (int32_t)min(off, (int64_t)0x7fffffff);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const int pages = pages_of(j);
+      bool fits = pages >= 0 && cu + n[j] <= p.max_tokens;
+      const int64_t need = fits ? pages : 0;
+      fits = fits && (need == 0 || off + need <= count);
+      // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
+      if (fits && need) atomicMax(&taken, (int32_t)(off + need));
+      if (b1 + j < p.B) {
+        cu_s[b1 + j] = (int32_t)min(cu, (int64_t)0x7fffffff);
+        ctx_s[b1 + j] = fits ? ctx[j] : ~ctx[j];
+        off_s[b1 + j] = (int32_t)min(off, (int64_t)0x7fffffff);
+      }
+      cu += n[j];
+      off += need;
     }
   }
   __syncthreads();
@@ -130,8 +176,16 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     }
   }
   const int lane = threadIdx.x & 31, warps = cl * (THREADS / 32);
-  auto last_at_most = [&](const int32_t* first, int64_t i) {             // the last request whose first token, or page, is at most i
-    int lo = 0, hi = p.B;
+  // The last request, from lo on, whose first token, or page, is at most i: strides that double, then bisection.
+  auto last_at_most = [&](const int32_t* first, int64_t i, int lo) {
+    int hi = p.B;
+    for (int step = 1; lo + step < p.B; step *= 2) {
+      if (first[lo + step] > i) {
+        hi = lo + step;
+        break;
+      }
+      lo += step;
+    }
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (first[mid] <= i) lo = mid;
@@ -139,13 +193,13 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     }
     return lo;
   };
-  // A warp has consecutive tokens, 32 kBatch at a time: a lane looks for its first one's request by bisection and goes on from there,
-  // and kBatch look-ups are under way at once.
+  // A warp has consecutive tokens, 32 kBatch at a time: a lane looks for each one's request from the last one's on, and kBatch look-ups are
+  // under way at once.
   constexpr int kBatch = 4;
   const int64_t all_tokens = min(tokens, (int64_t)p.max_tokens);
-  const int64_t each = ((int64_t)p.max_tokens + warps * 32 * kBatch - 1) / (warps * 32 * kBatch) * (32 * kBatch);
+  const int64_t each = ((int64_t)p.max_tokens + warps * 32 - 1) / (warps * 32) * 32;
   const int64_t begin = (rank * (THREADS / 32) + (threadIdx.x >> 5)) * each, end = min(begin + each, (int64_t)p.max_tokens);
-  int lo = begin + lane < all_tokens ? last_at_most(cu_s, begin + lane) : 0;
+  int lo = 0;
   for (int64_t t0 = begin + lane; t0 < end; t0 += 32 * kBatch) {
     int32_t position[kBatch];
     int id[kBatch];
@@ -155,7 +209,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
       position[i] = 0;
       id[i] = -1;
       if (t < all_tokens) {
-        while (lo + 1 < p.B && cu_s[lo + 1] <= t) ++lo;
+        lo = last_at_most(cu_s, t, lo);
         const int ctx = ctx_s[lo];
         if (ctx >= 0) {
           position[i] = ctx + (int32_t)(t - cu_s[lo]);
@@ -175,7 +229,7 @@ template <int THREADS> __global__ void __launch_bounds__(THREADS) plan_step_kern
     }
   }
   for (int i = rank * THREADS + threadIdx.x; i < taken; i += cl * THREADS) {
-    const int b = last_at_most(off_s, i), have = (int)(((int64_t)ctx_s[b] + p.page - 1) >> shift);
+    const int b = last_at_most(off_s, i, 0), have = (int)(((int64_t)ctx_s[b] + p.page - 1) >> shift);
     p.table[(int64_t)b * p.table_stride + have + i - off_s[b]] = p.free_pages[count - 1 - i];
   }
 }
@@ -244,8 +298,9 @@ int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t*
   LLMQRT_REQUIRE(blocks == 1 || workspace, "plan_step: null workspace");
   PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
              blocks > 1 ? ws_counters(workspace) : nullptr, (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
-  const int smem = (int)(3 * 4 * B), threads = few ? 128 : kPlanThreads;
-  auto kern = few ? plan_step_kernel<128> : plan_step_kernel<kPlanThreads>;
+  const int smem = (int)(3 * 4 * B), threads = few ? 128 : B <= 512 ? 512 : 1024;
+  // (8192 requests of one token: 16 us with eight a thread, 36 in eight rounds)
+  auto kern = few ? plan_step_kernel<128, 1> : B <= 512 ? plan_step_kernel<512, 1> : B <= 1024 ? plan_step_kernel<1024, 1> : plan_step_kernel<1024, 8>;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
   if (int rc = launch_chained(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)smem, (cudaStream_t)stream, 1, p)) return rc;
   return check_launch("plan_step");
