@@ -67,6 +67,16 @@ def test_large(M, N, K):
     _check(ops.fp8_linear_block(*args, torch.bfloat16), *args)
 
 
+@pytest.mark.parametrize("M,N,K", [(33, 37000, 272), (64, 37888, 384), (64, 19072, 1024), (48, 37761, 16), (50, 56000, 144)])
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_wide_layers_of_few_tokens(M, N, K, dt):
+    """More tiles of weight rows than SMs, an odd number of them among these."""
+    from llmqrt_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(M * N + K)
+    args = _inputs(M, N, K, g, DT[dt])
+    _check(ops.fp8_linear_block(*args, DT[dt]), *args)
+
+
 @pytest.mark.parametrize("M", [1, 50, 130, 600])
 @pytest.mark.parametrize("N,pad", [(200, 8), (200, 3), (129, 1)])
 def test_rows_of_wider_matrices(M, N, pad):
