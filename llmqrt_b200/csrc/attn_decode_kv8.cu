@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
 // 10 us a stage for 12 parts: one block has too few loads under way.)
 template <bool BF16, int D, int ROWS>
 __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Args p, int blocks, int each) {
-  constexpr int W = D / 32, kBatch = 8;
+  constexpr int W = D / 32, kBatch = 10;
   __shared__ float sm_o[16][D];
   __shared__ float2 sm_ml[16];
   __shared__ int64_t scan[2][16];
@@ -900,7 +900,7 @@ int launch(Kv8Args a, int B, void* workspace, cudaStream_t st) {
   if (int rc = launch_chained(kern, dim3((unsigned)blocks, (unsigned)columns, 1), dim3(kThreads), smem, st, 1, a)) return rc;
   if (int rc = check_launch("attn_decode_kv8")) return rc;
   if (blocks == 1) return LLMQRT_OK;
-  int each = 1;                                        // warps a row: eight parts each, one batch of loads, where the parts are that many
+  int each = 1;                                        // warps a row: about eight parts each, one batch of loads
   while (each < 16 && each * 8 * B < blocks) each *= 2;
   const int warps = std::max(4, each);
   if (int rc = launch_chained(attn_decode_kv8_merge_kernel<BF16, D, ROWS>, dim3((unsigned)ceil_div(a.Sq * a.Hq, warps / each), (unsigned)B),

@@ -9,19 +9,22 @@ launch:
     WQLinear_GEMM                         packed words / zeros / scales concatenated along N (as the reference)
     SqW8A8BBF16OBF16PerChannel            int8 rows, per-channel scales and bias concatenated (per-token activation scale)
     FP8DynamicLinear(per_tensor=False)    weight rows, per-channel scales and bias concatenated (per-token activation scale)
+    FP8BlockLinear                        weight rows, rows of block scales and bias concatenated, where all layers but the last have
+                                          a multiple of 128 outputs (a row of scales serves 128)
 
 Schemes with ONE weight scale per tensor (SqW8A8BBF16OBF16PerTensor, FP8DynamicLinear(per_tensor=True))
 and static activation scales (FP8StaticLinear) keep the reference's behaviour: q, k, v carry
 different scales, the scalar-alpha kernels cannot express that, and the tuple is returned unchanged.
 
 The concatenation is along output channels, so every output column is computed exactly as the
-unfused layer would: the fused result is bit-identical to torch.cat of the three separate outputs.
+unfused layer would: the fused result is bit-identical to torch.cat of the three separate outputs
+(FP8BlockLinear: but for the order of the fp32 sums, which goes by the layer's width).
 """
 from __future__ import annotations
 
 import torch
 
-from .linear import FP8DynamicLinear, SqW8A8BBF16OBF16PerChannel, WQLinear_GEMM
+from .linear import FP8BlockLinear, FP8DynamicLinear, SqW8A8BBF16OBF16PerChannel, WQLinear_GEMM
 from .linear.linear_base import forward_is
 
 
@@ -37,9 +40,17 @@ def _cat_bias(layers):
 
 def fusable(layer) -> bool:
     """Whether `layer`'s scheme allows projections of the same input to be fused."""
-    if isinstance(layer, (WQLinear_GEMM, SqW8A8BBF16OBF16PerChannel)):
+    if isinstance(layer, (WQLinear_GEMM, SqW8A8BBF16OBF16PerChannel, FP8BlockLinear)):
         return True
     return isinstance(layer, FP8DynamicLinear) and not layer.per_tensor
+
+
+def _fusable_together(layers) -> bool:
+    """Whether these projections of the same input, in this order, make one layer."""
+    first = layers[0]
+    if not fusable(first) or not all(type(l) is type(first) for l in layers):
+        return False
+    return not isinstance(first, FP8BlockLinear) or all(l.out_features % 128 == 0 for l in layers[:-1])
 
 
 def fuse_linears(linears, device=None):
@@ -49,6 +60,8 @@ def fuse_linears(linears, device=None):
     first = linears[0]
     if not all(type(l) is type(first) and l.in_features == first.in_features for l in linears) or not fusable(first):
         raise TypeError("fuse_linears: layers must share one fusable class and in_features")
+    if not _fusable_together(linears):
+        raise ValueError("fuse_linears: layers with block scales must have a multiple of 128 outputs, the last one excepted")
     out_features = sum(l.out_features for l in linears)
     has_bias = any(l.bias is not None for l in linears)
     if isinstance(first, WQLinear_GEMM):
@@ -69,6 +82,18 @@ def fuse_linears(linears, device=None):
         fused.bias = _cat_bias(linears)
         for l in linears:
             del l.qweight, l.weight_scale
+    elif isinstance(first, FP8BlockLinear):
+        dev = device if device is not None else first.weight.device
+        fused = FP8BlockLinear(first.in_features, out_features, has_bias, dev=dev, dtype=first.dtype)
+        at = 0
+        for l in linears:                                # (the layer's own buffers: torch does not concatenate float8 everywhere)
+            fused.weight.data[at:at + l.out_features].copy_(l.weight.data)
+            fused.weight_scale.data[at // 128:at // 128 + l.weight_scale.shape[0]].copy_(l.weight_scale.data)
+            at += l.out_features
+        if has_bias:
+            fused.bias.data.copy_(_cat_bias(linears))
+        for l in linears:
+            del l.weight, l.weight_scale
     else:                                                # FP8DynamicLinear, per token x per channel
         dev = device if device is not None else first.weight.device
         fused = FP8DynamicLinear(first.in_features, out_features, has_bias, dev=dev, dtype=first.dtype,
@@ -87,7 +112,7 @@ def fuse_linears(linears, device=None):
 def fuse_qkv(module, q_proj, k_proj, v_proj):
     """ref fused_utils.py:43-104: returns the fused qkv layer, or the tuple (q_proj, k_proj, v_proj)
     unchanged when the scheme cannot be fused."""
-    if not (fusable(q_proj) and type(k_proj) is type(q_proj) and type(v_proj) is type(q_proj)):
+    if not _fusable_together([q_proj, k_proj, v_proj]):
         return (q_proj, k_proj, v_proj)
     try:
         dev = next(iter(module.state_dict().values())).device
@@ -102,7 +127,7 @@ class FusedGateUpMLP(torch.nn.Module):
 
     def __init__(self, gate_proj, up_proj, down_proj):
         super().__init__()
-        self.gate_up = fuse_linears([gate_proj, up_proj]) if fusable(gate_proj) and type(up_proj) is type(gate_proj) else None
+        self.gate_up = fuse_linears([gate_proj, up_proj]) if _fusable_together([gate_proj, up_proj]) else None
         self.gate_proj, self.up_proj = (None, None) if self.gate_up is not None else (gate_proj, up_proj)
         self.down_proj = down_proj
 

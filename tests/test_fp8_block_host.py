@@ -74,3 +74,31 @@ def test_quantized_blocks():
     full = s.repeat_interleave(128, 0)[:300].repeat_interleave(128, 1)[:, :400]
     err = (q.float() * full - w).abs()
     assert (err <= w.abs() * 2.0 ** -4 * 1.001 + full * 2.0 ** -10 * 1.001).all() and (q.float().abs().amax() == 448)
+
+
+def _layers(outs, k=160, bias=(True, False, True)):
+    from llmqrt_b200.linear import FP8BlockLinear
+    g, layers = torch.Generator().manual_seed(1), []
+    for n, b in zip(outs, bias):
+        m = torch.nn.Linear(k, n, bias=b)
+        m.weight.data.copy_(torch.randn(n, k, generator=g))
+        layers.append(FP8BlockLinear.from_linear(m, init_only=False, dtype=torch.float16))
+    return layers
+
+
+def test_fused_projections():
+    """Rows of codes and of scales one below the other; a layer without a bias counts as one of zeros."""
+    from llmqrt_b200.fused_utils import FusedGateUpMLP, fuse_linears, fuse_qkv
+    layers = _layers((256, 128, 72))
+    w = torch.cat([l.weight.data.float() for l in layers])
+    s = torch.cat([l.weight_scale.data for l in layers])
+    bias = torch.cat([layers[0].bias.data, torch.zeros(128).half(), layers[2].bias.data])
+    fused = fuse_qkv(torch.nn.Module(), *layers)
+    assert fused.out_features == 456 and torch.equal(fused.weight.data.float(), w) and torch.equal(fused.weight_scale.data, s)
+    assert torch.equal(fused.bias.data, bias) and not hasattr(layers[0], "weight")
+    odd = _layers((200, 128, 72))
+    assert fuse_qkv(torch.nn.Module(), *odd) == tuple(odd)               # a row of scales would serve two layers
+    with pytest.raises(ValueError, match="128"):
+        fuse_linears(odd)
+    gate, up, down = _layers((192, 192, 64), bias=(False, False, False))
+    assert FusedGateUpMLP(gate, up, down).gate_up is None

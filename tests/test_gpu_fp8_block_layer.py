@@ -122,3 +122,30 @@ def test_layer(dt):
         lens = [n + m for n, m in zip(lens, now)]
         assert layer.cache.seq_lens.tolist() == lens
         layer.check(x, z, lens)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_fused_projections(dt, T):
+    """Projections of one input as one layer: each output as its own layer gives it, but for the order of the fp32 sums."""
+    from llmqrt_b200.fused_utils import FusedGateUpMLP, fuse_qkv
+    from llmqrt_b200.linear import FP8BlockLinear
+    g = torch.Generator(device="cuda").manual_seed(T)
+
+    def linear(n, k, bias):
+        m = torch.nn.Linear(k, n, bias=bias, device="cuda")
+        m.weight.data.copy_(torch.randn(n, k, generator=g, device="cuda") * k ** -0.5)
+        return FP8BlockLinear.from_linear(m, init_only=False, dtype=dt)
+    x = torch.randn(1, T, 512, generator=g, device="cuda").to(dt)
+    parts = [linear(n, 512, True) for n in (512, 128, 128)]
+    apart = torch.cat([l(x) for l in parts], -1)
+    half = torch.finfo(dt).eps / 2
+    assert rel_fro(fuse_qkv(torch.nn.Module(), *parts)(x), apart) < 2 * (half + 2.0 ** -16)      # (each off by its own rounding)
+    gate, up, down = linear(640, 512, False), linear(640, 512, False), linear(512, 640, False)
+    a, b = gate(x).double(), up(x).double()
+    w = down.weight.float().double() * down.weight_scale.double().repeat_interleave(128, 0).repeat_interleave(128, 1)
+    act = a * torch.sigmoid(a) * b
+    mlp = FusedGateUpMLP(gate, up, down)
+    assert mlp.gate_up is not None
+    # codes of the activations off by 2^-4 at most, and 2^-6 for their own roundings
+    assert ((mlp(x).double() - act @ w.T).abs() <= (act.abs() @ w.abs().T) * (2.0 ** -4 + 2.0 ** -6) + 1e-3).all()
