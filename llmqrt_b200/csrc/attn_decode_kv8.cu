@@ -19,12 +19,12 @@
 // Grid.  Few short sequences: clusters of up to eight blocks, which have a sequence's keys between them and merge their parts through
 // each other's shared memory.  Otherwise (blocks, Hkv * row tiles): as many blocks as fit at once, each with an equal piece of all
 // sequences' keys laid end to end, whatever their lengths; sequences that several blocks have had a part of are merged from
-// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 52.)
+// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 48.)
 // Page numbers outside the cache and rows behind the last key are not read (zeros take their place) and get no weight.
 //
-// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 52 us (4.3 TB/s: beginning a sequence costs a
-// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 34 us
-// (4.0 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 201 us (5.9 TB/s).
+// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 48 us (4.6 TB/s: beginning a sequence costs a
+// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 33 us
+// (4.1 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 198 us (6.0 TB/s).
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -210,7 +210,9 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
   __shared__ float q_scale[ROWS];
   __shared__ int q_sees[ROWS];                         // keys that a row's token sees
   pdl_wait();
-  pdl_trigger();
+  // (The merge kernel begins when this one's blocks have ended: let in earlier, its blocks take the SMs unevenly from those of the next
+  // call, 52 against 48 us for 64 sequences and 59 against 45 for 100 of 64-wide heads.)
+  if (p.cluster > 1) pdl_trigger();
   const int hkv = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles;
   const int rep = p.Hq / p.Hkv, rows = p.Sq * rep;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
