@@ -16,8 +16,9 @@
 //   block_split_kernel  few tokens: weights are the 128-lane operand (128 rows: one row of scales), the tokens the 16 .. 128
 //                       columns, and the reduction is shared out to a cluster, whose CTAs add their sums up through
 //                       distributed shared memory in rank order.
-// Measured: 64 x 37888 x 3584 29 us (its bytes alone 21.5), 1 x 4864 x 896 5.3 us; 4096 x 3584 x 18944 295 us, 1.9 PFLOP/s, 258 with
-// constant data: the board's 1000 W bound it, and every K block's sums on their way through registers.
+// Measured: 64 x 37888 x 3584 29 us (its bytes alone 21.5), 1 x 4864 x 896 5.3 us; 4096 x 3584 x 18944 256 us in a
+// burst and 293 under the board's 1000 W (1.9 PFLOP/s), where gemm_tc.cu's fp8 GEMM takes 239 and 266: every K block's sums pass
+// through registers.
 // All waits are bounded as in gemm_tc.cu.
 #include "gemm_w8a8.cuh"
 #include "tc_tiles.cuh"
