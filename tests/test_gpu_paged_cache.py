@@ -480,10 +480,20 @@ def test_attend_does_not_read_behind_the_last_key():
 
 @pytest.mark.parametrize("lens,Hq,Hkv,Sq,top", [([1, 0, 0, 2, 0], 4, 1, 1, 20000), ([0] * 300 + [1, 64, 65, 5000] + [0] * 9, 2, 1, 1, 9000),
                                                ([3000] + [1] * 130 + [129], 8, 8, 1, 40000), ([200, 70, 0, 64], 256, 256, 1, 9000),
-                                               ([777, 64], 512, 256, 16, 9000), ([6000, 5, 6001], 32, 2, 16, 9000)])
+                                               ([777, 64], 512, 256, 16, 9000), ([6000, 5, 6001], 32, 2, 16, 9000),
+                                               ([300, 64, 0], 1024, 1024, 1, 9000), ([130, 1], 1024, 64, 16, 9000)])
 def test_attend_shares(lens, Hq, Hkv, Sq, top):
     """Fewer keys than blocks, sequences without keys between others, heads that fill the machine by themselves."""
     _check_attend(lens, 16, Hq, Hkv, 64, Sq, "int8", torch.float16, top=top, width=-(-top // 16))
+
+
+@pytest.mark.parametrize("lens,Sq,top", [([700, 64, 2000, 1, 1300] * 13, 1, 9000), ([40000], 2, 40000), ([90, 300], 3, 512)])
+def test_attend_gives_the_same_bits_again(lens, Sq, top):
+    """Clusters' and blocks' parts are added up in one order, whoever is first."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    q, kc, vc, ks, vs, table, out = _check_attend(lens, 32, 14, 2, 128, Sq, "e4m3", torch.bfloat16, rotary=False, top=top, width=-(-top // 32))
+    for _ in range(5):
+        assert bits_equal(attn_decode_kv8(q, kc, vc, ks, vs, table, _i32(lens), top), out)
 
 
 def test_attend_many_sequences():
