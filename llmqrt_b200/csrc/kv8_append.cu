@@ -13,18 +13,20 @@
 // on every run.
 //
 // A block looks for runs in a window of the call's tokens, one window for each head, keys and values.  A decode step's tokens are runs
-// of their own: a warp each, four to a window.  Of many tokens a window has 32, and the block's two warps take each run together.
+// of their own: a warp each, four to a window.  Of many tokens a window has 32, and the block's two warps (four, where pages hold 64 or
+// more) take each run together.
 //
 // Bound by its chain of loads (slots, rows and positions, angles; 18 warps an SM) and 17 instructions an element, at half of what the
 // schedulers could issue: 17600 tokens of 4 heads of 128 take 17 us with their rows in L2 and 21 without, 58 MB at 2.7 TB/s of 6.5.
-// (A warp a run: 33 us; four warps: 18 and 24; eight: 26, as what a run costs before its rows is paid by each of them.)
+// (A warp a run: 33 us; four warps: 18 and 24; eight: 26, as what a run costs before its rows is paid by each of them.
+// Pages of 128, 8 heads: four warps 39 us, two 46; pages of 64, 3000 tokens: 8 and 11.  A block that goes over all heads of a run with the
+// next ones' rows on their way: 19.6 and 22.5.)
 #include "kv8.cuh"
 
 namespace llmqrt {
 namespace {
 
 constexpr int kWarps = 4;                              // a warp a run
-constexpr int kTeam = 2;                               // that share a run
 
 struct AppendArgs {
   uint8_t* cache[2];               // keys, values: [pages, Hkv, page, d]
@@ -216,14 +218,14 @@ extern "C" int llmqrt_kv8_append(void* k_cache, void* v_cache, float* k_scale, f
   a.num_slots = pages * page;
   a.T = (int)T; a.Hkv = (int)Hkv; a.page = (int)page; a.table_rows = (int)table_rows;
   // (64 tokens of a decode step: 2.6 us with a warp each)
-  const bool team = T > 2048;
+  const int team = T <= 2048 ? 0 : page >= 64 ? 4 : 2;
   a.window = team ? 32 : kWarps;
   const dim3 grid((unsigned)ceil_div(T, a.window), (unsigned)Hkv, 2);
-  auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(team ? kTeam * 32 : kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
+  auto go = [&](auto kern) { return launch_chained(kern, grid, dim3(team ? (unsigned)team * 32 : kWarps * 32), 0, (cudaStream_t)stream, 1, a); };
   const bool i8 = cache_type == LLMQRT_I8;
   auto pick = [&](auto tag) {
     using T_ = decltype(tag);
-#define LLMQRT_APPEND(D_, I_) (team ? go(kv8_append_kernel<T_, D_, I_, kTeam>) : go(kv8_append_kernel<T_, D_, I_, 1>))
+#define LLMQRT_APPEND(D_, I_) (team == 4 ? go(kv8_append_kernel<T_, D_, I_, 4>) : team == 2 ? go(kv8_append_kernel<T_, D_, I_, 2>) : go(kv8_append_kernel<T_, D_, I_, 1>))
     return d == 128 ? (i8 ? LLMQRT_APPEND(128, true) : LLMQRT_APPEND(128, false)) : (i8 ? LLMQRT_APPEND(64, true) : LLMQRT_APPEND(64, false));
 #undef LLMQRT_APPEND
   };
