@@ -13,13 +13,13 @@
 // on every run.
 //
 // A block looks for runs in a window of the call's tokens, one window for each head, keys and values.  A decode step's tokens are runs
-// of their own: a warp each, four to a window.  Of many tokens a window has 32, and the block's two warps (four, where pages hold 64 or
+// of their own: a warp each, four to a window (a run that is alone in its window gets all four).  Of many tokens a window has 32, and the block's two warps (four, where pages hold 64 or
 // more) take each run together.
 //
 // Bound by its chain of loads (slots, rows and positions, angles; 18 warps an SM) and 17 instructions an element, at half of what the
 // schedulers could issue: 17600 tokens of 4 heads of 128 take 17 us with their rows in L2 and 21 without, 58 MB at 2.7 TB/s of 6.5.
 // (A warp a run: 33 us; four warps: 18 and 24; eight: 26, as what a run costs before its rows is paid by each of them.
-// Pages of 128, 8 heads: four warps 39 us, two 46; pages of 64, 3000 tokens: 8 and 11.  A block that goes over all heads of a run with the
+// Pages of 128, 8 heads: four warps 39 us, two 46; pages of 64, 3000 tokens: 8 and 11. 1800 tokens of two prompts: 5.3, a warp a run 9.6.  A block that goes over all heads of a run with the
 // next ones' rows on their way: 19.6 and 22.5.)
 #include "kv8.cuh"
 
@@ -42,14 +42,14 @@ struct AppendArgs {
   int T, Hkv, page, table_rows, window;
 };
 
-// TEAM: warps that share a run: 1, or all of the block's.
+// TEAM: warps that share a run, all of the block's; 1: a warp a run, where the window has one alone all four.
 template <typename T, int D, bool INT8, int TEAM>
 __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ? 20 / TEAM : 5) kv8_append_kernel(AppendArgs p) {
-  constexpr int kLanes = D / 16, kRows = 32 / kLanes * TEAM;             // lanes of a row, rows that are taken at once
-  __shared__ float tops[2][TEAM];
+  constexpr int kLanes = D / 16, kBlockWarps = TEAM > 1 ? TEAM : kWarps;      // lanes of a row
+  __shared__ float tops[2][kBlockWarps];
   pdl_wait_then_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y, kind = blockIdx.z;
-  const int piece = lane % kLanes, sub = lane / kLanes + (TEAM > 1 ? warp * (32 / kLanes) : 0);
+  const int piece = lane % kLanes;
   const int w0 = blockIdx.x * p.window, w1 = min(p.T, w0 + p.window);
   const int shift = __ffs(p.page) - 1;
   // the runs that begin in the window: one bit a token (a window has at most 32)
@@ -59,8 +59,10 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
     begins = s >= 0 && s < p.num_slots && !(before + 1 == s && (s & (p.page - 1)) != 0);
   }
   unsigned runs = __ballot_sync(0xffffffffu, begins);
+  const bool together = TEAM > 1 || __popc(runs) == 1;
+  const int sub = lane / kLanes + (together ? warp * (32 / kLanes) : 0), rows = 32 / kLanes * (together ? kBlockWarps : 1);      // taken at once
   for (int nth = 0; runs; runs &= runs - 1, ++nth) {
-    if (TEAM == 1 && nth % kWarps != warp) continue;
+    if (!together && nth % kWarps != warp) continue;
     const int t0 = w0 + __ffs(runs) - 1;
     const int64_t s0 = p.slots[t0];
     const int row0 = (int)(s0 & (p.page - 1));
@@ -105,13 +107,13 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
       turn(lo, hi, at, x);
     };
     // The first rows are asked for before the run's length is known, and kept.
-    constexpr int kKeep = TEAM == 1 ? 1 : 4;
+    constexpr int kKeep = TEAM == 1 ? 2 : 4;
     const int most = min(p.page - row0, p.T - t0);
     const float was = row0 > 0 ? *scale : 0.f;
     uint4 lo[kKeep], hi[kKeep];
     int at[kKeep];
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) load(sub + k * kRows, sub + k * kRows < most, lo[k], hi[k], at[k]);
+    for (int k = 0; k < kKeep; ++k) load(sub + k * rows, sub + k * rows < most, lo[k], hi[k], at[k]);
     // length of the run: to the end of the page, or as far as the slots follow one another
     int n = 1;
     while (n < most) {
@@ -124,25 +126,25 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
     float top = 0.f;
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
-      if (sub + k * kRows >= n) continue;
+      if (sub + k * rows >= n) continue;
       float x[16];
       turn(lo[k], hi[k], at[k], x);
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[j]));
     }
 #pragma unroll 2
-    for (int i = sub + kKeep * kRows; i < n; i += kRows) {
+    for (int i = sub + kKeep * rows; i < n; i += rows) {
       float x[16];
       fetch(i, x);
 #pragma unroll
       for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(x[j]));
     }
     top = warp_max(top);
-    if constexpr (TEAM > 1) {                          // (two sets in turn: one barrier a run is enough, and none reads the old scale behind it)
+    if (together) {                                    // (two sets in turn: one barrier a run is enough, and none reads the old scale behind it)
       if (lane == 0) tops[nth & 1][warp] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < TEAM; ++w) top = fmaxf(top, tops[nth & 1][w]);
+      for (int w = 0; w < kBlockWarps; ++w) top = fmaxf(top, tops[nth & 1][w]);
     }
     const float now = fmaxf(was, kv8_scale<INT8>(top)), inv = __fdiv_rn(1.f, now);
     // lane `piece` of a row holds elements 8 piece .. + 7 and D / 2 further: two 8-byte stores
@@ -154,12 +156,12 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
     };
 #pragma unroll
     for (int k = 0; k < kKeep; ++k)
-      if (sub + k * kRows < n) {                       // (turned once more: as fp32 they would take twice the registers)
+      if (sub + k * rows < n) {                       // (turned once more: as fp32 they would take twice the registers)
         float x[16];
         turn(lo[k], hi[k], at[k], x);
-        store(sub + k * kRows, x);
+        store(sub + k * rows, x);
       }
-    for (int i = sub + kKeep * kRows; i < n; i += kRows) {
+    for (int i = sub + kKeep * rows; i < n; i += rows) {
       float x[16];
       fetch(i, x);
       store(i, x);
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
     if (now != was) {
       if (row0 > 0) {
         const float ratio = __fdiv_rn(was, now);
-        for (int i = sub; i < row0; i += kRows) {
+        for (int i = sub; i < row0; i += rows) {
           uint8_t* at = tile + (int64_t)i * D + piece * 16;
           float x[16];
           kv8_decode<INT8>(*reinterpret_cast<const uint4*>(at), x);
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(TEAM > 1 ? TEAM * 32 : kWarps * 32, TEAM > 1 ?
         }
       }
       __syncwarp();                                    // (every lane has read the old scale)
-      if (TEAM > 1 ? threadIdx.x == 0 : lane == 0) *scale = now;
+      if (together ? threadIdx.x == 0 : lane == 0) *scale = now;
     }
   }
 }
