@@ -16,7 +16,7 @@
 //   block_split_kernel  few tokens: weights are the 128-lane operand (128 rows: one row of scales), the tokens the 16 .. 128
 //                       columns, and the reduction is shared out to a cluster, whose CTAs add their sums up through
 //                       distributed shared memory in rank order.
-// Measured: 64 x 37888 x 3584 29 us (its bytes alone 21.5), 1 x 4864 x 896 5.3 us; 4096 x 3584 x 18944 256 us in a
+// Measured: 64 x 37888 x 3584 27.5 us (its bytes alone 21.5), 1 x 4864 x 896 4.9 us; 4096 x 3584 x 18944 256 us in a
 // burst and 293 under the board's 1000 W (1.9 PFLOP/s), where gemm_tc.cu's fp8 GEMM takes 239 and 266: every K block's sums pass
 // through registers.
 // All waits are bounded as in gemm_tc.cu.
@@ -67,29 +67,30 @@ __device__ __forceinline__ void load_now(const float* p, float& v) { asm volatil
 
 // ---- few tokens --------------------------------------------------------------------------------------
 // TMA warp, MMA warp, and four epilogue warps for each 32 tokens: with four for all of them they bound 128 tokens, 1370 cycles a
-// K block whose weights come in 700 (37888 x 3584: 44.2 us, now 35 to 37; 64 tokens 30.4 and 29.3).  What is left grows with the
-// activations, which each tile of weight rows fetches from L2 again (one token: 25.1 us, 5.4 TB/s).
+// K block whose weights come in 700 (37888 x 3584: 44.2 us, now 35 to 37).  Up to 64 tokens two CTAs share an SM, each with half the
+// ring and tensor memory: one's start and end lie beside the other's tiles (64 tokens 28.8, now 27.5 us; 4608 x 3584, one token: 9.3 and
+// 8.3).  What is left grows with the activations, which each tile of weight rows fetches from L2 again (one token: 24.1 us).
 template <int BN> constexpr int split_groups() { return BN <= 32 ? 1 : BN / 32; }
-template <int BN, int R> constexpr int split_threads() { return 64 + 128 * split_groups<BN>() * R; }
+template <int BN> constexpr int split_threads() { return 64 + 128 * split_groups<BN>(); }
+template <int BN> constexpr int split_per_sm() { return BN <= 64 ? 2 : 1; }
 constexpr int kSplitBufs = 4;                          // accumulators of BN columns
-// R: tiles of 128 weight rows that share an activation tile.
-template <int BN, int R> constexpr int split_stage_bytes() { return (R * kBM + BN) * kRowBytes; }
-template <int BN, int R> constexpr int split_stages() {
-  const int s = 200 * 1024 / split_stage_bytes<BN, R>();  // (some shared memory is left for the small kernels ahead in a chain)
+template <int BN> constexpr int split_stage_bytes() { return (kBM + BN) * kRowBytes; }
+template <int BN> constexpr int split_stages() {
+  const int s = 200 * 1024 / split_per_sm<BN>() / split_stage_bytes<BN>();      // (some shared memory is left for the small kernels ahead in a chain)
   return s > 10 ? 10 : s;
 }
-template <int BN, int R> constexpr int split_smem() { return split_stages<BN, R>() * split_stage_bytes<BN, R>() + 1024; }
-template <int BN, int R> constexpr uint32_t split_tmem_cols() { return kSplitBufs * BN * R; }
+template <int BN> constexpr int split_smem() { return split_stages<BN>() * split_stage_bytes<BN>() + 1024; }
+template <int BN> constexpr uint32_t split_tmem_cols() { return kSplitBufs * BN; }
 
 __device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[32]) { tc::tmem_ld_32x32(taddr, r); }
 __device__ __forceinline__ void ld_chunk(uint32_t taddr, uint32_t (&r)[16]) { tc::tmem_ld_32x16(taddr, r); }
 
-template <int BN, int R>
-__global__ void __launch_bounds__(split_threads<BN, R>(), 1)
+template <int BN>
+__global__ void __launch_bounds__(split_threads<BN>(), split_per_sm<BN>())
 block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, const BlockParams prm) {
-  constexpr int kStages = split_stages<BN, R>(), kStageBytes = split_stage_bytes<BN, R>();
+  constexpr int kStages = split_stages<BN>(), kStageBytes = split_stage_bytes<BN>();
   constexpr int kCols = BN < 32 ? BN : 32;             // columns (tokens) of an epilogue warp
-  constexpr int kGroups = split_groups<BN>(), kEpilogues = 4 * kGroups * R;
+  constexpr int kGroups = split_groups<BN>(), kEpilogues = 4 * kGroups;
   static_assert(kStages * kStageBytes >= BN * kBM * 4, "the ring holds the partial sums");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -120,7 +121,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     tc::tma_prefetch_descriptor(&tm_a);
   }
   if (warp == 1) {
-    tc::tmem_alloc(tc::smem_u32(&tmem_base_slot), split_tmem_cols<BN, R>());
+    tc::tmem_alloc(tc::smem_u32(&tmem_base_slot), split_tmem_cols<BN>());
     tc::tmem_relinquish();
   }
   tc::fence_before_sync();
@@ -138,8 +139,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   const int kb_count = (int)((int64_t)(rank + 1) * prm.k_blocks / S) - kb_begin;
 
   F2 acc[kCols / 2];                                   // epilogue: row quad * 32 + lane of the tile, tokens from c_begin on
-  const int quad = warp & 3, wrow = quad * 32 + lane, c_begin = (warp - 2) / 4 % kGroups * kCols;
-  const int r_tile = (warp - 2) / 4 / kGroups;         // which of the R tiles of weight rows
+  const int quad = warp & 3, wrow = quad * 32 + lane, c_begin = (warp - 2) / 4 * kCols;
   const float* a_scale = prm.a_scale;
 
   if (warp == 0) {
@@ -157,16 +157,14 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
       for (int i = 0; i < pre; ++i) {
         const uint32_t full = tc::smem_u32(&bar_full[i]);
         tc::mbar_arrive_expect_tx(full, kStageBytes);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes + r * kBM * kRowBytes), &tm_w, full, (kb_begin + i) * kRowBytes, (tp0 * R + r) * kBM);
+        tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes), &tm_w, full, (kb_begin + i) * kRowBytes, tp0 * kBM);
       }
       if (prm.early_w) {
         pdl_wait();
         pdl_trigger();
       }
       for (int i = 0; i < pre; ++i)
-        tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes + R * kBM * kRowBytes), &tm_a, tc::smem_u32(&bar_full[i]),
+        tc::tma_load_2d(tc::smem_u32(tiles + i * kStageBytes + kBM * kRowBytes), &tm_a, tc::smem_u32(&bar_full[i]),
                         (kb_begin + i) * kRowBytes, tq0 * BN);
       stage_i = pre == kStages ? 0 : pre;
       if (pre == kStages) phase = 1;
@@ -178,9 +176,8 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
           const uint32_t full = tc::smem_u32(&bar_full[stage_i]);
           const uint32_t sp = tc::smem_u32(tiles + stage_i * kStageBytes);
           tc::mbar_arrive_expect_tx(full, kStageBytes);
-#pragma unroll
-          for (int r = 0; r < R; ++r) tc::tma_load_2d(sp + r * kBM * kRowBytes, &tm_w, full, (kb_begin + it) * kRowBytes, (tp * R + r) * kBM);
-          tc::tma_load_2d(sp + R * kBM * kRowBytes, &tm_a, full, (kb_begin + it) * kRowBytes, tq * BN);
+          tc::tma_load_2d(sp, &tm_w, full, (kb_begin + it) * kRowBytes, tp * kBM);
+          tc::tma_load_2d(sp + kBM * kRowBytes, &tm_a, full, (kb_begin + it) * kRowBytes, tq * BN);
           if (++stage_i == kStages) { stage_i = 0; phase ^= 1u; }
           if ((it & 3) == 3 && *abort) { ok = false; break; }
         }
@@ -198,14 +195,12 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
         tc::mbar_wait_or_flag(tc::smem_u32(&bar_full[stage_i]), phase, abort_u32);
         __syncwarp();
         tc::fence_after_sync();
-        const uint32_t sp = tc::smem_u32(tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(buf * BN * R);
-        const uint64_t dw = tc::smem_desc_k_major_sw128(sp), da = tc::smem_desc_k_major_sw128(sp + R * kBM * kRowBytes);
+        const uint32_t sp = tc::smem_u32(tiles + stage_i * kStageBytes), d = tmem_base + (uint32_t)(buf * BN);
+        const uint64_t dw = tc::smem_desc_k_major_sw128(sp), da = tc::smem_desc_k_major_sw128(sp + kBM * kRowBytes);
         if (tc::elect_one()) {
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < kRowBytes / 32; ++j)
-              tc::mma_ss<tc::MMA_F8>(d + (uint32_t)(r * BN), dw + (uint64_t)(r * (kBM * kRowBytes >> 4) + 2 * j), da + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
+          for (int j = 0; j < kRowBytes / 32; ++j)
+            tc::mma_ss<tc::MMA_F8>(d, dw + (uint64_t)(2 * j), da + (uint64_t)(2 * j), prm.idesc, j > 0 ? 1u : 0u);
           tc::mma_commit(tc::smem_u32(&bar_empty[stage_i]));
           tc::mma_commit(tc::smem_u32(&bar_acc_full[buf]));
         }
@@ -220,11 +215,11 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     uint32_t acc_phase = 0;
     bool ready = false;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
-      const int tp = tile / prm.tiles_q * R + r_tile, tq = tile % prm.tiles_q;
+      const int tp = tile / prm.tiles_q, tq = tile % prm.tiles_q;
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
       // (tokens behind the last one: any valid scale, their columns are not written)
-      const float* ws = prm.w_scale + (int64_t)min(tp, (prm.N - 1) / kBM) * prm.k_blocks + kb_begin;
+      const float* ws = prm.w_scale + (int64_t)tp * prm.k_blocks + kb_begin;
       const float* as = a_scale + (int64_t)min(tq * BN + c_begin + lane, prm.M - 1) * prm.k_blocks + kb_begin;
       float next, w_next;
       load_now(ws, w_next);
@@ -239,7 +234,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
         if (!ready) tc::mbar_wait_or_flag(tc::smem_u32(&bar_acc_full[buf]), acc_phase, abort_u32);
         __syncwarp();
         tc::fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)((buf * R + r_tile) * BN + c_begin), empty = tc::smem_u32(&bar_acc_empty[buf]);
+        const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + c_begin), empty = tc::smem_u32(&bar_acc_empty[buf]);
         if (++buf == kSplitBufs) { buf = 0; acc_phase ^= 1u; }
         uint32_t v[kCols];
         ld_chunk(taddr, v);
@@ -272,7 +267,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
     }
   }
 
-  if (R == 1 && S > 1) {
+  if (S > 1) {
     // The ring is idle once every MMA of this CTA has been seen to finish: each CTA leaves its sums there, [token][row], and
     // takes its share of the tokens from all of them, in rank order.
     const int tp = first_tile / prm.tiles_q, tq = first_tile % prm.tiles_q, tokens = min(BN, prm.M - tq * BN);
@@ -330,7 +325,7 @@ block_split_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_consta
   if (S > 1) cluster_sync_all();                       // nobody leaves while a peer may read its sums
   if (warp == 1) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem_base, split_tmem_cols<BN, R>());
+    tc::tmem_dealloc(tmem_base, split_tmem_cols<BN>());
   }
   if (threadIdx.x == 0 && abort_flag && prm.status) *prm.status = 1u;
 }
@@ -711,7 +706,7 @@ template <int BN> const int* split_clusters() {
   static const int none[kMaxCluster + 1] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return none;
-  std::call_once(once[dev], [dev] { ask_clusters(block_split_kernel<BN, 1>, split_threads<BN, 1>(), split_smem<BN, 1>(), 1, kMaxCluster, known[dev]); });
+  std::call_once(once[dev], [dev] { ask_clusters(block_split_kernel<BN>, split_threads<BN>(), split_smem<BN>(), 1, kMaxCluster, known[dev]); });
   return known[dev];
 }
 template <int BN> int pair_clusters() {
@@ -723,17 +718,24 @@ template <int BN> int pair_clusters() {
   return known[dev][2];
 }
 
-// The cluster that shares a reduction: waves of co-resident clusters x (K blocks of a CTA + what a CTA costs beside them).
-int pick_splits(int64_t tiles, int k_blocks, const int* active, int* waves) {
-  const double fixed = 8., sms = sm_count();
+// The cluster that shares a reduction: rounds of co-resident clusters x (K blocks of a CTA + what a CTA costs beside them).  `active`:
+// clusters at once with one CTA an SM (all that the runtime answers for kernels with tensor memory).  Where `shared`, twice as many do,
+// at the price of the bandwidth they share and of their start: fitted to 15 layers, one to 64 tokens.  3584 x 18944, one token: eight CTAs
+// a tile 14.8 us, four (one an SM) 17.0; 17920 x 1536: two 9.3, one 8.4; with 64 tokens a second CTA gains nothing.
+int pick_splits(int64_t tiles, int k_blocks, const int* active, bool shared, int* waves) {
+  const double fixed = 8., fixed_shared = 12., sms = sm_count();
   int splits = 1;
   *waves = (int)ceil_div(tiles, (int64_t)sms);
   double best = *waves * (k_blocks + fixed);
-  for (int s = 2; s <= kMaxCluster && k_blocks >= 2 * s && tiles < sms; ++s) {
+  for (int s = 2; s <= kMaxCluster && k_blocks >= s && tiles < sms; ++s) {
     if (active[s] <= 0) continue;
-    const int w = (int)ceil_div(tiles, (int64_t)active[s]);
-    const double t = w * ((double)k_blocks / s + fixed);
-    if (t < best) { best = t; splits = s; *waves = w; }
+    int w = (int)ceil_div(tiles, (int64_t)active[s]);
+    double t = w * ((double)k_blocks / s + fixed);
+    if (shared && w == 2) {
+      const double both = k_blocks * std::max(1. / s, tiles / sms) + fixed_shared;
+      if (both < t) { t = both; w = 1; }
+    }
+    if (t <= best) { best = t; splits = s; *waves = w; }
   }
   return splits;
 }
@@ -767,23 +769,23 @@ struct Operands {
   int64_t lda, ldw, K;
 };
 
-template <int BN, int R = 1>
+template <int BN>
 int launch_split(const Operands& o, BlockParams prm, cudaStream_t st) {
-  prm.tiles_p = (int)ceil_div(prm.N, R * kBM);
+  prm.tiles_p = (int)ceil_div(prm.N, kBM);
   prm.tiles_q = (int)ceil_div(prm.M, BN);
   prm.idesc = tc::instr_desc(1, 0, 0, kBM, BN);
   const int64_t tiles = (int64_t)prm.tiles_p * prm.tiles_q;
   LLMQRT_REQUIRE(tiles <= 0x7fffffffll / kMaxCluster, "fp8 block linear: too many tiles");
   int waves;
-  prm.splits = R > 1 ? 1 : pick_splits(tiles, prm.k_blocks, split_clusters<BN>(), &waves);
+  prm.splits = pick_splits(tiles, prm.k_blocks, split_clusters<BN>(), BN <= 32, &waves);
   CUtensorMap tm_w, tm_a;
   if (int rc = make_operand_map(&tm_w, o.w, 1, prm.N, o.K, o.ldw, kBM)) return rc;
   if (int rc = make_operand_map(&tm_a, o.a, 1, prm.M, o.K, o.lda, BN)) return rc;
-  auto kern = block_split_kernel<BN, R>;
-  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), split_smem<BN, R>())) return rc;
-  const int64_t grid = prm.splits > 1 ? tiles * prm.splits : std::min(tiles, (int64_t)sm_count());
+  auto kern = block_split_kernel<BN>;
+  if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), split_smem<BN>())) return rc;
+  const int64_t grid = prm.splits > 1 ? tiles * prm.splits : std::min(tiles, (int64_t)sm_count() * split_per_sm<BN>());
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = config(kern, (int)grid, prm.splits, split_threads<BN, R>(), split_smem<BN, R>(), st, attr);
+  cudaLaunchConfig_t cfg = config(kern, (int)grid, prm.splits, split_threads<BN>(), split_smem<BN>(), st, attr);
   LLMQRT_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, tm_w, tm_a, prm));
   return check_launch("fp8 block linear");
 }
@@ -848,13 +850,7 @@ extern "C" int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint
   cudaStream_t st = (cudaStream_t)stream;
   if (M <= 16) return launch_split<16>(o, p, st);
   if (M <= 32) return launch_split<32>(o, p, st);
-  if (M <= 64) {
-    // Two tiles of weight rows to one of tokens halve what comes from L2 beside the weights, where that leaves the SMs' rounds as they
-    // are: 37888 x 3584 30.7 us among other calls, with one tile 32.3.
-    const int64_t tiles = ceil_div(N, kBM), sms = sm_count();
-    if (tiles > sms && 2 * ceil_div(ceil_div(tiles, 2), sms) <= ceil_div(tiles, sms)) return launch_split<64, 2>(o, p, st);
-    return launch_split<64>(o, p, st);
-  }
+  if (M <= 64) return launch_split<64>(o, p, st);
   if (M <= 128) return launch_split<128>(o, p, st);
   const Deal wide = deal_out<256>(M, N, p.k_blocks, workspace != nullptr), narrow = deal_out<128>(M, N, p.k_blocks, workspace != nullptr);
   const double pair = std::min(wide.us, narrow.us);
@@ -862,7 +858,7 @@ extern "C" int llmqrt_fp8_linear_block(const uint8_t* a, int64_t lda, const uint
   // mostly behind the tokens comes slowly).  130 x 300 x 3584 7.7 us, in pairs 12.1; 512 x 1536 x 3584 15.8 and 11.6.
   if (M <= 512 && (M - 1) % 64 >= 15) {
     int waves;
-    const int s = pick_splits(ceil_div(N, kBM) * ceil_div(M, 64), p.k_blocks, split_clusters<64>(), &waves);
+    const int s = pick_splits(ceil_div(N, kBM) * ceil_div(M, 64), p.k_blocks, split_clusters<64>(), false, &waves);
     if (s > 1 && 6. + waves * (0.45 * p.k_blocks / s + 2.5) < pair) return launch_split<64>(o, p, st);
   }
   return wide.us < narrow.us ? launch_pair<256>(o, p, wide, st) : launch_pair<128>(o, p, narrow, st);
