@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -156,6 +157,10 @@ Tensor rows(const Tensor& x) {
 }
 Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType dt) {
   return at::empty(shape, like.options().dtype(dt).requires_grad(false));
+}
+// The same straight from the allocator, 0.3 us less than by the dispatcher: for calls of several results and a few microseconds.
+Tensor result_of(const Tensor& like, at::IntArrayRef shape, at::ScalarType dt) {
+  return at::detail::empty_cuda(shape, dt, like.device(), std::nullopt);
 }
 c10::SmallVector<int64_t, 6> out_shape(const Tensor& x, int64_t n) {
   c10::SmallVector<int64_t, 6> s(x.sizes().begin(), x.sizes().end());
@@ -357,7 +362,7 @@ FAST_FN(fp8_linear_block) {
   Call c(same_device({&x, &w, &bias, &as, &ws}));
   const Tensor x2 = aligned_rows(x), w2 = aligned_rows(w);
   const int64_t N = w.size(0);
-  Tensor out = empty(x, {M, N}, od);
+  Tensor out = result_of(x, {M, N}, od);
   check(llmqrt_fp8_linear_block(static_cast<const uint8_t*>(ptr(x2)), row_stride(x2), static_cast<const uint8_t*>(ptr(w2)), row_stride(w2), ptr(bias), bd,
                                 static_cast<const float*>(ptr(as)), static_cast<const float*>(ptr(ws)), mptr(out), dt, N, M, N, K, c.workspace(),
                                 c.stream, w2.data_ptr() == w.data_ptr() ? flags : 0));
@@ -520,7 +525,7 @@ FAST_FN(quantize_fp8_block) {
   Call c(same_device({&x}));
   const Tensor x2 = aligned_rows(x);
   const int64_t M = x2.size(0), K = x2.size(1);
-  Tensor q = empty(x, {M, K}, at::kFloat8_e4m3fn), s = empty(x, {M, (K + kBlock - 1) / kBlock}, at::kFloat);
+  Tensor q = result_of(x, {M, K}, at::kFloat8_e4m3fn), s = result_of(x, {M, (K + kBlock - 1) / kBlock}, at::kFloat);
   check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, row_stride(x2), static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), c.stream));
   gil.done();
   return wrap_tuple(q, s);
@@ -545,8 +550,8 @@ FAST_FN(rmsnorm_fp8_block) {
   Tensor w = w0.contiguous();
   if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) w = w.clone();
   const int64_t M = x2.size(0);
-  Tensor q = empty(x, {M, H}, at::kFloat8_e4m3fn), s = empty(x, {M, (H + kBlock - 1) / kBlock}, at::kFloat), h;
-  if (res.defined()) h = empty(x, x.sizes(), x.scalar_type());
+  Tensor q = result_of(x, {M, H}, at::kFloat8_e4m3fn), s = result_of(x, {M, (H + kBlock - 1) / kBlock}, at::kFloat), h;
+  if (res.defined()) h = result_of(x, x.sizes(), x.scalar_type());
   check(llmqrt_rmsnorm_fp8_block(ptr(x2), row_stride(x2), ptr(r2), r2.defined() ? row_stride(r2) : 0, mptr(h), ptr(w), eps,
                                  static_cast<uint8_t*>(mptr(q)), static_cast<float*>(mptr(s)), xd, M, H, c.stream));
   gil.done();
@@ -1141,9 +1146,9 @@ FAST_FN(plan_step) {
   if (seq.defined()) int32_vector(seq, B, "seq_lens", "plan_step");
   TORCH_CHECK(max_tokens >= 0, "plan_step: bad max_tokens");
   Call c(same_device({&ctx, &fresh, &table, &pages, &count, &left, &seq}));
-  if (!seq.defined()) seq = empty(ctx, {B}, at::kInt);
-  Tensor cu = empty(ctx, {B + 1}, at::kInt), slots = empty(ctx, {max_tokens}, at::kLong);
-  Tensor positions = empty(ctx, {max_tokens}, at::kInt);
+  if (!seq.defined()) seq = result_of(ctx, {B}, at::kInt);
+  Tensor cu = result_of(ctx, {B + 1}, at::kInt), slots = result_of(ctx, {max_tokens}, at::kLong);
+  Tensor positions = result_of(ctx, {max_tokens}, at::kInt);
   auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(mptr(t)); };
   check(llmqrt_plan_step(i32(ctx), i32(fresh), i32(table), table_stride(table), i32(pages), i32(count), i32(left), i32(seq), i32(cu),
                          static_cast<int64_t*>(mptr(slots)), i32(positions), B, table.size(1), pages.size(0), page, max_tokens, c.workspace(),
@@ -1234,7 +1239,7 @@ FAST_FN(attn_decode_kv8) {
                       (q.stride(3) == 1 && q.stride(2) == d && (Sq == 1 || (q.stride(1) >= Hq * d && q.stride(1) % 8 == 0)) &&
                        (B == 1 || (q.stride(0) >= 0 && q.stride(0) % 8 == 0)) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0);
   if (!usable) q = q.clone(at::MemoryFormat::Contiguous);
-  Tensor out = empty(q, q0.sizes(), q.scalar_type());
+  Tensor out = result_of(q, q0.sizes(), q.scalar_type());
   const int64_t token = Sq > 1 ? q.stride(1) : Hq * d;
   check(llmqrt_attn_decode_kv8(ptr(q), B > 1 ? q.stride(0) : Sq * token, token, ptr(kc), ptr(vc), type, kc.stride(0), kc.stride(1),
                                static_cast<const float*>(ptr(ks)), static_cast<const float*>(ptr(vs)), static_cast<const int32_t*>(ptr(table)),
