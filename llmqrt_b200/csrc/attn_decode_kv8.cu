@@ -9,8 +9,7 @@
 // with warp-level MMAs: keys (or columns of V) are the sixteen rows, the query heads that share the KV head the eight columns.
 //   S^T = K Q^T     : a lane's K fragment is 16 contiguous bytes of two keys' rows; Q is loaded with the same permutation of d.
 //   O^T += V^T P^T  : the fragment wants two keys a register: bytes of two rows are interleaved before they are converted.
-// (With the query rows as the sixteen, half of them idle, it took twice the MMAs and accumulators, three blocks an SM, and 64 us where
-// this takes 58.)
+// (With the query rows as the sixteen, half of them idle, it took twice the MMAs and accumulators, and 64 us where this took 58.)
 // Scales stay out of the products: k_scale multiplies S; v_scale, over the greatest one of the pages so far (a second running
 // reference beside the softmax's maximum), multiplies P.  Q in fp16 is exact for fp16 and, its row multiplied by a power of two, for
 // bf16.  For an fp16 result what the rounding of Q (rotated here) and of P to fp16 left over takes MMAs of its own, so that the
@@ -19,12 +18,12 @@
 // Grid.  Few short sequences: clusters of up to eight blocks, which have a sequence's keys between them and merge their parts through
 // each other's shared memory.  Otherwise (blocks, Hkv * row tiles): as many blocks as fit at once, each with an equal piece of all
 // sequences' keys laid end to end, whatever their lengths; sequences that several blocks have had a part of are merged from
-// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 48.)
+// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 47.)
 // Page numbers outside the cache and rows behind the last key are not read (zeros take their place) and get no weight.
 //
-// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 48 us (4.6 TB/s: beginning a sequence costs a
-// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 33 us
-// (4.1 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 198 us (6.0 TB/s).
+// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 47 us (4.7 TB/s: beginning a sequence costs a
+// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 32 us
+// (4.2 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 196 us (6.0 TB/s).
 #include <algorithm>
 #include <map>
 #include <mutex>
@@ -36,7 +35,10 @@ namespace llmqrt {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 16 * kWarps;
-template <int D> constexpr int kv8_ring() { return D == 128 ? 3 : 5; }  // stages of a warp, 16 keys each
+// Blocks an SM, and stages of a warp, 16 keys each.  (64 sequences, 8 query heads of 128: four blocks 48.4 us and spills, three 47.4, two
+// with a longer ring 46.7 but 50 in fp16; one long sequence, 16 rows: three 33.2, two 32.)
+template <int D, int ROWS> constexpr int kv8_per_sm() { return ROWS == 8 ? (D == 128 ? 3 : 4) : D == 128 ? 2 : 3; }
+template <int D, int ROWS> constexpr int kv8_ring() { return D == 128 && ROWS == 8 ? 3 : 4; }
 constexpr int kSpan = 4096;                            // keys whose page numbers and scales a block holds at a time
 constexpr int kSwitch = 6;                             // what another sequence costs a block, in units of kStep keys (4: 54, 6 to 10: 51.6, 16: 52.5 us)
 constexpr int kMaxBlocks = 1024;                       // that one KV head's keys are shared out to
@@ -196,7 +198,7 @@ template <int D> __device__ __forceinline__ uint32_t v_offset(int row, int chunk
 
 // ROWS: rows of queries that a block's tile holds, 8 or 16.
 template <int D, bool INT8, bool BF16, int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 2 : 3) attn_decode_kv8_kernel(const Kv8Args p) {
+__global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_kv8_kernel(const Kv8Args p) {
   constexpr int NJ = D / 64;                           // 16-byte pieces of a key's row a lane takes
   constexpr int NE = D / 8;                            // columns of the output a lane's V pieces hold
   constexpr int TILE = 16 * D, STAGE = 2 * TILE;
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : !BF16 && D == 128 ? 
 
   // ---- the ring's first stages ----
   // A lane's pieces of a tile are 512 bytes apart in both memories; their swizzle is one of two.
-  constexpr int kRing = kv8_ring<D>();
+  constexpr int kRing = kv8_ring<D, ROWS>();
   constexpr int CPR = D / 16, kPieces = CPR / 2;       // 16-byte pieces of a row, and of a lane
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)(warp * kRing * STAGE);
   const uint32_t k_dst = k_offset<D>(lane / CPR, lane % CPR);
@@ -838,7 +840,7 @@ __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Arg
   else *reinterpret_cast<uint32_t*>(dst) = round_pair<BF16>(o[0] * inv, o[1] * inv);
 }
 
-template <int D> constexpr int kv8_smem() { return kWarps * kv8_ring<D>() * 2 * 16 * D; }
+template <int D, int ROWS> constexpr int kv8_smem() { return kWarps * kv8_ring<D, ROWS>() * 2 * 16 * D; }
 
 // Clusters of `cluster` blocks of a kernel that can be resident at once (asked once per device and kernel).
 int max_active_clusters(const void* kern, int cluster, int smem) {
@@ -872,7 +874,7 @@ int max_active_clusters(const void* kern, int cluster, int smem) {
 
 template <int D, bool INT8, bool BF16, int ROWS>
 int launch(Kv8Args a, int B, void* workspace, cudaStream_t st) {
-  constexpr int smem = kv8_smem<D>();
+  constexpr int smem = kv8_smem<D, ROWS>();
   static_assert(smem >= (kWarps * ROWS * (D + 4 + 2) + ROWS * (D + 2)) * 4, "the rings hold the merge tile");
   auto kern = attn_decode_kv8_kernel<D, INT8, BF16, ROWS>;
   a.tiles = (int)ceil_div((int64_t)a.Sq * (a.Hq / a.Hkv), ROWS);
