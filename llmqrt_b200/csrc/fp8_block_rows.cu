@@ -55,34 +55,40 @@ template <typename T> __device__ __forceinline__ uint32_t add_pairs(uint32_t a, 
   return *reinterpret_cast<const uint32_t*>(&s);
 }
 
-// Unit-slot i of the matrix: row i / (16 groups), unit i % (16 groups); slots behind a row's last unit are empty.
+// Blocks (threads of a row's piece, rows), grid (rows, pieces); unit k of a thread is threadIdx.x + k * blockDim.x of its piece.  A lane divides for the group of one
+// of its units, and passes the factor on.
 template <typename T, int U>
 __global__ void __launch_bounds__(256)
-quantize_fp8_block_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale, int64_t M,
-                          int K, int groups) {
+quantize_fp8_block_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale, int64_t M, int K,
+                          int groups) {
   pdl_wait_then_trigger();
-  const int per_row = groups * kGroupUnits;
-  const int64_t slots = M * per_row, first = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  const int units = K / 8, lane = threadIdx.x & 31, u0 = blockIdx.y * (blockDim.x * U) + threadIdx.x;
+  const int64_t m = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (m >= M) return;                                  // (the whole warp)
   uint4 v[U];
-  int64_t row[U];
-  int unit[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const int64_t i = first + k * 256;
-    row[k] = i / per_row;
-    unit[k] = (int)(i - row[k] * per_row);
-    v[k] = make_uint4(0, 0, 0, 0);
-    if (i < slots && unit[k] * 8 < K) v[k] = ldg_cg_16B(x + row[k] * ldx + unit[k] * 8);
+    const int u = u0 + k * blockDim.x;
+    v[k] = u < units ? ldg_cg_16B(x + m * ldx + u * 8) : make_uint4(0, 0, 0, 0);
   }
+  const int mine = lane & (U - 1);
+  float top = 0.f;
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const float top = fmaxf(half_warp_max(absmax8<T>(v[k], 0.f)), kFloor);
-    if (first + k * 256 >= slots) continue;            // (a whole group at a time)
+    const float top_k = half_warp_max(absmax8<T>(v[k], 0.f));
+    if (k == mine) top = top_k;
+  }
+  top = fmaxf(top, kFloor);
+  const float c_mine = __fdiv_rn(kE4m3Max, top);
+  const int in_group = lane & (kGroupUnits - 1), u_mine = u0 - in_group + in_group * (int)blockDim.x;
+  if (in_group < U && u_mine < units) scale[m * groups + u_mine / kGroupUnits] = __fdiv_rn(top, kE4m3Max);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int u = u0 + k * blockDim.x;
+    const float c = __shfl_sync(0xffffffffu, c_mine, lane - mine + k);
     float t[8];
     unpack8<T>(v[k], t);
-    if (unit[k] * 8 < K)
-      *reinterpret_cast<uint2*>(q + row[k] * K + unit[k] * 8) = to_e4m3x8(t, __fdiv_rn(kE4m3Max, top));
-    if (unit[k] % kGroupUnits == 0) scale[row[k] * groups + unit[k] / kGroupUnits] = __fdiv_rn(top, kE4m3Max);
+    if (u < units) *reinterpret_cast<uint2*>(q + m * K + u * 8) = to_e4m3x8(t, c);
   }
 }
 
@@ -188,15 +194,14 @@ int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, 
   if (int rc = check_rows("quantize_fp8_block", x, ldx, q, scale, x_dtype, M, K)) return rc;
   if (M == 0) return LLMQRT_OK;
   const int groups = (int)ceil_div(K, kGroup);
-  const int64_t slots = M * groups * kGroupUnits;
   // Four units a thread once that still leaves every SM its 2048 threads.
-  const int U = slots >= (int64_t)sm_count() * 2048 * 4 ? 4 : 1;
-  const int64_t blocks = ceil_div(slots, 256 * U);
-  LLMQRT_REQUIRE(blocks <= 0x7fffffffll, "quantize_fp8_block: too many rows");
+  const int units = (int)(K / 8), U = M * units >= (int64_t)sm_count() * 2048 * 4 ? 4 : 1;
+  const int64_t pieces = ceil_div(units, 256 * U);
+  const unsigned threads = (unsigned)ceil_div(ceil_div(units, pieces * U), 32) * 32, rows = 256 / threads;
   auto go = [&](auto kern, auto tag) {
     using T = decltype(tag);
-    return launch_chained(kern, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, 1, static_cast<const T*>(x), ldx, q,
-                          scale, M, (int)K, groups);
+    return launch_chained(kern, dim3((unsigned)ceil_div(M, (int64_t)rows), (unsigned)pieces), dim3(threads, rows), 0, (cudaStream_t)stream, 1,
+                          static_cast<const T*>(x), ldx, q, scale, M, (int)K, groups);
   };
   const int rc = x_dtype == LLMQRT_F16 ? (U == 4 ? go(quantize_fp8_block_kernel<__half, 4>, __half()) : go(quantize_fp8_block_kernel<__half, 1>, __half()))
                  : U == 4 ? go(quantize_fp8_block_kernel<__nv_bfloat16, 4>, __nv_bfloat16())
