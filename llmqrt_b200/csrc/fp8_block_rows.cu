@@ -12,8 +12,10 @@
 // (glue.cu's norm rounds to T twice on the way, as the reference's does; its int8 scale is one per row.)
 //
 // HBM-bound where rows are many, once a lane works out the factor of one of its units only and passes it on (the divisions, of all
-// of them in every lane, held the schedulers at 3/4 of their rate: 37.7 us): 8191 rows of 3584 with a residual take 33 us back to back
-// and 36 among others, 6.2 and 5.7 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us of the GPU, the call 7 with its three allocations.
+// of them in every lane, held the norm's schedulers at 3/4 of their rate: 37.7 us): 8191 rows of 3584 with a residual take 33 us back
+// to back and 36 among others, 6.2 and 5.7 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us of the GPU, the call 6.4 with its three
+// allocations.  The quantizer: 4096 rows of 18944 40 us, 8192 of 3584 15.3, 5.8 TB/s (52.7 and 22 with blocks that went over the units
+// of all rows, whose places took the registers of the loads).
 #include <type_traits>
 
 #include "common.cuh"
@@ -197,7 +199,7 @@ int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, 
   // Four units a thread once that still leaves every SM its 2048 threads.
   const int units = (int)(K / 8), U = M * units >= (int64_t)sm_count() * 2048 * 4 ? 4 : 1;
   const int64_t pieces = ceil_div(units, 256 * U);
-  const unsigned threads = (unsigned)ceil_div(ceil_div(units, pieces * U), 32) * 32, rows = 256 / threads;
+  const unsigned threads = (unsigned)ceil_div(ceil_div(units, pieces * U), 32) * 32, rows = U == 1 ? 256 / threads : 1;
   auto go = [&](auto kern, auto tag) {
     using T = decltype(tag);
     return launch_chained(kern, dim3((unsigned)ceil_div(M, (int64_t)rows), (unsigned)pieces), dim3(threads, rows), 0, (cudaStream_t)stream, 1,
