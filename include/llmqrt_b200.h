@@ -317,7 +317,8 @@ int llmqrt_attn_decode_step(const void* q, int64_t q_batch_stride, const void* k
  *   block_table [B, width] the new pages, behind those in use;   free_left[1] the pages left (may be free_count);
  *   seq_lens [B]           context + new tokens, or context (may be context);   cu_new [B + 1] running sum of the new tokens;
  *   slots, positions [max_tokens]  of new token t of all requests, back to back: -1 and 0 behind the last one and for those of
- *                          a request that gets nothing. */
+ *                          a request that gets nothing.
+ * The workspace may be null where a single block does (max_tokens up to 1024, at most 256 requests). */
 int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t* block_table, int64_t table_stride,
                      const int32_t* free_pages, const int32_t* free_count, int32_t* free_left, int32_t* seq_lens, int32_t* cu_new,
                      int64_t* slots, int32_t* positions, int64_t B, int64_t width, int64_t pool, int64_t page, int64_t max_tokens,

@@ -297,7 +297,7 @@ int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t*
   const int blocks = few ? 1 : (int)std::min<int64_t>(128, std::max<int64_t>(1, ceil_div(std::max(max_tokens, 4 * B), 1024)));
   LLMQRT_REQUIRE(blocks == 1 || workspace, "plan_step: null workspace");
   PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
-             blocks > 1 ? ws_counters(workspace) : nullptr, (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
+             blocks > 1 ? ws_counters(workspace) + LLMQRT_WS_NUM_COUNTERS - 1 : nullptr, (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
   const int smem = (int)(3 * 4 * B), threads = few ? 128 : B <= 512 ? 512 : 1024;
   // (8192 requests of one token: 16 us with eight a thread, 36 in eight rounds)
   auto kern = few ? plan_step_kernel<128, 1> : B <= 512 ? plan_step_kernel<512, 1> : B <= 1024 ? plan_step_kernel<1024, 1> : plan_step_kernel<1024, 8>;
