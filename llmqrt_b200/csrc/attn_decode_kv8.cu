@@ -11,7 +11,9 @@
 //   O^T += V^T P^T  : the fragment wants two keys a register: bytes of two rows are interleaved before they are converted.
 // (With the query rows as the sixteen, half of them idle, it took twice the MMAs and accumulators, and 64 us where this took 58.)
 // Scales stay out of the products: k_scale multiplies S; v_scale, over the greatest one of the pages so far (a second running
-// reference beside the softmax's maximum), multiplies P.  Q in fp16 is exact for fp16 and, its row multiplied by a power of two, for
+// reference beside the softmax's maximum), multiplies P.  A page whose scale is far from the reference (2^8 below it, or above 2^50,
+// where the reference ends) has products of its own, which are scaled in fp32 as they join O, so that no scale, an infinity included, takes
+// bits from the other pages or touches rows that do not see the page.  Q in fp16 is exact for fp16 and, its row multiplied by a power of two, for
 // bf16.  For an fp16 result what the rounding of Q (rotated here) and of P to fp16 left over takes MMAs of its own, so that the
 // result is off by its own rounding alone; bf16's own rounding is eight times as large.
 //
@@ -45,6 +47,7 @@ constexpr int kMaxBlocks = 1024;                       // that one KV head's key
 constexpr int kMaxPages = kSpan / 16 + 1;              // pages that these touch
 constexpr int kClusterMergeMaxLen = 8192;              // greatest bound on the lengths for which a sequence gets one cluster
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHead = 0x1p24f;                       // parts of O are kept so much smaller: sums of values near fp32's end do not pass it
 
 struct Kv8Args {
   const uint16_t* q;               // [B, Sq, Hq, D]
@@ -408,8 +411,9 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
       for (int c = 0; c < 4; ++c) o[e][h][c] = 0.f;
   // The reference that a row's scores are taken against moves only when one exceeds it by more than 2^kSlack: P is then at most
   // that, fp16 rounds it all the same, and most steps need no maximum over the lanes and leave O and the sums alone.
-  // (kLift takes P to the upper end of fp16's range, 2^15: a page whose scale is 2^-20 of the greatest one keeps some bits.)
-  constexpr float kSlack = 6.f, kLift = 512.f, kNothing = -1e30f;
+  // (kLift takes P to the upper end of fp16's range, 2^15: with a share of 2^-8 all of its bits last down to 2^-15 of the greatest P.  The
+  // reference stays within 2^-50 .. 2^50: fp32 holds O at either end, whatever scales the append makes, 2^-49 .. 2^120.)
+  constexpr float kSlack = 6.f, kLift = 512.f, kNothing = -1e30f, kNear = 0x1p-8f, kRefLeast = 0x1p-50f, kRefMost = 0x1p50f;
   float m_run[G][2], l_run[G][2], v_ref = 0.f, v_inv = 0.f;
   int sees_all = 0x7fffffff;                           // keys that every row of the tile sees
 #pragma unroll
@@ -490,12 +494,17 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
       for (int h = 0; h < G; ++h)
 #pragma unroll
         for (int c = 0; c < 2; ++c) beyond |= fmaxf(pv[h][0][c], pv[h][1][c]) > m_run[h][c] + kSlack;
-      if (__any_sync(0xffffffffu, beyond) || vs > v_ref) {
-        const float ref_corr = vs > v_ref ? v_ref / vs : 1.f;
-        if (vs > v_ref) {
-          v_ref = vs;
-          v_inv = kLift / vs;
+      float v_share = vs * v_inv;
+      bool far = false;
+      const bool fits = fabsf(v_share) >= kLift * kNear && fabsf(v_share) <= kLift * 1.001f;      // (one ulp above it is the reference itself; NaN: no)
+      if (__any_sync(0xffffffffu, beyond) || !fits) {
+        const float ref = fminf(fmaxf(fabsf(vs), kRefLeast), kRefMost), ref_corr = ref > v_ref ? v_ref / ref : 1.f;
+        if (ref > v_ref) {
+          v_ref = ref;
+          v_inv = kLift / ref;
         }
+        far = good && !(fabsf(vs) >= kNear * v_ref && fabsf(vs) <= v_ref);
+        v_share = far ? kLift : vs * v_inv;
 #pragma unroll
         for (int h = 0; h < G; ++h)
 #pragma unroll
@@ -515,7 +524,6 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
             }
           }
       }
-      const float v_share = vs * v_inv;
 #pragma unroll
       for (int h = 0; h < G; ++h)
 #pragma unroll
@@ -534,17 +542,58 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
             if (key0 + 8 * (i >> 1) + g >= sees[h][i & 1]) pv[h][i >> 1][i & 1] = 0.f;
       }
       uint32_t pa[G][2], pr[G][2];                       // of row g: keys 2t, 2t + 1 and 2t + 8, 2t + 9
+      auto pack_p = [&]() {
 #pragma unroll
-      for (int h = 0; h < G; ++h)
+        for (int h = 0; h < G; ++h)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const uint32_t whole_p = pack_half(pv[h][kb][0], pv[h][kb][1]);
-          pa[h][kb] = transpose_8x8(whole_p);
-          if constexpr (REST) {
-            const float2 f = unpack_half(whole_p);
-            pr[h][kb] = transpose_8x8(pack_half(pv[h][kb][0] - f.x, pv[h][kb][1] - f.y));
+          for (int kb = 0; kb < 2; ++kb) {
+            const uint32_t whole_p = pack_half(pv[h][kb][0], pv[h][kb][1]);
+            pa[h][kb] = transpose_8x8(whole_p);
+            if constexpr (REST) {
+              const float2 f = unpack_half(whole_p);
+              pr[h][kb] = transpose_8x8(pack_half(pv[h][kb][0] - f.x, pv[h][kb][1] - f.y));
+            }
           }
+      };
+      // A word of V of each of a lane's four keys, as the MMA's operands: columns 2e and 2e + 1 from b0[2e], b0[2e + 1], b1[2e], b1[2e + 1].
+      auto unpack_v = [](uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&b0)[4], uint32_t (&b1)[4]) {
+        kv8_word_to_half<INT8>(__byte_perm(w0, w1, 0x5140), b0[0], b0[1]);
+        kv8_word_to_half<INT8>(__byte_perm(w0, w1, 0x7362), b0[2], b0[3]);
+        kv8_word_to_half<INT8>(__byte_perm(w2, w3, 0x5140), b1[0], b1[1]);
+        kv8_word_to_half<INT8>(__byte_perm(w2, w3, 0x7362), b1[2], b1[3]);
+      };
+      auto v_word = [&](int s, int w) {                  // word w of key 2t, 2t + 1, 2t + 8, 2t + 9
+        const int r = 2 * t + (s & 1) + 8 * (s >> 1);
+        const uint32_t at = D == 128 ? v_offset<D>(r, g) : v_offset<D>(r, g >> 1) + (uint32_t)((g & 1) * 8);
+        uint32_t v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(st + TILE + at + 4u * (uint32_t)w));
+        return INT8 ? v : v & ~__vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);      // (a NaN is seen to below)
+      };
+      if (__builtin_expect(far, 0)) {
+        pack_p();
+        const float apart = vs / v_ref;
+#pragma unroll
+        for (int w = 0; w < NE / 4; ++w) {
+          uint32_t b0[4], b1[4];
+          unpack_v(v_word(0, w), v_word(1, w), v_word(2, w), v_word(3, w), b0, b1);
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+              float n[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_16816<false>(n, b0[e], b0[e + 1], b1[e], b1[e + 1], pa[h][0], pa[h][1]);
+              if constexpr (REST) mma_16816<false>(n, b0[e], b0[e + 1], b1[e], b1[e + 1], pr[h][0], pr[h][1]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (key0 < sees[h][c & 1]) o[2 * w + e / 2][h][c] += n[c] * apart;      // (0 * infinity is not 0)
+            }
         }
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pv[h][i >> 1][i & 1] = 0.f;
+      }
+      pack_p();
 
       // ---- O^T += V^T P^T: a lane holds d = NE g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9 ----
       uint32_t vw[4][NE / 4];
@@ -606,10 +655,7 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
 #pragma unroll
       for (int w = 0; w < NE / 4; ++w) {
         uint32_t b0[4], b1[4];
-        kv8_word_to_half<INT8>(__byte_perm(vw[0][w], vw[1][w], 0x5140), b0[0], b0[1]);
-        kv8_word_to_half<INT8>(__byte_perm(vw[0][w], vw[1][w], 0x7362), b0[2], b0[3]);
-        kv8_word_to_half<INT8>(__byte_perm(vw[2][w], vw[3][w], 0x5140), b1[0], b1[1]);
-        kv8_word_to_half<INT8>(__byte_perm(vw[2][w], vw[3][w], 0x7362), b1[2], b1[3]);
+        unpack_v(vw[0][w], vw[1][w], vw[2][w], vw[3][w], b0, b1);
 #pragma unroll
         for (int e = 0; e < 4; e += 2)
 #pragma unroll
@@ -640,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
   float* sm_l = sm_m + kWarps * ROWS;
   float* cl_o = sm_l + kWarps * ROWS;                  // [ROWS][D] and [ROWS][2]: for the cluster's merge
   float* cl_ml = cl_o + ROWS * D;
-  const float unlift = v_ref * (1.f / kLift);
+  const float unlift = v_ref * (1.f / (kLift * kHead));
 #pragma unroll
   for (int h = 0; h < G; ++h)
 #pragma unroll
@@ -684,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
       }
     }
     if (whole) {
-      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      const float inv = lsum == 0.f ? 0.f : kHead / lsum;
       *reinterpret_cast<uint2*>(p.out + out_row(r) * D + dd) = make_uint2(round_pair<BF16>(sum.x * inv, sum.y * inv), round_pair<BF16>(sum.z * inv, sum.w * inv));
     } else {
       float* po = p.cluster > 1 ? cl_o + r * D + dd : p.part_o + (slot + r) * D + dd;
@@ -721,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
           osum += po[c] * f;
         }
       }
-      p.out[out_row(r) * D + dd] = round_bits<BF16>(lsum == 0.f ? 0.f : osum / lsum);
+      p.out[out_row(r) * D + dd] = round_bits<BF16>(lsum == 0.f ? 0.f : osum / lsum * kHead);
     }
     cluster_arrive();                                  // nobody leaves while a peer may still read its partial
     cluster_wait();
@@ -834,7 +880,7 @@ __global__ void __launch_bounds__(512) attn_decode_kv8_merge_kernel(const Kv8Arg
     }
   }
   if (!on) return;
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  const float inv = lsum == 0.f ? 0.f : kHead / lsum;
   uint16_t* dst = p.out + ((int64_t)b * p.Sq * p.Hq + r) * D + lane * W;
   if constexpr (W == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(round_pair<BF16>(o[0] * inv, o[1] * inv), round_pair<BF16>(o[2] * inv, o[3] * inv));
   else *reinterpret_cast<uint32_t*>(dst) = round_pair<BF16>(o[0] * inv, o[1] * inv);
