@@ -567,14 +567,42 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           for (int c = 0; c < kLd; c += 2) acc[(kLd * k + c) / 2] = f2_fma(f2_of(r[k & 1][c], r[k & 1][c + 1]), ss, acc[(kLd * k + c) / 2]);
         }
       }
-      if (tc::warp_aborted(abort)) break;
+      // The clusters that share a tile are counted off warp by warp; the last of them finds the counter full, and sets it to zero.
+      auto counted_off = [&](int c_first, int c_last) {
+        __syncwarp();
+        int before = 0;
+        int* counter = prm.counters + ((tile - prm.whole_tiles) * 2 + (int)rank) * 8 + warp - 4;
+        if (lane == 0) {
+          before = atomicAdd(counter, 1);
+          if (before == c_last - c_first) *counter = 0;
+        }
+        return __shfl_sync(0xffffffffu, before, 0) == c_last - c_first;
+      };
+      auto shared_by = [&](int& c_first, int& c_last) {
+        const int64_t total = (int64_t)(prm.tiles_p * prm.tiles_q - prm.whole_tiles) * prm.k_blocks, u0 = (int64_t)(tile - prm.whole_tiles) * prm.k_blocks;
+        c_first = sharer_of(u0, total, prm.sharers);
+        c_last = sharer_of(u0 + prm.k_blocks - 1, total, prm.sharers);
+        return total;
+      };
+      if (tc::warp_aborted(abort)) {
+        // A wait has run out: the results are void, but the warp counts itself off all the same, here and for what is left of its share, so
+        // that the next call finds the counters at zero.
+        do {
+          if (k1 - k0 < prm.k_blocks) {
+            int c_first, c_last;
+            shared_by(c_first, c_last);
+            counted_off(c_first, c_last);
+          }
+        } while (work.next(prm, tile, k0, k1));
+        break;
+      }
       pair_tile_coords(tile, prm.tiles_p, prm.tiles_q, tp, tq);
       const int row0 = tp * 2 * kBM + (int)rank * kBM + quad * 32, x0 = tq * BN + half * kCols;
       if (k1 - k0 < prm.k_blocks) {
         // a tile of several clusters: this one's sums to the workspace, four columns of a row a store
         const int shared = tile - prm.whole_tiles;
-        const int64_t total = (int64_t)(prm.tiles_p * prm.tiles_q - prm.whole_tiles) * prm.k_blocks, u0 = (int64_t)shared * prm.k_blocks;
-        const int c_first = sharer_of(u0, total, prm.sharers), c_last = sharer_of(u0 + prm.k_blocks - 1, total, prm.sharers);
+        int c_first, c_last;
+        const int64_t total = shared_by(c_first, c_last);
         const int64_t mine = (int64_t)((int)rank * 8 + warp - 4) * (kCols * 32);
         auto slot_of = [&](int c) {                    // a cluster has two slots: for the tile that its share begins with, and the last one
           const int begins = (int)(c * total / prm.sharers / prm.k_blocks);
@@ -589,14 +617,8 @@ block_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
           __stcg(reinterpret_cast<float4*>(dst + i * 128), v);
         }
         __threadfence();
-        __syncwarp();
-        int before = 0;
-        int* counter = prm.counters + (shared * 2 + (int)rank) * 8 + warp - 4;
-        if (lane == 0) before = atomicAdd(counter, 1);
-        before = __shfl_sync(0xffffffffu, before, 0);
-        if (before < c_last - c_first) continue;       // another cluster will finish the tile
+        if (!counted_off(c_first, c_last)) continue;   // another cluster will finish the tile
         __threadfence();
-        if (lane == 0) *counter = 0;
 #pragma unroll
         for (int i = 0; i < kCols / 2; ++i) acc[i] = f2(0.f, 0.f);
         for (int c = c_first; c <= c_last; ++c) {
