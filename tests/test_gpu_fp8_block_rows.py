@@ -131,3 +131,23 @@ def test_rows_refuse():
         glue.rmsnorm_fp8_block(x, x[0], 1e-6, x[:1])
     with pytest.raises(TypeError):
         glue.rmsnorm_fp8_block(x, x[0].float(), 1e-6)
+
+
+@pytest.mark.parametrize("M,K", [(4096, 3584), (4097, 3584), (10000, 1000), (1300, 8200), (300, 32768), (600, 18944), (100000, 136)])
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_quantize_many_rows(M, K, dt):
+    """So many features that a thread takes four units of them: the bits of the same rows a few at a time, and the definition's codes."""
+    from llmqrt_b200.ops import quantize_fp8_block
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    x = (torch.randn(M, K, generator=g, device="cuda") * torch.logspace(-3, 3, M, device="cuda")[:, None]).to(DT[dt])
+    x[M // 2] = 0
+    x[M // 3, K // 2:] = float("inf")
+    x[M // 3, 0] = float("nan")
+    assert M * K // 8 >= torch.cuda.get_device_properties(0).multi_processor_count * 2048 * 4
+    q, scale = quantize_fp8_block(x)
+    rows = torch.cat([torch.arange(0, 70), torch.arange(M // 3 - 9, M // 3 + 9), torch.arange(M // 2 - 9, M // 2 + 9), torch.arange(M - 70, M)]).unique().cuda()
+    few = quantize_fp8_block(x[rows])
+    assert bits_equal(q[rows], few[0]) and bits_equal(scale[rows], few[1])
+    ok = torch.arange(M, device="cuda") != M // 3
+    for part in torch.arange(M, device="cuda")[ok].split(20_000_000 // K):
+        _check(q[part], scale[part], x[part].double(), 3)
