@@ -94,9 +94,12 @@ int llmqrt_quantize_fp8_alpha(const void* x, int x_dtype, int64_t M, int64_t K, 
 
 /* FP8 e4m3 quantization with a scale for each token and group of 128 features, x's rows 16-byte aligned, K a multiple of 8:
  * scale[m, g] = max(absmax of the group, 1e-12) / 448, q = e4m3(x * (448 / that maximum)); nothing is rounded to x's
- * type in between.  q [M, K] and scale [M, ceil(K / 128)] are contiguous. */
+ * type in between.  q [M, K] and scale [M, ceil(K / 128)] are contiguous.  K at most 32768, as in llmqrt_rmsnorm_fp8_block; _wide takes rows of
+ * up to 134 million features, which a layer's inputs may need. */
 int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale,
                               llmqrt_stream_t stream);
+int llmqrt_quantize_fp8_block_wide(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale,
+                                   llmqrt_stream_t stream);
 
 /* RMS norm whose result leaves as llmqrt_quantize_fp8_block would have it: with h = T(x + residual), written to h_out (both
  * or neither), or h = x,  y = h * weight / sqrt(mean(h^2) + eps) in fp32, quantized without a rounding to T.  Rows of x and

@@ -62,6 +62,7 @@ _PROTOS = {
     "llmqrt_attn_decode_step": (c_int, [P, I64, P, P, I64, P, P, I64, I32, P, P, I64, I64, I64, P, c_int32, P, I32,
                                         I64, I64, I64, I64, I64, F, P, P]),
     "llmqrt_quantize_fp8_block": (c_int, [P, I32, I64, I64, I64, P, P, P]),
+    "llmqrt_quantize_fp8_block_wide": (c_int, [P, I32, I64, I64, I64, P, P, P]),
     "llmqrt_rmsnorm_fp8_block": (c_int, [P, I64, P, I64, P, P, F, P, P, I32, I64, I64, P]),
     "llmqrt_plan_step": (c_int, [P, P, P, I64, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, P, P]),
     "llmqrt_release_pages": (c_int, [P, P, P, I64, P, P, I64, I64, I64, I64, P]),

@@ -385,7 +385,7 @@ FAST_FN(fp8_block) {
   const int64_t M = x2.size(0), N = w.size(0);
   Tensor out = empty(x, out_shape(x, N), x.scalar_type());
   QuantScratch s(x, M, K, M * groups);
-  check(llmqrt_quantize_fp8_block(ptr(x2), xd, M, K, row_stride(x2), s.q, s.scale, c.stream));
+  check(llmqrt_quantize_fp8_block_wide(ptr(x2), xd, M, K, row_stride(x2), s.q, s.scale, c.stream));
   check(llmqrt_fp8_linear_block(s.q, K, static_cast<const uint8_t*>(ptr(w2)), row_stride(w2), ptr(bias), bd, s.scale, static_cast<const float*>(ptr(ws)),
                                 mptr(out), xd, N, M, N, K, c.workspace(), c.stream, w2.data_ptr() == w.data_ptr() ? LLMQRT_GEMM_STATIC_WEIGHT : 0));
   gil.done();

@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kGroup = 128, kGroupUnits = kGroup / 8;
 constexpr float kE4m3Max = 448.f, kFloor = 1e-12f;
-constexpr int kMaxUnits = 4096;                        // units of eight features of a row
+constexpr int kMaxUnits = 4096;                        // units of eight features of a row that one block takes
+constexpr int64_t kMaxWide = 8 * 256 * 65535ll;       // features of a row in pieces
 template <int U> constexpr int row_threads() { return U == 1 ? 1024 : 512; }
 
 __device__ __forceinline__ float half_warp_max(float v) {
@@ -173,10 +174,10 @@ rmsnorm_fp8_block_kernel(const T* __restrict__ x, int64_t ldx, const T* __restri
   }
 }
 
-int check_rows(const char* what, const void* x, int64_t ldx, const void* q, const void* scale, int dtype, int64_t M, int64_t K) {
+int check_rows(const char* what, const void* x, int64_t ldx, const void* q, const void* scale, int dtype, int64_t M, int64_t K, int64_t most) {
   LLMQRT_REQUIRE(dtype == LLMQRT_F16 || dtype == LLMQRT_BF16, "%s: dtype must be fp16 or bf16", what);
-  LLMQRT_REQUIRE(M >= 0 && M <= 0x7fffffffll && K > 0 && K % 8 == 0 && K <= (int64_t)kMaxUnits * 8,
-                 "%s: rows must have a multiple of 8 features, at most %d (got %lld)", what, kMaxUnits * 8, (long long)K);
+  LLMQRT_REQUIRE(M >= 0 && M <= 0x7fffffffll && K > 0 && K % 8 == 0 && K <= most,
+                 "%s: rows must have a multiple of 8 features, at most %lld (got %lld)", what, (long long)most, (long long)K);
   if (M == 0) return LLMQRT_OK;
   LLMQRT_REQUIRE(x && q && scale, "%s: null pointer", what);
   LLMQRT_REQUIRE(ldx >= K && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0,
@@ -193,7 +194,13 @@ extern "C" {
 
 int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale,
                               llmqrt_stream_t stream) {
-  if (int rc = check_rows("quantize_fp8_block", x, ldx, q, scale, x_dtype, M, K)) return rc;
+  if (int rc = check_rows("quantize_fp8_block", x, ldx, q, scale, x_dtype, M, K, kMaxUnits * 8)) return rc;
+  return llmqrt_quantize_fp8_block_wide(x, x_dtype, M, K, ldx, q, scale, stream);
+}
+
+int llmqrt_quantize_fp8_block_wide(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, uint8_t* q, float* scale,
+                                   llmqrt_stream_t stream) {
+  if (int rc = check_rows("quantize_fp8_block", x, ldx, q, scale, x_dtype, M, K, kMaxWide)) return rc;
   if (M == 0) return LLMQRT_OK;
   const int groups = (int)ceil_div(K, kGroup);
   // Four units a thread once that still leaves every SM its 2048 threads.
@@ -214,7 +221,7 @@ int llmqrt_quantize_fp8_block(const void* x, int x_dtype, int64_t M, int64_t K, 
 
 int llmqrt_rmsnorm_fp8_block(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* h_out, const void* weight,
                              float eps, uint8_t* q, float* scale, int dtype, int64_t M, int64_t H, llmqrt_stream_t stream) {
-  if (int rc = check_rows("rmsnorm_fp8_block", x, ldx, q, scale, dtype, M, H)) return rc;
+  if (int rc = check_rows("rmsnorm_fp8_block", x, ldx, q, scale, dtype, M, H, kMaxUnits * 8)) return rc;
   if (M == 0) return LLMQRT_OK;
   LLMQRT_REQUIRE(weight && (reinterpret_cast<uintptr_t>(weight) & 15) == 0, "rmsnorm_fp8_block: weight must be 16-byte aligned");
   LLMQRT_REQUIRE((residual == nullptr) == (h_out == nullptr), "rmsnorm_fp8_block: residual and h_out go together");

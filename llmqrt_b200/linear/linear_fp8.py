@@ -169,7 +169,7 @@ class FP8BlockLinear(LinearBase):
     weight * its block's scale), activations quantized per token and 128 features.  The reference has scales per tensor and
     per row only (linear_fp8.py:134-313).  `weight` holds the fp8 values themselves.
 
-    forward(x) quantizes x and multiplies, two kernels and one native call; `forward_quantized` takes what
+    forward(x) quantizes x (any number of features) and multiplies, two kernels and one native call; `forward_quantized` takes what
     glue.rmsnorm_fp8_block or ops.quantize_fp8_block left."""
 
     def __init__(self, in_features, out_features, bias, dev="cuda:0", dtype=torch.bfloat16):

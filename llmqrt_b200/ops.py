@@ -65,7 +65,8 @@ def quantize_fp8_static(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 
 def quantize_fp8_block(x: torch.Tensor):
     """A scale for each token and group of 128 features (the last group may be shorter): returns (q e4m3 [M, K], scale fp32
-    [M, ceil(K / 128)]), scale = max(absmax, 1e-12) / 448 and q = e4m3(x / scale) without a rounding to x's type in between."""
+    [M, ceil(K / 128)]), scale = max(absmax, 1e-12) / 448 and q = e4m3(x / scale) without a rounding to x's type in between.
+    K a multiple of 8, at most 32768; longer rows in pieces of a multiple of 128 (`FP8BlockLinear.forward` takes them whole)."""
     return L.fast.quantize_fp8_block(x)
 
 

@@ -186,3 +186,22 @@ def test_norm_into_linear(M):
     n = h.double() / (h.double().square().mean(1, keepdim=True) + 1e-6).sqrt()
     plain = layer(n.half())                                   # normed in 64 bits, quantized by the layer: codes may round the other way
     assert (plain.double() - y.double()).norm() / y.double().norm() < 2.0 ** -4
+
+
+@pytest.mark.parametrize("K", [32768, 32784, 53248])
+@pytest.mark.parametrize("M", [1, 3, 700])
+def test_module_of_many_inputs(M, K):
+    """Layers of more inputs than one block of the quantizer takes: the codes are those of the row in pieces."""
+    from llmqrt_b200 import ops
+    from llmqrt_b200.linear import FP8BlockLinear
+    g = torch.Generator(device="cuda").manual_seed(K + M)
+    layer = FP8BlockLinear(K, 200, True, dtype=torch.float16)
+    a, w, bias, a_s, w_s = _inputs(1, 200, K, g, torch.float16)
+    for p, v in ((layer.weight, w), (layer.weight_scale, w_s), (layer.bias, bias)):
+        p.data.copy_(v)
+    x = (torch.randn(M, K + 8, generator=g, device="cuda") * 1e-3).half()[:, :K]
+    y = layer(x)
+    pieces = [ops.quantize_fp8_block(x[:, i:i + 16384]) for i in range(0, K, 16384)]
+    q, s = torch.cat([p[0].view(torch.uint8) for p in pieces], 1).view(F8), torch.cat([p[1] for p in pieces], 1)
+    assert bits_equal(layer.forward_quantized(q, s), y)
+    _check(y, q, w, bias, s, w_s)
