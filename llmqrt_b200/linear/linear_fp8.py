@@ -167,7 +167,7 @@ def quantize_blocks(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 class FP8BlockLinear(LinearBase):
     """e4m3 weights with an fp32 scale for each block of 128 x 128 (weight_scale [ceil(out / 128), ceil(in / 128)], a value is
     weight * its block's scale), activations quantized per token and 128 features.  The reference has scales per tensor and
-    per row only (linear_fp8.py:134-313).  `weight` holds the fp8 values themselves.
+    per row only (linear_fp8.py:134-313).  `weight` holds the fp8 values themselves, whatever type the module is converted to.
 
     forward(x) quantizes x (any number of features) and multiplies, two kernels and one native call; `forward_quantized` takes what
     glue.rmsnorm_fp8_block or ops.quantize_fp8_block left."""
@@ -181,6 +181,20 @@ class FP8BlockLinear(LinearBase):
         self.weight = P(torch.zeros((out_features, in_features), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn), requires_grad=False)
         self.weight_scale = P(torch.ones((-(-out_features // 128), -(-in_features // 128)), dtype=torch.float32, device=dev), requires_grad=False)
         self.bias = P(torch.zeros(out_features, dtype=dtype, device=dev), requires_grad=False) if bias else None
+
+    def _apply(self, fn, recurse=True):
+        """Moves go with the module, changes of type do not: half() or to(dtype) leave the codes and their scales what they are."""
+        kept = {id(p): whole for p, whole in ((self._parameters.get("weight"), torch.uint8), (self._parameters.get("weight_scale"), torch.int32))
+                if p is not None}
+
+        def move(t):
+            whole = kept.get(id(t))
+            if whole is None:
+                return fn(t)
+            bits = t.detach().view(whole)
+            out = fn(bits)
+            return (out if out.dtype == whole else bits.to(out.device)).view(t.dtype)
+        return super()._apply(move, recurse)
 
     @classmethod
     def from_linear(cls, module: torch.nn.Linear, w_bit=8, group_size=128, init_only=True, dtype=torch.bfloat16):

@@ -102,3 +102,26 @@ def test_fused_projections():
         fuse_linears(odd)
     gate, up, down = _layers((192, 192, 64), bias=(False, False, False))
     assert FusedGateUpMLP(gate, up, down).gate_up is None
+
+
+@pytest.mark.parametrize("change", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.float(), lambda m: m.to(torch.float16), lambda m: m.to("cpu", torch.bfloat16),
+                                    lambda m: m.type(torch.float16), lambda m: m.to("cpu"), lambda m: m.share_memory()])
+def test_conversions_keep_codes_and_scales(change):
+    """A module's conversions to other types reach the layer's bias alone."""
+    layer = _layers((200,))[0]
+    layer.weight.data.view(torch.uint8)[3, 5] = 0x7F             # (a NaN and a scale that no 16-bit type holds)
+    layer.weight_scale.data[0, 0] = 1e-9
+    w, s = layer.weight.data.view(torch.uint8).clone(), layer.weight_scale.data.clone()
+    names = [n for n, _ in layer.named_parameters()]
+    whole = change(torch.nn.Sequential(layer, torch.nn.Linear(4, 4)))
+    assert whole[0] is layer and [n for n, _ in layer.named_parameters()] == names and isinstance(layer.weight, torch.nn.Parameter)
+    assert layer.weight.dtype == F8 and torch.equal(layer.weight.data.view(torch.uint8), w) and not layer.weight.requires_grad
+    assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale.data, s)
+    assert layer.bias.dtype in (whole[1].weight.dtype, torch.float16)
+
+
+def test_layer_without_storage():
+    from llmqrt_b200.linear import FP8BlockLinear
+    layer = FP8BlockLinear(160, 130, True, dev="meta").half().to_empty(device="cpu")
+    assert layer.weight.dtype == F8 and layer.weight.shape == (130, 160) and layer.weight.device.type == "cpu"
+    assert layer.weight_scale.dtype == torch.float32 and layer.weight_scale.shape == (2, 2)

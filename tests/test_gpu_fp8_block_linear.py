@@ -205,3 +205,12 @@ def test_module_of_many_inputs(M, K):
     q, s = torch.cat([p[0].view(torch.uint8) for p in pieces], 1).view(F8), torch.cat([p[1] for p in pieces], 1)
     assert bits_equal(layer.forward_quantized(q, s), y)
     _check(y, q, w, bias, s, w_s)
+
+
+def test_module_moved_and_converted():
+    from llmqrt_b200.linear import FP8BlockLinear
+    src = torch.nn.Linear(272, 130, bias=False)
+    layer = FP8BlockLinear.from_linear(src, init_only=False, dtype=torch.float16)
+    x = torch.randn(5, 272, device="cuda").half()
+    y = layer.cuda()(x)
+    assert bits_equal(torch.nn.Sequential(layer).half()(x), y) and bits_equal(layer.bfloat16().cpu().to("cuda")(x), y)
