@@ -73,8 +73,11 @@ def _as_index(sel, size: int) -> torch.Tensor:
     return idx
 
 
-def _whole_blocks(idx: torch.Tensor, block: int, what: str) -> torch.Tensor:
-    """`idx` must consist of whole aligned runs of `block` consecutive values; returns the run numbers."""
+def _whole_blocks(idx: torch.Tensor, block: int, what: str, size: int = 0) -> torch.Tensor:
+    """`idx` must consist of whole aligned runs of `block` consecutive values; returns the run numbers.  The last run of `size` values
+    may be shorter, where the selection ends with it."""
+    if size % block and idx.numel() and int(idx[-1]) == size - 1:
+        idx = torch.cat([idx, torch.arange(size, -(-size // block) * block)])
     if idx.numel() % block:
         raise ValueError(f"{what}: selection must cover whole blocks of {block}")
     runs = idx.reshape(-1, block)
@@ -87,8 +90,8 @@ def _whole_blocks(idx: torch.Tensor, block: int, what: str) -> torch.Tensor:
 def shard_linear_state(state: dict, method: str, mode: str, sel, keep_bias: bool = True) -> dict:
     """The shard of one quantized linear layer's state dict for Megatron tensor parallelism.
 
-    method: "awq" | "sq" | "fp8_static_quant" | "fp8_dynamic_quant" (the registry keys of
-            linear.method_to_linear).
+    method: "awq" | "sq" | "fp8_static_quant" | "fp8_dynamic_quant" | "fp8_block_quant" (the registry keys
+            of linear.method_to_linear).
     mode:   "column" -- `sel` selects OUTPUT channels (q/k/v by heads, gate, up): weight rows, per-channel
             scales and bias follow;  "row" -- `sel` selects INPUT channels (o_proj, down_proj): the
             partial outputs of the ranks are summed afterwards, per-channel scales are replicated and
@@ -97,6 +100,7 @@ def shard_linear_state(state: dict, method: str, mode: str, sel, keep_bias: bool
     AWQ constraints: output channels travel in packed words of 8 columns, input channels in
     quantization groups, so selections must cover whole aligned blocks of 8 (column) or of the group
     size (row); split_points(..., unit=group_size) yields such row boundaries.
+    Block-scaled fp8: a scale serves 128 x 128 values, so selections cover whole aligned blocks of 128 (the layer's last one may be shorter).
     Per-tensor scalars (SmoothQuant per-tensor weight / input scales, FP8 per-tensor scales) are copied.
     """
     out = {}
@@ -128,6 +132,15 @@ def shard_linear_state(state: dict, method: str, mode: str, sel, keep_bias: bool
             if name in state:
                 out[name] = state[name]
         n_axis = idx if mode == "column" else None
+    elif method == "fp8_block_quant":
+        w, ws = state["weight"], state["weight_scale"]
+        size = w.shape[0 if mode == "column" else 1]
+        idx = _as_index(sel, size)
+        blocks = _whole_blocks(idx, 128, f"block-scaled fp8 {mode} shard", size)
+        codes = w.view(torch.uint8)                                                # (float8 cannot be indexed everywhere)
+        out["weight"] = (codes[idx] if mode == "column" else codes[:, idx]).contiguous().view(w.dtype)
+        out["weight_scale"] = ws[blocks] if mode == "column" else ws[:, blocks]
+        n_axis = idx if mode == "column" else None
     else:
         raise ValueError(f"unknown quantization method {method!r}")
     bias = state.get("bias")
@@ -145,7 +158,7 @@ def shard_decoder_layer(layer_state: dict, method: str, num_heads: int, num_kv_h
     output channels, o_proj / down_proj by the matching input channels.  `layer_state` maps the
     projection names ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj") to
     the state dicts of the layers; returns the same structure for this rank.  The intermediate
-    dimension is cut on multiples of the AWQ group size (or 16 for the 8-bit schemes)."""
+    dimension is cut on multiples of the AWQ group size (or 16 for the 8-bit schemes, 128 with block scales)."""
     names = prefix_map or {k: k for k in ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")}
     q_heads, kv_heads = head_assignment(num_heads, num_kv_heads, tp, rank)
     q_idx, kv_idx = rows_of_heads(q_heads, head_dim), rows_of_heads(kv_heads, head_dim)
@@ -155,8 +168,9 @@ def shard_decoder_layer(layer_state: dict, method: str, num_heads: int, num_kv_h
         unit = inter // down["scales"].shape[0]
     else:
         inter = down["qweight" if method == "sq" else "weight"].shape[1]
-        unit = 16
-    b = split_points(inter, tp, unit)
+        unit = 128 if method == "fp8_block_quant" else 16
+    b = split_points(inter, tp, unit) if method != "fp8_block_quant" else \
+        [min(x, inter) for x in split_points(-(-inter // unit) * unit, tp, unit)]
     mlp = (b[rank], b[rank + 1])
     out = {
         names["q_proj"]: shard_linear_state(layer_state[names["q_proj"]], method, "column", q_idx),

@@ -125,3 +125,52 @@ def test_layer_without_storage():
     layer = FP8BlockLinear(160, 130, True, dev="meta").half().to_empty(device="cpu")
     assert layer.weight.dtype == F8 and layer.weight.shape == (130, 160) and layer.weight.device.type == "cpu"
     assert layer.weight_scale.dtype == torch.float32 and layer.weight_scale.shape == (2, 2)
+
+
+def _dequantized(state):
+    w, s = state["weight"].float(), state["weight_scale"]
+    return w * s.repeat_interleave(128, 0)[:w.shape[0]].repeat_interleave(128, 1)[:, :w.shape[1]]
+
+
+def _state(n, k, bias, seed):
+    from llmqrt_b200.linear import FP8BlockLinear
+    g = torch.Generator().manual_seed(seed)
+    m = torch.nn.Linear(k, n, bias=bias)
+    for p in m.parameters():
+        p.data.copy_(torch.randn(p.shape, generator=g))
+    return FP8BlockLinear.from_linear(m, init_only=False, dtype=torch.float16).state_dict()
+
+
+def test_tensor_parallel_shards():
+    """Shards of a layer are the layer's own values, fit the layer class, and make up the whole."""
+    from llmqrt_b200 import tp
+    from llmqrt_b200.linear import FP8BlockLinear
+    state = _state(700, 400, True, 3)                            # (last blocks of 60 outputs and 16 inputs)
+    full = _dequantized(state)
+    cuts = [(0, 256), (256, 384), (384, 700)]
+    parts = [tp.shard_linear_state(state, "fp8_block_quant", "column", c) for c in cuts]
+    assert torch.equal(torch.cat([_dequantized(p) for p in parts]), full) and torch.equal(torch.cat([p["bias"] for p in parts]), state["bias"])
+    for p, (a, b) in zip(parts, cuts):
+        FP8BlockLinear(400, b - a, True, dev="cpu", dtype=torch.float16).load_state_dict(p)
+    cuts = [(0, 128), (128, 400)]
+    parts = [tp.shard_linear_state(state, "fp8_block_quant", "row", c, keep_bias=i == 0) for i, c in enumerate(cuts)]
+    assert torch.equal(torch.cat([_dequantized(p) for p in parts], 1), full)
+    assert torch.equal(parts[0]["bias"], state["bias"]) and not parts[1]["bias"].any()
+    picked = tp.shard_linear_state(state, "fp8_block_quant", "column", list(range(512, 640)) + list(range(0, 128)))
+    assert torch.equal(_dequantized(picked), torch.cat([full[512:640], full[:128]]))
+    for mode, sel in (("column", (0, 64)), ("column", (64, 192)), ("column", (640, 690)), ("row", (0, 200)), ("column", list(range(640, 700)) + list(range(128)))):
+        with pytest.raises(ValueError, match="128"):
+            tp.shard_linear_state(state, "fp8_block_quant", mode, sel)
+
+
+@pytest.mark.parametrize("world", [1, 2, 4])
+@pytest.mark.parametrize("inter", [1024, 1040])
+def test_tensor_parallel_decoder_layer(world, inter):
+    from llmqrt_b200 import tp
+    H, heads, kv, d = 512, 8, 4, 128
+    layer = {n: _state(o, i, b, s) for s, (n, o, i, b) in enumerate([("q_proj", heads * d, H, True), ("k_proj", kv * d, H, True), ("v_proj", kv * d, H, True),
+             ("o_proj", H, heads * d, False), ("gate_proj", inter, H, False), ("up_proj", inter, H, False), ("down_proj", H, inter, False)])}
+    ranks = [tp.shard_decoder_layer(layer, "fp8_block_quant", heads, kv, d, world, r) for r in range(world)]
+    for name, state in layer.items():
+        axis = 1 if name in ("o_proj", "down_proj") else 0
+        assert torch.equal(torch.cat([_dequantized(r[name]) for r in ranks], axis), _dequantized(state)), name
