@@ -8,8 +8,8 @@
 // once, the pages again where the first sum turns a request down -- and keeps the sums in shared memory; tokens and pages are then
 // dealt out, each finding its request by bisection.  The stack's count and the lengths may be updated in place: the last block to
 // have read them writes them.
-// On the GPU 3.8 us for 64 requests of one token (four warps, which wait for one another less than sixteen: 5.6), 5.9 us for 131072
-// tokens of 333 requests, 128 blocks (a cluster of eight, which the instructions of a token bound: 13 us), 16 us for 8192 requests.
+// On the GPU 3.5 us for 64 requests of one token (four warps, which wait for one another less than sixteen: 5.6), 5.4 us for 131072
+// tokens of 333 requests, 128 blocks (a cluster of eight, which the instructions of a token bound: 13 us), 16.5 us for 8192 requests.
 #include <algorithm>
 
 #include "common.cuh"
@@ -83,7 +83,7 @@ template <int THREADS> __device__ __forceinline__ void block_exclusive_sums(int6
   __syncthreads();                                     // (the words may be used again)
 }
 
-// EACH: neighbouring requests that a thread adds up.
+// EACH: neighbouring requests that a thread adds up; THREADS * EACH >= B.
 template <int THREADS, int EACH> __global__ void __launch_bounds__(THREADS) plan_step_kernel(PlanArgs p) {
   extern __shared__ int32_t plan_smem[];
   __shared__ longlong2 warp_sums[THREADS / 32];
@@ -96,62 +96,56 @@ template <int THREADS, int EACH> __global__ void __launch_bounds__(THREADS) plan
   __shared__ int32_t taken;
   if (threadIdx.x == 0) taken = 0;
   __syncthreads();
-  int64_t tokens = 0, wanted = 0;
-  for (int b0 = 0; b0 < p.B; b0 += THREADS * EACH) {
-    const int b1 = b0 + (int)threadIdx.x * EACH;
-    int ctx[EACH], n[EACH];
+  const int b1 = (int)threadIdx.x * EACH;
+  int ctx[EACH], n[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    ctx[j] = b1 + j < p.B ? max(p.context[b1 + j], 0) : 0;
+    n[j] = b1 + j < p.B ? max(p.fresh[b1 + j], 0) : 0;
+  }
+  // pages that a request takes; -1: more than its row of the table has
+  auto pages_of = [&](int j) {
+    const int64_t have = ((int64_t)ctx[j] + p.page - 1) >> shift, all = ((int64_t)ctx[j] + n[j] + p.page - 1) >> shift;
+    return all <= p.width ? (int)(all - have) : -1;
+  };
+  int64_t my_tokens = 0, my_pages = 0;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    my_tokens += n[j];
+    my_pages += max(pages_of(j), 0);
+  }
+  // (where no request is turned down for its tokens, the pages' sum need not wait for the tokens')
+  longlong2 before, sum;
+  block_exclusive_sums<THREADS>(my_tokens, my_pages, warp_sums, before, sum);
+  const int64_t tokens = sum.x;
+  int64_t cu = before.x, off = before.y;
+  if (tokens > p.max_tokens) {
+    my_pages = 0;
+    int64_t end = cu;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      ctx[j] = b1 + j < p.B ? max(p.context[b1 + j], 0) : 0;
-      n[j] = b1 + j < p.B ? max(p.fresh[b1 + j], 0) : 0;
+      end += n[j];
+      if (end <= p.max_tokens) my_pages += max(pages_of(j), 0);
     }
-    // pages that a request takes; -1: more than its row of the table has
-    auto pages_of = [&](int j) {
-      const int64_t have = ((int64_t)ctx[j] + p.page - 1) >> shift, all = ((int64_t)ctx[j] + n[j] + p.page - 1) >> shift;
-      return all <= p.width ? (int)(all - have) : -1;
-    };
-    int64_t my_tokens = 0, my_pages = 0;
+    longlong2 before_again, sum_again;
+    block_exclusive_sums<THREADS>(my_pages, 0, warp_sums, before_again, sum_again);
+    off = before_again.x;
+  }
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      my_tokens += n[j];
-      my_pages += max(pages_of(j), 0);
+  for (int j = 0; j < EACH; ++j) {
+    const int pages = pages_of(j);
+    bool fits = pages >= 0 && cu + n[j] <= p.max_tokens;
+    const int64_t need = fits ? pages : 0;
+    fits = fits && (need == 0 || off + need <= count);
+    // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
+    if (fits && need) atomicMax(&taken, (int32_t)(off + need));
+    if (b1 + j < p.B) {
+      cu_s[b1 + j] = (int32_t)min(cu, (int64_t)0x7fffffff);
+      ctx_s[b1 + j] = fits ? ctx[j] : ~ctx[j];
+      off_s[b1 + j] = (int32_t)min(off, (int64_t)0x7fffffff);
     }
-    // (where no request is turned down for its tokens, the pages' sum need not wait for the tokens')
-    longlong2 before, sum;
-    block_exclusive_sums<THREADS>(my_tokens, my_pages, warp_sums, before, sum);
-    int64_t cu = tokens + before.x, off = wanted + before.y, sum_pages = sum.y;
-    const bool too_many = tokens + sum.x > p.max_tokens;
-    if (too_many) {
-      my_pages = 0;
-      int64_t end = cu;
-#pragma unroll
-      for (int j = 0; j < EACH; ++j) {
-        end += n[j];
-        if (end <= p.max_tokens) my_pages += max(pages_of(j), 0);
-      }
-      longlong2 before_again, sum_again;
-      block_exclusive_sums<THREADS>(my_pages, 0, warp_sums, before_again, sum_again);
-      off = wanted + before_again.x;
-      sum_pages = sum_again.x;
-    }
-    tokens += sum.x;
-    wanted += sum_pages;
-#pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const int pages = pages_of(j);
-      bool fits = pages >= 0 && cu + n[j] <= p.max_tokens;
-      const int64_t need = fits ? pages : 0;
-      fits = fits && (need == 0 || off + need <= count);
-      // (the requests that get pages are the first ones that want any: their pages are the stack's topmost)
-      if (fits && need) atomicMax(&taken, (int32_t)(off + need));
-      if (b1 + j < p.B) {
-        cu_s[b1 + j] = (int32_t)min(cu, (int64_t)0x7fffffff);
-        ctx_s[b1 + j] = fits ? ctx[j] : ~ctx[j];
-        off_s[b1 + j] = (int32_t)min(off, (int64_t)0x7fffffff);
-      }
-      cu += n[j];
-      off += need;
-    }
+    cu += n[j];
+    off += need;
   }
   __syncthreads();
   bool last = cl == 1;
@@ -299,7 +293,8 @@ int llmqrt_plan_step(const int32_t* context, const int32_t* new_tokens, int32_t*
   PlanArgs p{context, new_tokens, block_table, table_stride, free_pages, free_count, free_left, seq_lens, cu_new, slots, positions,
              blocks > 1 ? ws_counters(workspace) + LLMQRT_WS_NUM_COUNTERS - 1 : nullptr, (int)B, (int)width, (int)pool, (int)page, (int)max_tokens};
   const int smem = (int)(3 * 4 * B), threads = few ? 128 : B <= 512 ? 512 : 1024;
-  // (8192 requests of one token: 16 us with eight a thread, 36 in eight rounds)
+  // (8192 requests of one token: 16.5 us with eight a thread, 36 in eight rounds)
+  static_assert(1024 * 8 >= kPlanMaxRequests, "one round of a block");
   auto kern = few ? plan_step_kernel<128, 1> : B <= 512 ? plan_step_kernel<512, 1> : B <= 1024 ? plan_step_kernel<1024, 1> : plan_step_kernel<1024, 8>;
   if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return rc;
   if (int rc = launch_chained(kern, dim3((unsigned)blocks), dim3((unsigned)threads), (size_t)smem, (cudaStream_t)stream, 1, p)) return rc;

@@ -99,6 +99,11 @@ def test_plan_step(B, page, top_ctx, top_new, width, pool, count, most):
     assert again[2].tolist() == slots and dev_table.tolist() == table
 
 
+@pytest.mark.parametrize("B,most", [(128, 256), (128, 257), (129, 256), (512, 1500), (513, 700), (1024, 1500), (1025, 1500), (8191, 9000), (8192, 30000)])
+def test_plan_step_at_the_borders_of_its_forms(B, most):
+    test_plan_step(B, 16, 50, 3, 8, 9000, B // 2, most)
+
+
 def test_plan_step_without_requests():
     from llmqrt_b200.paged_cache import plan_step
     e, table, count = _i32([]), torch.zeros(0, 4, dtype=torch.int32, device="cuda"), _i32([2])
