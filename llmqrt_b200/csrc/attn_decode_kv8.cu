@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, kv8_per_sm<D, ROWS>()) attn_decode_k
   // that, fp16 rounds it all the same, and most steps need no maximum over the lanes and leave O and the sums alone.
   // (kLift takes P to the upper end of fp16's range, 2^15: with a share of 2^-8 all of its bits last down to 2^-15 of the greatest P.  The
   // reference stays within 2^-50 .. 2^50: fp32 holds O at either end, whatever scales the append makes, 2^-49 .. 2^120.)
-  constexpr float kSlack = 6.f, kLift = 512.f, kNothing = -1e30f, kNear = 0x1p-8f, kRefLeast = 0x1p-50f, kRefMost = 0x1p50f;
+  constexpr float kSlack = 6.f, kLift = 512.f, kNothing = -3.4028235e38f, kNear = 0x1p-8f, kRefLeast = 0x1p-50f, kRefMost = 0x1p50f;
   float m_run[G][2], l_run[G][2], v_ref = 0.f, v_inv = 0.f;
   int sees_all = 0x7fffffff;                           // keys that every row of the tile sees
 #pragma unroll

@@ -719,3 +719,24 @@ def test_runs_on_the_current_stream():
         out = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32([600]), 608)
     torch.cuda.current_stream().wait_stream(side)
     assert rel_fro(out, _attend(q[:, None], kc, vc, ks, vs, table, [600], 608, 0.0, None, None)[:, 0]) < 2.0 ** -11 + 2.0 ** -16
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("top", [112, 9000])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_attend_scores_far_below_zero(d, top, kind):
+    """Scores of -1e31 and less: the greatest of them gets the weight all the same."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    g = _gen(19)
+    kc, vc, ks, vs = _cache(g, kind, 7, 2, 16, d)
+    codes = torch.randint(2, 16, (7, 2, 16, 1), generator=g, device="cuda").expand(7, 2, 16, d)
+    kc.copy_(-codes.float())
+    kc[4, 0, 5], kc[1, 1, 15] = -1.0, -1.0
+    ks[:] = 1e13
+    q = torch.full((1, 2, d), 1e18, device="cuda").bfloat16()
+    table = torch.full((1, -(-top // 16)), -1, dtype=torch.int32, device="cuda")
+    table[0, :7] = torch.arange(7)
+    out = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32([105]), top)
+    want = torch.stack([vc[4, 0, 5].float() * vs[4, 0], vc[1, 1, 15].float() * vs[1, 1]])
+    # (one weight of 1: the result's own rounding, 2^-8)
+    assert ((out[0].float() - want).abs() <= want.abs() * 2.0 ** -8).all()
