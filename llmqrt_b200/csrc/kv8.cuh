@@ -5,13 +5,13 @@
 
 namespace llmqrt {
 
-constexpr float kKv8Floor = 1e-12f;                    // least maximum that a scale is made for
+constexpr float kKv8Floor = 1e-12f, kKv8Most = 3.3895314e38f;      // least and greatest (bf16's) maximum that a scale is made for
 
 // The scale for values of at most `top`.  int8: top / 127.  e4m3: the least power of two that brings top within 448 -- a
 // floating-point code loses nothing by a scale up to twice as large as it could be, and requantizing by a power of two only
-// rounds where a value leaves e4m3's normal numbers.  An infinity counts as the greatest number.
+// rounds where a value leaves e4m3's normal numbers.  An infinity counts as the greatest number of bf16.
 template <bool INT8> __device__ __forceinline__ float kv8_scale(float top) {
-  top = fminf(fmaxf(top, kKv8Floor), 3.0e38f);
+  top = fminf(fmaxf(top, kKv8Floor), kKv8Most);
   if constexpr (INT8) return __fdiv_rn(top, 127.f);
   const uint32_t u = __float_as_uint(__fdiv_rn(top, 448.f));
   return __uint_as_float((u + 0x7fffffu) & 0x7f800000u);

@@ -740,3 +740,20 @@ def test_attend_scores_far_below_zero(d, top, kind):
     want = torch.stack([vc[4, 0, 5].float() * vs[4, 0], vc[1, 1, 15].float() * vs[1, 1]])
     # (one weight of 1: the result's own rounding, 2^-8)
     assert ((out[0].float() - want).abs() <= want.abs() * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_append_greatest_values(kind):
+    """bf16's greatest numbers are finite ones: within half a step of their codes."""
+    from llmqrt_b200.paged_cache import kv8_append
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.linspace(-1, 1, 64, device="cuda").mul(top).bfloat16().clamp(-top, top)[None, None]
+    kc, vc = (torch.zeros(1, 1, 16, 64, dtype=torch.int8, device="cuda").view(CACHE[kind]) for _ in range(2))
+    ks, vs = (torch.zeros(1, 1, device="cuda") for _ in range(2))
+    kv8_append(kc, vc, ks, vs, x, x, torch.tensor([0], device="cuda"))
+    want = x[0, 0].double()
+    for codes, s in ((kc, ks), (vc, vs)):
+        got = codes[0, 0, 0].float().double() * s.double()[0, 0]
+        # (half a step: 2^-4 of an e4m3 value, 1/254 of the greatest int8 one; three fp32 roundings, 2^-24 each)
+        tol = want.abs() * 2.0 ** -4 + 2.0 ** -10 * s.double() if kind == "e4m3" else torch.full_like(want, top / 254)
+        assert ((got - want).abs() <= tol + 3 * 2.0 ** -24 * top).all()
