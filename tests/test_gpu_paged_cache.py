@@ -757,3 +757,32 @@ def test_append_greatest_values(kind):
         # (half a step: 2^-4 of an e4m3 value, 1/254 of the greatest int8 one; three fp32 roundings, 2^-24 each)
         tol = want.abs() * 2.0 ** -4 + 2.0 ** -10 * s.double() if kind == "e4m3" else torch.full_like(want, top / 254)
         assert ((got - want).abs() <= tol + 3 * 2.0 ** -24 * top).all()
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,Sq,d", [([10000], 1024, 1024, 1, 64), ([14000, 30, 0], 1024, 1024, 1, 128), ([24000], 1024, 512, 4, 128),
+                                              ([12000], 1024, 64, 16, 64), ([9000, 4097], 1024, 64, 16, 128), ([30000, 5], 512, 32, 16, 64)])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_attend_shares_longer_than_a_span(lens, Hq, Hkv, Sq, d, kind, dt):
+    """So many heads that a block takes more than 4096 keys of a sequence, whose page numbers and scales it fetches again and again: each
+    row against the definition."""
+    from llmqrt_b200.paged_cache import attn_decode_kv8
+    rows = Sq * Hq // Hkv
+    columns = Hkv * (-(-rows // 16) if rows > 8 else 1)
+    # (four blocks an SM and four waves of them, the most there are: the keys of a block's share, less what beginning sequences counts)
+    blocks = 4 * 4 * torch.cuda.get_device_properties(0).multi_processor_count // columns
+    assert sum(lens) // blocks > 4096 + 640 * len(lens)
+    g = _gen(max(lens) + Hkv)
+    P = sum(-(-n // 32) for n in lens) + 1
+    kc, vc, ks, vs = _cache(g, kind, P, Hkv, 32, d)
+    table = _tables(g, lens, 32, 1000, P)
+    q = torch.randn(len(lens), Sq, Hq, d, generator=g, device="cuda").to(DT[dt])
+    out = attn_decode_kv8(q, kc, vc, ks, vs, table, _i32(lens), 32000)
+    assert torch.isfinite(out).all()
+    # the result's rounding (and bf16's P in fp16), and a warp's sums of up to 24000 / 64 steps of two roundings each, 2^-23 as tensor cores cut
+    # off: 2^-13.4 of a row at most
+    tol = (2.0 ** -11 if dt == "fp16" else 2.0 ** -8 + 2.0 ** -11) + 2.0 ** -13.4
+    for h in range(0, Hq, 128):                                  # (some heads at a time: 64 bits take room)
+        k0, k1 = h * Hkv // Hq, (h + 128) * Hkv // Hq
+        want = _attend(q[:, :, h:h + 128], kc[:, k0:k1], vc[:, k0:k1], ks[:, k0:k1], vs[:, k0:k1], table, lens, 32000, 0.0, None, None)
+        assert ((out[:, :, h:h + 128].double() - want).norm(dim=-1) <= tol * want.norm(dim=-1)).all()
