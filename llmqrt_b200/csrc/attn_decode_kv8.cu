@@ -20,12 +20,13 @@
 // Grid.  Few short sequences: clusters of up to eight blocks, which have a sequence's keys between them and merge their parts through
 // each other's shared memory.  Otherwise (blocks, Hkv * row tiles): as many blocks as fit at once, each with an equal piece of all
 // sequences' keys laid end to end, whatever their lengths; sequences that several blocks have had a part of are merged from
-// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 47.)
+// the workspace by a second kernel.  (Pieces of one length for all sequences: 64 ragged sequences took 60 to 71 us, now 48.)
 // Page numbers outside the cache and rows behind the last key are not read (zeros take their place) and get no weight.
 //
-// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 47 us (4.7 TB/s: beginning a sequence costs a
-// block 4 us, the last blocks end 6 us behind the others, the merge takes 4); one sequence of 131072 keys and two tokens 32 us
-// (4.2 TB/s; 20 us of it at 6.7); 32 sequences of up to 30000 keys and 8 KV heads 196 us (6.0 TB/s).
+// Measured, HBM at 6.5 TB/s: 64 sequences of 750 .. 6000 keys, 28 heads on 4 of 128, 48 us (4.7 TB/s: beginning a sequence costs a
+// block 4 us, the last blocks end 8 us behind the median, the merge takes 5); one sequence of 131072 keys and two tokens 32.5 us
+// (4.1 TB/s; 20 us of it at 6.7, the merge 6); 32 sequences of up to 30000 keys and 8 KV heads 185 us (6.1 TB/s).  Five sequences of up to
+// 300 keys 5.0 us.
 #include <algorithm>
 #include <map>
 #include <mutex>

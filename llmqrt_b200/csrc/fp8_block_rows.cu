@@ -13,7 +13,7 @@
 //
 // HBM-bound where rows are many, once a lane works out the factor of one of its units only and passes it on (the divisions, of all
 // of them in every lane, held the norm's schedulers at 3/4 of their rate: 37.7 us): 8191 rows of 3584 with a residual take 33 us back
-// to back and 36 among others, 6.2 and 5.7 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us of the GPU, the call 6.4 with its three
+// to back and 35 among others, 6.2 and 5.9 TB/s of 6.5 (7 bytes a feature); 64 rows take 2 us of the GPU, the call 6.5 with its three
 // allocations.  The quantizer: 4096 rows of 18944 40 us, 8192 of 3584 15.3, 5.8 TB/s (52.7 and 22 with blocks that went over the units
 // of all rows, whose places took the registers of the loads).
 #include <type_traits>

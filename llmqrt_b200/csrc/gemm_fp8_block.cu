@@ -16,7 +16,7 @@
 //   block_split_kernel  few tokens: weights are the 128-lane operand (128 rows: one row of scales), the tokens the 16 .. 128
 //                       columns, and the reduction is shared out to a cluster, whose CTAs add their sums up through
 //                       distributed shared memory in rank order.
-// Measured: 64 x 37888 x 3584 27.5 us (its bytes alone 21.5), 1 x 4864 x 896 4.9 us; 4096 x 3584 x 18944 256 us in a
+// Measured on the GPU: 64 x 37888 x 3584 28 us (its bytes alone 21.5), 1 x 4864 x 896 5.0 us; 4096 x 3584 x 18944 256 us in a
 // burst and 293 under the board's 1000 W (1.9 PFLOP/s), where gemm_tc.cu's fp8 GEMM takes 239 and 266: every K block's sums pass
 // through registers.
 // All waits are bounded as in gemm_tc.cu.
@@ -68,7 +68,7 @@ __device__ __forceinline__ void load_now(const float* p, float& v) { asm volatil
 // ---- few tokens --------------------------------------------------------------------------------------
 // TMA warp, MMA warp, and four epilogue warps for each 32 tokens: with four for all of them they bound 128 tokens, 1370 cycles a
 // K block whose weights come in 700 (37888 x 3584: 44.2 us, now 35 to 37).  Up to 64 tokens two CTAs share an SM, each with half the
-// ring and tensor memory: one's start and end lie beside the other's tiles (64 tokens 28.8, now 27.5 us; 4608 x 3584, one token: 9.3 and
+// ring and tensor memory: one's start and end lie beside the other's tiles (64 tokens 28.8, then 27.5 us; 4608 x 3584, one token: 9.3 and
 // 8.3).  What is left grows with the activations, which each tile of weight rows fetches from L2 again (one token: 24.1 us).
 template <int BN> constexpr int split_groups() { return BN <= 32 ? 1 : BN / 32; }
 template <int BN> constexpr int split_threads() { return 64 + 128 * split_groups<BN>(); }
