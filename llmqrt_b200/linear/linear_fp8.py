@@ -185,7 +185,7 @@ class FP8BlockLinear(LinearBase):
     def _apply(self, fn, recurse=True):
         """Moves go with the module, changes of type do not: half() or to(dtype) leave the codes and their scales what they are."""
         kept = {id(p): whole for p, whole in ((self._parameters.get("weight"), torch.uint8), (self._parameters.get("weight_scale"), torch.int32))
-                if p is not None}
+                if p is not None and p.element_size() == whole.itemsize}
 
         def move(t):
             whole = kept.get(id(t))

@@ -174,3 +174,12 @@ def test_tensor_parallel_decoder_layer(world, inter):
     for name, state in layer.items():
         axis = 1 if name in ("o_proj", "down_proj") else 0
         assert torch.equal(torch.cat([_dequantized(r[name]) for r in ranks], axis), _dequantized(state)), name
+
+
+def test_conversion_of_a_layer_with_other_types():
+    """Parameters that are not the layer's own types (a state dict assigned as it was) are converted like any."""
+    layer = _layers((200,))[0]
+    layer.weight_scale = torch.nn.Parameter(layer.weight_scale.data.half(), requires_grad=False)
+    layer.weight = torch.nn.Parameter(layer.weight.data.float(), requires_grad=False)
+    layer.bfloat16()
+    assert layer.weight_scale.dtype == layer.weight.dtype == torch.bfloat16 and layer.weight.shape == (200, 160)
